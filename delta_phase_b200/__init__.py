@@ -11,8 +11,13 @@ from .kernels import (
     cuda_available,
     decode_step,
     delta_phase_chunkwise_fused,
+    distill_loss,
+    distill_loss_and_grad,
+    gated_scan,
+    gated_scan_step,
     gram_matrix_cuda,
     laplace_chunkwise,
+    layer_norm,
     triton_available,
 )
 from .layers import (
@@ -47,4 +52,9 @@ __all__ = [
     "gram_matrix_cuda",
     "decode_step",
     "laplace_chunkwise",
+    "layer_norm",
+    "gated_scan",
+    "gated_scan_step",
+    "distill_loss",
+    "distill_loss_and_grad",
 ]

@@ -50,6 +50,15 @@ _SIG = {
     "dp_ffn_noalloc_max_tokens": (ctypes.c_size_t, [_I, _I]),
     "dp_ln_conv_silu": (_I, [_P, _I, _P, _P, ctypes.c_float, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "dp_ln_conv_step": (_I, [_P, _I, _P, _P, ctypes.c_float, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "dp_layernorm_fwd": (_I, [_P, _I, _P, _P, _P, ctypes.c_float, _P, _P, _I, _P, _P, ctypes.c_int64, _I, _P]),
+    "dp_layernorm_bwd_workspace_size": (ctypes.c_size_t, [ctypes.c_int64, _I]),
+    "dp_layernorm_bwd": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P, ctypes.c_int64, _I, _P,
+                              ctypes.c_size_t, _P]),
+    "dp_scan_tile": (_I, []),
+    "dp_scan_fwd": (_I, [_P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I64P, _P]),
+    "dp_scan_bwd": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I64P, _P]),
+    "dp_scan_step": (_I, [_P, _P, _P, _P, _I, _I, _P, _I, _I, _I64P, _P]),
+    "dp_distill": (_I, [_P, _I, _P, _I, _P, _I, _P, _P, ctypes.c_float, _P, _P, _I, _I, _I, _I, _I64P, _P]),
     "dp_layernorm": (_I, [_P, _I, _P, _P, _P, ctypes.c_float, _P, _P, _I, ctypes.c_int64, _I, _P]),
 }
 
@@ -418,3 +427,89 @@ def ln_conv_step(x, ln_w, ln_b, eps, conv_w, conv_b, conv_state, out):
                                    ptr(conv_b) if conv_b is not None else None, ptr(conv_state), ptr(out),
                                    dtype_code(out), B, d, k, stream_of(dev))
     _check("dp_ln_conv_step", rc)
+
+
+def layernorm_fwd(x, ln_w, ln_b, eps, y, mean, rstd, residual=None, sum_out=None):
+    """dp_layernorm_fwd: s = x (+ residual, s written to sum_out); y = LayerNorm(s); the rows'
+    mean and rstd are kept for layernorm_bwd.  (rows, d) tensors, contiguous; residual, sum_out,
+    mean, rstd and the parameters float32."""
+    dev = require_cuda(x, ln_w, ln_b, y, mean, rstd, residual, sum_out)
+    rows, d = x.shape
+    with torch.cuda.device(dev):
+        rc = lib().dp_layernorm_fwd(ptr(x), dtype_code(x), ptr(residual), ptr(ln_w), ptr(ln_b), float(eps),
+                                    ptr(sum_out), ptr(y), dtype_code(y), ptr(mean), ptr(rstd), rows, d,
+                                    stream_of(dev))
+    _check("dp_layernorm_fwd", rc)
+
+
+def layernorm_bwd(s, dy, ln_w, mean, rstd, grad_sum=None, dx=None, grad_residual=None, grad_w=None, grad_b=None):
+    """dp_layernorm_bwd: the gradients asked for (tensors that are not None) of layernorm_fwd;
+    s is its sum_out, or x where there was no residual."""
+    dev = require_cuda(s, dy, ln_w, mean, rstd, grad_sum, dx, grad_residual, grad_w, grad_b)
+    rows, d = s.shape
+    ws = None
+    if grad_w is not None or grad_b is not None:
+        ws = torch.empty(max(1, int(lib().dp_layernorm_bwd_workspace_size(rows, d))), device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        rc = lib().dp_layernorm_bwd(ptr(s), dtype_code(s), ptr(dy), dtype_code(dy), ptr(ln_w), ptr(mean), ptr(rstd),
+                                    ptr(grad_sum), ptr(dx), DP_F32 if dx is None else dtype_code(dx),
+                                    ptr(grad_residual), ptr(grad_w), ptr(grad_b), rows, d, ptr(ws),
+                                    0 if ws is None else ws.numel(), stream_of(dev))
+    _check("dp_layernorm_bwd", rc)
+
+
+DP_SCAN_DECAY, DP_SCAN_SIGMOID = 0, 1
+
+
+def scan_tile():
+    """Tokens per saved state of dp_scan_fwd."""
+    return int(lib().dp_scan_tile())
+
+
+def scan_fwd(x, gate, mode, state_in, out, state_out, saved=None):
+    """dp_scan_fwd: x, gate, out (B, L, D) of one dtype with unit channel stride; states (B, D)
+    float32 contiguous; saved (B, ceil(L / scan_tile()), D) float32 contiguous or None."""
+    dev = require_cuda(x, gate, state_in, out, state_out, saved)
+    B, L, D = x.shape
+    st = strides_array((x.stride(0), x.stride(1), gate.stride(0), gate.stride(1), out.stride(0), out.stride(1)))
+    with torch.cuda.device(dev):
+        rc = lib().dp_scan_fwd(ptr(x), ptr(gate), dtype_code(x), int(mode), ptr(state_in), ptr(out), ptr(state_out),
+                               ptr(saved), B, L, D, st, stream_of(dev))
+    _check("dp_scan_fwd", rc)
+
+
+def scan_bwd(x, gate, grad_out, mode, saved, grad_state_out, grad_x, grad_gate, grad_state_in):
+    """dp_scan_bwd: grad_x, grad_gate (B, L, D) contiguous of x's dtype, grad_state_in (B, D)
+    float32 or None; saved as scan_fwd wrote it."""
+    dev = require_cuda(x, gate, grad_out, saved, grad_state_out, grad_x, grad_gate, grad_state_in)
+    B, L, D = x.shape
+    st = strides_array((x.stride(0), x.stride(1), gate.stride(0), gate.stride(1), grad_out.stride(0),
+                        grad_out.stride(1)))
+    with torch.cuda.device(dev):
+        rc = lib().dp_scan_bwd(ptr(x), ptr(gate), ptr(grad_out), dtype_code(x), int(mode), ptr(saved),
+                               ptr(grad_state_out), ptr(grad_x), ptr(grad_gate), ptr(grad_state_in), B, L, D, st,
+                               stream_of(dev))
+    _check("dp_scan_bwd", rc)
+
+
+def scan_step(state_in, state_out, x, gate, mode, out):
+    """dp_scan_step: one token; states (B, D) float32 contiguous (may be the same tensor); x,
+    gate, out (B, D) of one dtype with unit channel stride."""
+    dev = require_cuda(state_in, state_out, x, gate, out)
+    B, D = x.shape
+    with torch.cuda.device(dev):
+        rc = lib().dp_scan_step(ptr(state_in), ptr(state_out), ptr(x), ptr(gate), dtype_code(x), int(mode), ptr(out),
+                                B, D, strides_array((x.stride(0), gate.stride(0), out.stride(0))), stream_of(dev))
+    _check("dp_scan_step", rc)
+
+
+def distill(z, index, teacher, weight, grad, tau, loss=None, dz=None):
+    """dp_distill: z (B, L, V) with unit stride over V; index (int64 or int32), teacher
+    (B, L, K), weight, grad, loss (B, L) and dz (B, L, V) contiguous; loss and / or dz."""
+    dev = require_cuda(z, index, teacher, weight, grad, loss, dz)
+    B, L, V = z.shape
+    with torch.cuda.device(dev):
+        rc = lib().dp_distill(ptr(z), dtype_code(z), ptr(index), index.element_size(), ptr(teacher),
+                              dtype_code(teacher), ptr(weight), ptr(grad), float(tau), ptr(loss), ptr(dz), B, L, V,
+                              index.shape[-1], strides_array((z.stride(0), z.stride(1))), stream_of(dev))
+    _check("dp_distill", rc)

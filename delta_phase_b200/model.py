@@ -14,6 +14,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _capi
+from .kernels.distill import distill_loss_and_grad
 from .layers import ComplexBetaDeltaPhaseBlock, DeltaPhaseHolographicBlock
 
 
@@ -174,6 +175,24 @@ class DeltaPhaseModel(nn.Module):
             h, s = block._step_fresh(h, states[i], keep_fp32=True)
             new_states.append(s)
         return self._head_step(h), new_states
+
+    def distill_step(self, input_ids: torch.Tensor, teacher_index: torch.Tensor, teacher_logits: torch.Tensor,
+                     temperature: float = 1.0, weight: Optional[torch.Tensor] = None,
+                     states: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
+        """Forward and backward pass of one distillation step: logits of ``input_ids`` (B, L)
+        against the teacher's top logits ``teacher_index`` / ``teacher_logits`` (B, L, K), loss
+        and logit gradient in one pass (:func:`distill_loss_and_grad`).  ``weight`` (B, L) scales
+        each token's loss (0 for padding); None takes the mean over the tokens.  Parameter
+        gradients are accumulated as by ``loss.backward()``; returns the detached loss, summed
+        over the tokens.  There is no counterpart in the reference."""
+        if not torch.is_grad_enabled():
+            raise RuntimeError("distill_step computes gradients: call it with gradients enabled")
+        logits = self.forward(input_ids, states)
+        if weight is None:
+            weight = torch.full(input_ids.shape, 1.0 / max(1, input_ids.numel()), device=logits.device)
+        loss, grad = distill_loss_and_grad(logits, teacher_index, teacher_logits, temperature, weight)
+        logits.backward(grad)
+        return loss.sum()
 
     def print_substrate_report(self):
         print("=" * 72)

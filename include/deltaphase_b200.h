@@ -351,6 +351,99 @@ DP_API int dp_layernorm(const void *x, int x_dtype, const float *residual, const
                         const float *ln_b, float eps, float *sum_out, void *y, int y_dtype, int64_t rows,
                         int d, void *stream);
 
+/*
+ * Layer norm for training: the block's norm1, norm_retrieved and norm2
+ * (delta_phase/layers.py:177-244) with what the backward pass needs kept.
+ *   s = x (+ residual); m = mean(s); r = 1 / sqrt(mean((s - m)^2) + eps) per row;
+ *   y = (s - m) r ln_w + ln_b
+ *   x : (rows, d) of x_dtype;  residual, sum_out (= s) : (rows, d) float32, both or neither
+ *   ln_w, ln_b : (d) float32 or NULL (1 and 0);  y : (rows, d) of y_dtype
+ *   mean, rstd : (rows) float32, written
+ * All tensors contiguous; any d >= 1.  sum_out may be residual (the sum in place).
+ */
+DP_API int dp_layernorm_fwd(const void *x, int x_dtype, const float *residual, const float *ln_w,
+                        const float *ln_b, float eps, float *sum_out, void *y, int y_dtype, float *mean,
+                        float *rstd, int64_t rows, int d, void *stream);
+
+/*
+ * Backward of dp_layernorm_fwd: with n = (s - m) r and g = ln_w dy,
+ *   ds = r (g - mean(g) - n mean(g n)) + grad_sum;  grad_w = sum_rows dy n;  grad_b = sum_rows dy
+ *   s        : (rows, d) of s_dtype: sum_out, or x where there was no residual
+ *   dy       : (rows, d) of dy_dtype;  grad_sum : (rows, d) float32, the gradient that reaches
+ *              sum_out, or NULL (= 0);  mean, rstd : as the forward wrote them
+ *   dx       : (rows, d) of dx_dtype, ds rounded, or NULL;  grad_residual : (rows, d) float32,
+ *              ds, or NULL;  grad_w, grad_b : (d) float32 or NULL
+ *   workspace: dp_layernorm_bwd_workspace_size(rows, d) bytes, 16-byte aligned (not needed
+ *              when grad_w and grad_b are NULL)
+ * The sums over the rows have a fixed order: the same inputs give the same bits.
+ */
+DP_API size_t dp_layernorm_bwd_workspace_size(int64_t rows, int d);
+DP_API int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int dy_dtype, const float *ln_w,
+                        const float *mean, const float *rstd, const float *grad_sum, void *dx, int dx_dtype,
+                        float *grad_residual, float *grad_w, float *grad_b, int64_t rows, int d,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Gated linear recurrence over a sequence, per channel: h_t = a_t h_{t-1} + u_t, out_t = h_t.
+ * The vector-state counterpart of LaplacePhaseCore's per-row decay
+ * (delta_phase/layers.py:481-561).
+ *   DP_SCAN_DECAY   a = exp(gate) (gate = log a; -inf drops the state), u = x
+ *   DP_SCAN_SIGMOID a = sigmoid(gate), u = (1 - a) x
+ *   x, gate, out : (B, L, D) of `dtype`, unit channel stride, any batch and token strides
+ *   state_in     : (B, D) float32 or NULL (= 0);  state_out : (B, D) float32, not state_in
+ *   saved        : (B, ceil(L / dp_scan_tile()), D) float32, the state before each tile, for
+ *                  dp_scan_bwd; or NULL
+ *   strides[6]   : {sb, st} of x, gate, out
+ * The state is float32 throughout; the order of all sums is fixed by L.  Any L >= 0.  The
+ * kernels compute h - (1 - a) h for a h: a state that has become infinite continues as NaN.
+ */
+enum dp_scan_mode { DP_SCAN_DECAY = 0, DP_SCAN_SIGMOID = 1 };
+DP_API int dp_scan_tile(void);
+DP_API int dp_scan_fwd(const void *x, const void *gate, int dtype, int mode, const float *state_in, void *out,
+                   float *state_out, float *saved, int B, int L, int D, const int64_t *strides, void *stream);
+
+/*
+ * Backward of dp_scan_fwd: gradients of x, gate and the initial state, given grad_out
+ * (B, L, D) of `dtype` and grad_state_out (B, D) float32 or NULL (= 0).
+ *   saved             : as dp_scan_fwd wrote it for the same x, gate and state_in
+ *   grad_x, grad_gate : (B, L, D) of `dtype`, contiguous;  grad_state_in : (B, D) float32 or NULL
+ *   strides[6]        : {sb, st} of x, gate, grad_out
+ */
+DP_API int dp_scan_bwd(const void *x, const void *gate, const void *grad_out, int dtype, int mode,
+                   const float *saved, const float *grad_state_out, void *grad_x, void *grad_gate,
+                   float *grad_state_in, int B, int L, int D, const int64_t *strides, void *stream);
+
+/*
+ * One token of the recurrence: state_out = a state_in + u, out = state_out.
+ *   state_in, state_out : (B, D) float32, contiguous; may alias (in-place update)
+ *   x, gate, out        : (B, D) of `dtype`, unit channel stride;  strides[3] : sb of x, gate, out
+ */
+DP_API int dp_scan_step(const float *state_in, float *state_out, const void *x, const void *gate, int dtype,
+                    int mode, void *out, int B, int D, const int64_t *strides, void *stream);
+
+/*
+ * Distillation from a teacher's top logits: the loss, its gradient, or both in one pass over
+ * the student's logits.  Per row, with p = softmax(teacher / tau) over the row's K entries and
+ * q = softmax(z / tau) over its V logits:
+ *   loss  = weight tau^2 sum_k p_k (log p_k - log q_{index_k})
+ *   dz_v  = grad weight tau (q_v - sum_{k: index_k = v} p_k)
+ *   z       : (B, L, V) of z_dtype, unit stride over V; a row is one (b, t)
+ *   index   : (B, L, K) contiguous, int64 (index_bytes 8) or int32 (4); an entry outside
+ *             0 .. V - 1 is padding and left out; an index may occur more than once
+ *   teacher : (B, L, K) of teacher_dtype, contiguous; -inf leaves the entry out
+ *   weight  : (B, L) float32, contiguous, or NULL (= 1).  A row of weight 0 and a row without
+ *             entries have loss 0 and gradient 0, whatever z holds
+ *   grad    : (B, L) float32, contiguous, the gradient that reaches each row's loss, or NULL
+ *             (= 1); where it is 0, so is the row's gradient, whatever z holds
+ *   loss    : (B, L) float32, contiguous, or NULL
+ *   dz      : (B, L, V) of z_dtype, contiguous, not z, or NULL (loss and dz not both NULL)
+ *   strides[2] : {sb, st} of z
+ * Limits: 1 <= K <= 1024; V times the element size below 1 MiB; 1e-30 < tau < 1e30.
+ */
+DP_API int dp_distill(const void *z, int z_dtype, const void *index, int index_bytes,
+                  const void *teacher, int teacher_dtype, const float *weight, const float *grad, float tau,
+                  float *loss, void *dz, int B, int L, int V, int K, const int64_t *strides, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
