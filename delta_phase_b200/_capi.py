@@ -429,87 +429,117 @@ def ln_conv_step(x, ln_w, ln_b, eps, conv_w, conv_b, conv_state, out):
     _check("dp_ln_conv_step", rc)
 
 
-def layernorm_fwd(x, ln_w, ln_b, eps, y, mean, rstd, residual=None, sum_out=None):
-    """dp_layernorm_fwd: s = x (+ residual, s written to sum_out); y = LayerNorm(s); the rows'
-    mean and rstd are kept for layernorm_bwd.  (rows, d) tensors, contiguous; residual, sum_out,
-    mean, rstd and the parameters float32."""
-    dev = require_cuda(x, ln_w, ln_b, y, mean, rstd, residual, sum_out)
-    rows, d = x.shape
-    with torch.cuda.device(dev):
-        rc = lib().dp_layernorm_fwd(ptr(x), dtype_code(x), ptr(residual), ptr(ln_w), ptr(ln_b), float(eps),
-                                    ptr(sum_out), ptr(y), dtype_code(y), ptr(mean), ptr(rstd), rows, d,
-                                    stream_of(dev))
-    _check("dp_layernorm_fwd", rc)
+# ---- training-step operators.  Their smallest calls are bound by the host, so these wrappers
+# look up the device and the stream by index and pass plain addresses.
+def _device_index(*tensors):
+    """The CUDA device index that all given tensors share (raises as require_cuda does)."""
+    idx = None
+    for t in tensors:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i < 0:
+            raise RuntimeError("deltaphase_b200 kernels require CUDA tensors")
+        if idx is None:
+            idx = i
+        elif i != idx:
+            raise RuntimeError("all tensors must be on the same CUDA device")
+    return idx
 
 
-def layernorm_bwd(s, dy, ln_w, mean, rstd, grad_sum=None, dx=None, grad_residual=None, grad_w=None, grad_b=None):
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(name, idx, *args):
+    """Entry point ``name`` on the current stream of device ``idx``."""
+    f = getattr(_lib or lib(), name)
+    if torch._C._cuda_getDevice() == idx:
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _check(name, rc)
+
+
+_I64x2, _I64x3, _I64x6 = ctypes.c_int64 * 2, ctypes.c_int64 * 3, ctypes.c_int64 * 6
+
+
+def layernorm_fwd(x, ln_w, ln_b, eps, y, stats, residual=None, sum_out=None):
+    """dp_layernorm_fwd: s = x (+ residual, s written to sum_out); y = LayerNorm(s).  x, y,
+    residual, sum_out (..., d) contiguous; stats (2, rows) float32 takes the rows' mean and rstd
+    for layernorm_bwd; residual, sum_out and the parameters float32."""
+    idx = _device_index(x, ln_w, ln_b, y, stats, residual, sum_out)
+    d = x.shape[-1]
+    rows = x.numel() // d
+    mean = stats.data_ptr()
+    _call("dp_layernorm_fwd", idx, x.data_ptr(), dtype_code(x), _addr(residual), _addr(ln_w), _addr(ln_b), eps,
+          _addr(sum_out), y.data_ptr(), dtype_code(y), mean, mean + 4 * rows, rows, d)
+
+
+def layernorm_bwd(s, dy, ln_w, stats, grad_sum=None, dx=None, grad_residual=None, grad_w=None, grad_b=None):
     """dp_layernorm_bwd: the gradients asked for (tensors that are not None) of layernorm_fwd;
     s is its sum_out, or x where there was no residual."""
-    dev = require_cuda(s, dy, ln_w, mean, rstd, grad_sum, dx, grad_residual, grad_w, grad_b)
-    rows, d = s.shape
-    ws = None
+    idx = _device_index(s, dy, ln_w, stats, grad_sum, dx, grad_residual, grad_w, grad_b)
+    d = s.shape[-1]
+    rows = s.numel() // d
+    ws, nbytes = None, 0
     if grad_w is not None or grad_b is not None:
-        ws = torch.empty(max(1, int(lib().dp_layernorm_bwd_workspace_size(rows, d))), device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        rc = lib().dp_layernorm_bwd(ptr(s), dtype_code(s), ptr(dy), dtype_code(dy), ptr(ln_w), ptr(mean), ptr(rstd),
-                                    ptr(grad_sum), ptr(dx), DP_F32 if dx is None else dtype_code(dx),
-                                    ptr(grad_residual), ptr(grad_w), ptr(grad_b), rows, d, ptr(ws),
-                                    0 if ws is None else ws.numel(), stream_of(dev))
-    _check("dp_layernorm_bwd", rc)
+        nbytes = (_lib or lib()).dp_layernorm_bwd_workspace_size(rows, d)
+        ws = torch.empty(nbytes, device=s.device, dtype=torch.uint8)
+    mean = stats.data_ptr()
+    _call("dp_layernorm_bwd", idx, s.data_ptr(), dtype_code(s), dy.data_ptr(), dtype_code(dy), _addr(ln_w), mean,
+          mean + 4 * rows, _addr(grad_sum), _addr(dx), DP_F32 if dx is None else dtype_code(dx),
+          _addr(grad_residual), _addr(grad_w), _addr(grad_b), rows, d, _addr(ws), nbytes)
 
 
 DP_SCAN_DECAY, DP_SCAN_SIGMOID = 0, 1
+_scan_tile = None
 
 
 def scan_tile():
     """Tokens per saved state of dp_scan_fwd."""
-    return int(lib().dp_scan_tile())
+    global _scan_tile
+    if _scan_tile is None:
+        _scan_tile = int(lib().dp_scan_tile())
+    return _scan_tile
 
 
 def scan_fwd(x, gate, mode, state_in, out, state_out, saved=None):
     """dp_scan_fwd: x, gate, out (B, L, D) of one dtype with unit channel stride; states (B, D)
     float32 contiguous; saved (B, ceil(L / scan_tile()), D) float32 contiguous or None."""
-    dev = require_cuda(x, gate, state_in, out, state_out, saved)
+    idx = _device_index(x, gate, state_in, out, state_out, saved)
     B, L, D = x.shape
-    st = strides_array((x.stride(0), x.stride(1), gate.stride(0), gate.stride(1), out.stride(0), out.stride(1)))
-    with torch.cuda.device(dev):
-        rc = lib().dp_scan_fwd(ptr(x), ptr(gate), dtype_code(x), int(mode), ptr(state_in), ptr(out), ptr(state_out),
-                               ptr(saved), B, L, D, st, stream_of(dev))
-    _check("dp_scan_fwd", rc)
+    _call("dp_scan_fwd", idx, x.data_ptr(), gate.data_ptr(), dtype_code(x), mode, _addr(state_in), out.data_ptr(),
+          state_out.data_ptr(), _addr(saved), B, L, D,
+          _I64x6(*x.stride()[:2], *gate.stride()[:2], *out.stride()[:2]))
 
 
 def scan_bwd(x, gate, grad_out, mode, saved, grad_state_out, grad_x, grad_gate, grad_state_in):
     """dp_scan_bwd: grad_x, grad_gate (B, L, D) contiguous of x's dtype, grad_state_in (B, D)
     float32 or None; saved as scan_fwd wrote it."""
-    dev = require_cuda(x, gate, grad_out, saved, grad_state_out, grad_x, grad_gate, grad_state_in)
+    idx = _device_index(x, gate, grad_out, saved, grad_state_out, grad_x, grad_gate, grad_state_in)
     B, L, D = x.shape
-    st = strides_array((x.stride(0), x.stride(1), gate.stride(0), gate.stride(1), grad_out.stride(0),
-                        grad_out.stride(1)))
-    with torch.cuda.device(dev):
-        rc = lib().dp_scan_bwd(ptr(x), ptr(gate), ptr(grad_out), dtype_code(x), int(mode), ptr(saved),
-                               ptr(grad_state_out), ptr(grad_x), ptr(grad_gate), ptr(grad_state_in), B, L, D, st,
-                               stream_of(dev))
-    _check("dp_scan_bwd", rc)
+    _call("dp_scan_bwd", idx, x.data_ptr(), gate.data_ptr(), grad_out.data_ptr(), dtype_code(x), mode,
+          saved.data_ptr(), _addr(grad_state_out), grad_x.data_ptr(), grad_gate.data_ptr(), _addr(grad_state_in),
+          B, L, D, _I64x6(*x.stride()[:2], *gate.stride()[:2], *grad_out.stride()[:2]))
 
 
 def scan_step(state_in, state_out, x, gate, mode, out):
     """dp_scan_step: one token; states (B, D) float32 contiguous (may be the same tensor); x,
     gate, out (B, D) of one dtype with unit channel stride."""
-    dev = require_cuda(state_in, state_out, x, gate, out)
+    idx = _device_index(state_in, state_out, x, gate, out)
     B, D = x.shape
-    with torch.cuda.device(dev):
-        rc = lib().dp_scan_step(ptr(state_in), ptr(state_out), ptr(x), ptr(gate), dtype_code(x), int(mode), ptr(out),
-                                B, D, strides_array((x.stride(0), gate.stride(0), out.stride(0))), stream_of(dev))
-    _check("dp_scan_step", rc)
+    _call("dp_scan_step", idx, state_in.data_ptr(), state_out.data_ptr(), x.data_ptr(), gate.data_ptr(),
+          dtype_code(x), mode, out.data_ptr(), B, D, _I64x3(x.stride(0), gate.stride(0), out.stride(0)))
 
 
-def distill(z, index, teacher, weight, grad, tau, loss=None, dz=None):
-    """dp_distill: z (B, L, V) with unit stride over V; index (int64 or int32), teacher
-    (B, L, K), weight, grad, loss (B, L) and dz (B, L, V) contiguous; loss and / or dz."""
-    dev = require_cuda(z, index, teacher, weight, grad, loss, dz)
-    B, L, V = z.shape
-    with torch.cuda.device(dev):
-        rc = lib().dp_distill(ptr(z), dtype_code(z), ptr(index), index.element_size(), ptr(teacher),
-                              dtype_code(teacher), ptr(weight), ptr(grad), float(tau), ptr(loss), ptr(dz), B, L, V,
-                              index.shape[-1], strides_array((z.stride(0), z.stride(1))), stream_of(dev))
-    _check("dp_distill", rc)
+def distill(z, B, L, sb, st, index, teacher, weight, grad, tau, loss=None, dz=None):
+    """dp_distill: z read as (B, L, V) with strides sb, st and unit stride over V = its last
+    dimension; index (int64 or int32), teacher (B, L, K), weight, grad, loss (B, L) and dz
+    (B, L, V) contiguous; loss and / or dz."""
+    idx = _device_index(z, index, teacher, weight, grad, loss, dz)
+    _call("dp_distill", idx, z.data_ptr(), dtype_code(z), index.data_ptr(), index.element_size(), teacher.data_ptr(),
+          dtype_code(teacher), _addr(weight), _addr(grad), tau, _addr(loss), _addr(dz), B, L, z.shape[-1],
+          index.shape[-1], _I64x2(sb, st))

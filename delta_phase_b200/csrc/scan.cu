@@ -7,91 +7,160 @@
 //   decay: dx = p, dgate = q h_{t-1};  sigmoid: dx = d p, dgate = q d (h_{t-1} - x)
 //   and dL/dh_{-1} = q_0.
 //
-// Everything is kept in terms of the drop d, not of a: a close to 1 has lost the digits of
-// 1 - a, which is what a long memory consists of.  h - d h is one fused multiply-add, exact
-// in d, and a gate that drops the state (d = 1) leaves exactly nothing of it.
+// The recurrence runs on -d, not on a: a close to 1 has lost the digits of 1 - a, which is
+// what a long memory consists of.  h - d h is one fused multiply-add, exact in d, and a gate
+// that drops the state (d = 1) leaves exactly nothing of it.
 //
-// Layout: a lane owns the channels of one 4-byte word (two 16-bit values or one float), a
-// warp kTok consecutive tokens of its 32 words, a block kWarps warps (kTile tokens), and a
-// thread-block cluster up to 16 consecutive tiles of one sequence.  Each warp reduces its
-// tokens to an affine map h -> (1 - d) h + H, the maps are combined through shared memory
-// inside the block and through distributed shared memory inside the cluster (one cluster
-// barrier per 16 tiles), and each warp then runs the recurrence over its tokens again from
-// the exact state that reaches it: every input is read from HBM once, the order of all sums
-// is fixed.  A cluster walks over a long sequence in steps of its span.
+// Layout: a lane owns the channels of one 4-byte word (two 16-bit values, packed two-wide
+// float32 arithmetic, or one float), a warp kTok consecutive tokens of its 32 words, a block
+// kWarps warps (kTile tokens), and a thread-block cluster up to 16 consecutive tiles of one
+// sequence.  Each warp reduces its tokens to an affine map of the state, the maps are combined
+// through shared memory inside the block and through distributed shared memory inside the
+// cluster (one cluster barrier per span), and each warp then runs the recurrence over its
+// tokens again from the exact state that reaches it: every input is read from HBM once and
+// the order of all sums is fixed.  A cluster walks over a long sequence in steps of its span;
+// the next span's words are on their way to shared memory (cp.async) while one is computed.
+// Every thread copies the words it reads itself, so staging needs no barrier.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "dp_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace dp {
+
+int *device_error_ptr();
+
 namespace {
 
-constexpr int kTok = 16;               // tokens per warp
-constexpr int kWarps = 8;              // warps per block
-constexpr int kTile = kTok * kWarps;   // tokens per block; one saved state per tile
+using namespace ptx;
+
+constexpr int kTok = 16;              // tokens per warp
+constexpr int kWarps = 8;             // warps per block
+constexpr int kTile = kTok * kWarps;  // tokens per block; one saved state per tile
 constexpr int kMaxCluster = 16;
 constexpr int kThreads = kWarps * 32;
 
-// ---------------------------------------------------------------- gates
-// 1 - exp(g).  float32: the library's accurate form.  16-bit inputs: a Taylor polynomial
-// near 0 (|g| < 1/4: the first term left out is below 5e-8 of the value) and the hardware
-// exponential elsewhere (relative error below 1e-6), far below the rounding of g itself.
-template <typename T>
-__device__ __forceinline__ float drop_of_log(float g) {
-  float p = fmaf(g, 1.f / 720.f, 1.f / 120.f);
-  p = fmaf(g, p, 1.f / 24.f);
-  p = fmaf(g, p, 1.f / 6.f);
-  p = fmaf(g, p, 0.5f);
-  p = fmaf(g, p, 1.f);
-  return fabsf(g) < 0.25f ? -g * p : 1.f - __expf(g);
-}
-template <>
-__device__ __forceinline__ float drop_of_log<float>(float g) { return -expm1f(g); }
-
-// 1 - sigmoid(f) = 1 / (1 + exp(f))
-template <typename T>
-__device__ __forceinline__ float drop_of_logit(float f) { return __fdividef(1.f, 1.f + __expf(f)); }
-template <>
-__device__ __forceinline__ float drop_of_logit<float>(float f) { return 1.f / (1.f + expf(f)); }
-
-template <typename T, int MODE>
-__device__ __forceinline__ float drop_of(float g) {
-  return MODE == DP_SCAN_SIGMOID ? drop_of_logit<T>(g) : drop_of_log<T>(g);
-}
-
-// The affine map of some tokens: h -> (1 - d) h + H.
-struct Map {
-  float d, H;
-};
-__device__ __forceinline__ float apply(const Map &m, float h) { return fmaf(-m.d, h, h) + m.H; }
-
 // ---------------------------------------------------------------- words of channels
-// V channels of type T in a word (V = 2: a 16-bit pair, 4-byte aligned; V = 1: one value).
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float add_(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul_(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 fma_(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 add_(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul_(float2 a, float2 b) { return __fmul2_rn(a, b); }
+template <typename F>
+__device__ __forceinline__ F all_(float v);
+template <>
+__device__ __forceinline__ float all_<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float2 all_<float2>(float v) { return make_float2(v, v); }
+
+// V channels of type T in a 4-byte word: V = 2 for 16-bit pairs, V = 1 for a float or, where
+// pairs cannot be loaded, for one 16-bit value.
 template <typename T, int V>
-struct Word;
-template <typename T>
-struct Word<T, 1> {
-  T v;
-  __device__ __forceinline__ float get(int) const { return to_f32(v); }
-  __device__ __forceinline__ void set(int, float x) { v = from_f32<T>(x); }
+struct Lane;
+template <>
+struct Lane<float, 1> {
+  using F = float;
+  static __device__ __forceinline__ F get(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ void store(float *p, F v) { *p = v; }
 };
 template <typename T>
-struct __align__(4) Word<T, 2> {
-  T v[2];
-  __device__ __forceinline__ float get(int i) const { return to_f32(v[i]); }
-  __device__ __forceinline__ void set(int i, float x) { v[i] = from_f32<T>(x); }
+struct Lane<T, 1> {
+  using F = float;
+  static __device__ __forceinline__ F get(uint32_t w) {
+    const unsigned short h = (unsigned short)w;
+    return to_f32(*reinterpret_cast<const T *>(&h));
+  }
+  static __device__ __forceinline__ void store(T *p, F v) { *p = from_f32<T>(v); }
 };
-template <typename T, int V>
-__device__ __forceinline__ Word<T, V> word_zero() {
-  Word<T, V> w;
-#pragma unroll
-  for (int i = 0; i < V; ++i) w.set(i, 0.f);
-  return w;
+template <>
+struct Lane<__nv_bfloat16, 2> {
+  using F = float2;
+  static __device__ __forceinline__ F get(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16 *p, F v) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __float22bfloat162_rn(v);
+  }
+};
+template <>
+struct Lane<__half, 2> {
+  using F = float2;
+  static __device__ __forceinline__ F get(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+  static __device__ __forceinline__ void store(__half *p, F v) {
+    *reinterpret_cast<__half2 *>(p) = __float22half2_rn(v);
+  }
+};
+
+// ---------------------------------------------------------------- gates: -d = a - 1
+__device__ __forceinline__ float ex2_(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 ex2_(float2 x) { return make_float2(ex2_(x.x), ex2_(x.y)); }
+__device__ __forceinline__ float rcp_(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 rcp_(float2 x) { return make_float2(rcp_(x.x), rcp_(x.y)); }
+__device__ __forceinline__ float near0(float g, float a, float b) { return fabsf(g) < 0.0625f ? a : b; }
+__device__ __forceinline__ float2 near0(float2 g, float2 a, float2 b) {
+  return make_float2(near0(g.x, a.x, b.x), near0(g.y, a.y, b.y));
+}
+// 16-bit gates: exp(g) - 1 by its Taylor series g + ... + g^4/24 where |g| < 1/16 (the first
+// term left out is below 2^-22 of the value), by the hardware exponential elsewhere (its
+// error of 2^-22 against |a - 1| > 0.06: below 2^-18), far below the rounding of g itself;
+// sigmoid(f) - 1 = -1 / (1 + exp(f)) within a few 2^-22.  float32: the library's functions.
+template <typename T, int MODE, typename F>
+__device__ __forceinline__ F neg_drop(F g) {
+  if constexpr (sizeof(T) == 4) {
+    return MODE == DP_SCAN_SIGMOID ? -1.f / (1.f + expf(g)) : expm1f(g);
+  } else if constexpr (MODE == DP_SCAN_SIGMOID) {
+    return mul_(rcp_(add_(ex2_(mul_(g, all_<F>(1.4426950408889634f))), all_<F>(1.f))), all_<F>(-1.f));
+  } else {
+    F p = fma_(g, all_<F>(1.f / 24.f), all_<F>(1.f / 6.f));
+    p = fma_(p, g, all_<F>(0.5f));
+    p = fma_(p, g, all_<F>(1.f));
+    const F e = ex2_(mul_(g, all_<F>(1.4426950408889634f)));
+    return near0(g, mul_(g, p), add_(e, all_<F>(-1.f)));
+  }
+}
+
+// h' = h - d h + u from n = -d; u = x or d x
+template <int MODE, typename F>
+__device__ __forceinline__ F step_(F n, F h, F x) {
+  if constexpr (MODE == DP_SCAN_SIGMOID)
+    return fma_(n, fma_(x, all_<F>(-1.f), h), h);  // h - d (h - x)
+  else
+    return add_(fma_(n, h, h), x);
+}
+
+// ---------------------------------------------------------------- affine maps of the state
+// What some tokens do to the state: h -> a h + H.  16-bit inputs keep a itself (kTok factors,
+// each rounded once: far below the outputs' rounding).  float32 keeps n = a - 1 like the
+// tokens do; a dropped state (n = -1) then stays dropped by a test, not by rounding.
+template <bool EXACT, typename F>
+struct __align__(2 * sizeof(F)) Map {
+  F a, H;
+};
+template <bool EXACT, typename F>
+__device__ __forceinline__ F apply(const Map<EXACT, F> &m, F h) {
+  return EXACT ? add_(fma_(m.a, h, h), m.H) : fma_(m.a, h, m.H);
+}
+template <bool EXACT, typename F>
+__device__ __forceinline__ F compose(F r, F w) {  // first r, then w
+  if constexpr (EXACT)
+    return r == -1.f || w == -1.f ? -1.f : fmaf(w, r, r) + w;
+  else
+    return mul_(w, r);
 }
 
 struct ScanArgs {
@@ -102,291 +171,361 @@ struct ScanArgs {
   void *out, *dx, *dgate;
   const float *dhL;             // (B, D) or null
   float *dh0;                   // (B, D) or null
-  int64_t xs[2], gs[2], os[2];  // strides of x, gate and of out (forward) or dout (backward)
+  int64_t xb, gb, ob;  // batch strides of x, gate and of out (forward) or dout (backward), elements
+  int xt, gt, ot;      // their token strides, bytes
   int B, L, D, tiles_c, cs;
+  int *err;  // device error word
 };
 
-// Shared memory of another block may be written only once that block runs.
-__device__ __forceinline__ void scan_start(int cs) {
-  if (cs > 1) cg::this_cluster().sync();
+// (B, D) and saved states: V consecutive floats
+__device__ __forceinline__ void load_state(const float *p, float &v) { v = *p; }
+__device__ __forceinline__ void load_state(const float *p, float2 &v) { v = make_float2(p[0], p[1]); }
+__device__ __forceinline__ void store_state(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_state(float *p, float2 v) { p[0] = v.x, p[1] = v.y; }
+
+// p + t tokens of st bytes
+template <typename T>
+__device__ __forceinline__ T *at(T *p, int64_t t, int st) {
+  using C = std::conditional_t<std::is_const_v<T>, const char, char>;
+  return reinterpret_cast<T *>(reinterpret_cast<C *>(p) + t * st);
 }
-// Every block's map has reached every block of the cluster.  The buffers alternate, so one
-// barrier per span is enough: a block that writes a buffer again has passed the barrier of
-// the span between, which every thread that read the buffer has reached.
-__device__ __forceinline__ void scan_sync(int cs) {
-  if (cs > 1)
-    cg::this_cluster().sync();
-  else
-    __syncthreads();
+// The same for a small i: one 32 x 32 -> 64 bit multiply-add.
+template <typename T>
+__device__ __forceinline__ T *token(T *p, int i, int st) {
+  using C = std::conditional_t<std::is_const_v<T>, const char, char>;
+  return reinterpret_cast<T *>(reinterpret_cast<C *>(p) + (int64_t)i * st);
 }
+
+template <int BYTES>
+__device__ __forceinline__ void copy_word(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
+// Copies the words of kTok tokens, st bytes apart, into the thread's own slots; tokens from n
+// on are zero.  p points at the first token where n > 0, else at any valid element.
+template <typename T, int V>
+__device__ __forceinline__ void stage(uint32_t *slot, const T *p, int st, int n) {
+  if constexpr (sizeof(T) * V == 4) {
+    const uint32_t s = (uint32_t)__cvta_generic_to_shared(slot);
+    if (n == kTok) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) copy_word<4>(s + i * kThreads * 4, token(p, i, st));
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kTok; ++i) {
+        if (i < n)
+          copy_word<4>(s + i * kThreads * 4, token(p, i, st));
+        else
+          copy_word<0>(s + i * kThreads * 4, p);
+      }
+    }
+  } else {
+    unsigned short w[kTok];
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) w[i] = i < n ? *reinterpret_cast<const unsigned short *>(token(p, i, st)) : 0;
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) slot[i * kThreads] = w[i];
+  }
+}
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+__device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
+
+// The exchange of the blocks' maps inside a cluster: each block sends its map to every block
+// (st.async, counted in bytes on the receiver's mbarrier) and waits for the maps of all; there
+// is no cluster-wide barrier.  The buffers alternate: a block sends a span's map after all its
+// warps have left the span before (__syncthreads), so whoever has received the maps of span s
+// may send those of span s + 1 into the buffer of span s - 1.  No message is left when a block
+// ends: it has received all that is sent to it.
+__device__ __forceinline__ void cluster_start(uint64_t *bar, int cs) {
+  if (cs == 1) return;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar[0], 1);
+    mbar_init(&bar[1], 1);
+    fence_mbar_init();
+  }
+  cg::this_cluster().sync();  // the barriers exist in every block before the first message
+}
+__device__ __forceinline__ uint32_t peer_addr(const void *p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void send(uint32_t dst, uint32_t bar, float a, float b) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];\n" ::"r"(dst),
+               "f"(a), "f"(b), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void send(uint32_t dst, uint32_t bar, float2 a, float2 b) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];\n" ::"r"(dst),
+      "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"(bar)
+      : "memory");
+}
+// Waits for the span's maps; a wait that lasts kWaitNs (it cannot, unless a block of the
+// cluster died) is recorded in the device error word and the walk goes on without waiting.
+constexpr uint64_t kWaitNs = 2000000000ull;
+__device__ __forceinline__ bool wait_maps(uint64_t *bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (globaltimer() - t0 > kWaitNs) return false;
+  }
+}
+
+// The n = -d of a thread's tokens from the staged gates; tokens past the end keep the state.
+template <typename T, int V, int MODE, typename F>
+__device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[kTok]) {
+#pragma unroll
+  for (int i = 0; i < kTok; ++i) nd[i] = neg_drop<T, MODE>(Lane<T, V>::get(slot[i * kThreads]));
+  if (n < kTok) {
+#pragma unroll
+    for (int i = 0; i < kTok; ++i)
+      if (i >= n) nd[i] = all_<F>(0.f);
+  }
+}
+
+// The map of a thread's tokens.
+template <typename T, int V, int MODE, typename F>
+__device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok]) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  Map<EXACT, F> m = {all_<F>(EXACT ? 0.f : 1.f), all_<F>(0.f)};
+#pragma unroll
+  for (int i = 0; i < kTok; ++i) {
+    m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(xw[i * kThreads]));
+    m.a = fma_(nd[i], m.a, m.a);
+    if constexpr (EXACT) m.a = add_(m.a, nd[i]);
+  }
+  if constexpr (EXACT) {
+    float least = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) least = fminf(least, nd[i]);
+    if (least == -1.f) m.a = -1.f;
+  }
+  return m;
+}
+
+template <typename F, bool EXACT, int NX>
+struct ScanShared {
+  uint32_t gate[kTok][kThreads];
+  uint32_t x[NX][2][kTok][kThreads];        // x, and dout in the backward pass
+  Map<EXACT, F> wmap[2][kWarps][32];        // the warps' maps
+  Map<EXACT, F> bmap[2][kMaxCluster][32];   // the blocks' maps
+  uint64_t bar[2];                          // one per buffer of bmap
+};
+template <typename F, bool EXACT>
+struct ScanSharedBwd : ScanShared<F, EXACT, 2> {
+  F wq[2][kWarps][32];  // H of the warps' gradient maps
+};
 
 // ---------------------------------------------------------------- forward
 template <typename T, int V, int MODE>
-__global__ void __launch_bounds__(kThreads) scan_fwd_kernel(ScanArgs a) {
-  constexpr int C = 32 * V;
-  __shared__ Map wmap[2][kWarps][C];
-  __shared__ Map bmap[2][kMaxCluster][C];
+__global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanArgs a) {
+  using F = typename Lane<T, V>::F;
+  constexpr bool EXACT = sizeof(T) == 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto &sh = *reinterpret_cast<ScanShared<F, EXACT, 1> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
-  const int b = chain / a.tiles_c, c0 = (chain % a.tiles_c) * C;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = c0 + lane * V;
+  const int b = chain / a.tiles_c, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = (chain % a.tiles_c) * 32 * V + lane * V, cc = min(c, a.D - V);
   const bool on = c < a.D;  // D is a multiple of V
-  const T *x = static_cast<const T *>(a.x) + b * a.xs[0] + c;
-  const T *gate = static_cast<const T *>(a.gate) + b * a.gs[0] + c;
-  T *out = static_cast<T *>(a.out) + b * a.os[0] + c;
-  float h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = on && a.h0 ? a.h0[(int64_t)b * a.D + c + v] : 0.f;
+  const T *x = static_cast<const T *>(a.x) + b * a.xb + cc;
+  const T *gate = static_cast<const T *>(a.gate) + b * a.gb + cc;
+  T *out = static_cast<T *>(a.out) + b * a.ob + cc;
   const int span = a.cs * kTile, tiles = (a.L + kTile - 1) / kTile;
-  scan_start(a.cs);
-  int buf = 0;
-  for (int64_t base = 0; base < a.L; base += span, buf ^= 1) {
-    const int64_t tile0 = base + rank * kTile, t0 = tile0 + warp * kTok;
-    const int n = (int)min((int64_t)kTok, max((int64_t)0, (int64_t)a.L - t0));
-    Word<T, V> xw[kTok], gw[kTok];
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (on && i < n) {
-        xw[i] = *reinterpret_cast<const Word<T, V> *>(x + (t0 + i) * a.xs[1]);
-        gw[i] = *reinterpret_cast<const Word<T, V> *>(gate + (t0 + i) * a.gs[1]);
-      }
-    }
-    float d[kTok][V];
-    Map m[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) m[v] = {0.f, 0.f};
-    float dmax[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) dmax[v] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (!(on && i < n)) xw[i] = word_zero<T, V>();
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        d[i][v] = on && i < n ? drop_of<T, MODE>(gw[i].get(v)) : 0.f;
-        const float xv = xw[i].get(v), u = MODE == DP_SCAN_SIGMOID ? d[i][v] * xv : xv;
-        m[v].H = fmaf(-d[i][v], m[v].H, m[v].H) + u;
-        m[v].d = fmaf(-d[i][v], m[v].d, m[v].d) + d[i][v];
-        dmax[v] = fmaxf(dmax[v], d[i][v]);
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (dmax[v] == 1.f) m[v].d = 1.f;  // a dropped state stays dropped: no rounding brings it back
-      wmap[buf][warp][lane * V + v] = m[v];
-    }
+  const int off = rank * kTile + warp * kTok;
+  auto fetch = [&](int64_t base, int buf) {
+    const int64_t t0 = min(base + off, (int64_t)a.L - 1);  // byte offsets from here in 64 bits
+    const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off)));
+    stage<T, V>(&sh.gate[0][threadIdx.x], at(gate, t0, a.gt), a.gt, n);
+    stage<T, V>(&sh.x[0][buf][0][threadIdx.x], at(x, t0, a.xt), a.xt, n);
+    stage_commit();
+  };
+  fetch(0, 0);
+  F h = all_<F>(0.f);
+  if (on && a.h0) load_state(a.h0 + (int64_t)b * a.D + c, h);
+  cluster_start(sh.bar, a.cs);
+  int buf = 0, phase = 0;
+  bool alive = true;
+  for (int64_t base = 0; base < a.L; base += span, buf ^= 1, ++phase) {
+    const int64_t t0 = base + off;
+    const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - t0));
+    const uint32_t *xw = &sh.x[0][buf][0][threadIdx.x];
+    F nd[kTok];
+    stage_wait();
+    load_gates<T, V, MODE>(&sh.gate[0][threadIdx.x], n, nd);
+    if (base + span < a.L) fetch(base + span, buf ^ 1);
+    sh.wmap[buf][warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
     __syncthreads();
     // the block's map, by its last warp, to every block of the cluster
     if (warp == kWarps - 1) {
+      Map<EXACT, F> r = sh.wmap[buf][0][lane];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        Map r = wmap[buf][0][lane * V + v];
-        bool drop = r.d == 1.f;
-#pragma unroll
-        for (int j = 1; j < kWarps; ++j) {
-          const Map w = wmap[buf][j][lane * V + v];
-          r.H = apply(w, r.H);
-          r.d = fmaf(-w.d, r.d, r.d) + w.d;
-          drop |= w.d == 1.f;
-        }
-        if (drop) r.d = 1.f;
-        if (a.cs > 1) {
-          for (int k = 0; k < a.cs; ++k) cg::this_cluster().map_shared_rank(&bmap[buf][rank][lane * V + v], k)[0] = r;
-        } else {
-          bmap[buf][0][lane * V + v] = r;
-        }
+      for (int j = 1; j < kWarps; ++j) {
+        const Map<EXACT, F> w = sh.wmap[buf][j][lane];
+        r.H = apply(w, r.H);
+        r.a = compose<EXACT>(r.a, w.a);
+      }
+      if (a.cs > 1) {
+        if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
+        for (int k = 0; k < a.cs; ++k)
+          send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+      } else {
+        sh.bmap[buf][0][lane] = r;
       }
     }
-    scan_sync(a.cs);
+    if (a.cs == 1)
+      __syncthreads();
+    else if (alive && !wait_maps(&sh.bar[buf], phase >> 1 & 1))
+      alive = false;
     // the state that reaches this block, this warp, and the next span
-    float in[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) in[v] = h[v];
-    for (int k = 0; k < a.cs; ++k)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (k == rank) in[v] = h[v];
-        h[v] = apply(bmap[buf][k][lane * V + v], h[v]);
-      }
-    if (warp == 0 && a.saved && on && tile0 < a.L)
-#pragma unroll
-      for (int v = 0; v < V; ++v) a.saved[((int64_t)b * tiles + tile0 / kTile) * a.D + c + v] = in[v];
-    for (int j = 0; j < warp; ++j)
-#pragma unroll
-      for (int v = 0; v < V; ++v) in[v] = apply(wmap[buf][j][lane * V + v], in[v]);
+    F in = h;
+    for (int k = 0; k < a.cs; ++k) {
+      if (k == rank) in = h;
+      h = apply(sh.bmap[buf][k][lane], h);
+    }
+    if (warp == 0 && a.saved && on && n > 0)
+      store_state(a.saved + ((int64_t)b * tiles + t0 / kTile) * a.D + c, in);
+    for (int j = 0; j < warp; ++j) in = apply(sh.wmap[buf][j][lane], in);
+    const int lim = on ? n : 0;
+    T *o = at(out, t0, a.ot);
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      Word<T, V> o;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float xv = xw[i].get(v), u = MODE == DP_SCAN_SIGMOID ? d[i][v] * xv : xv;
-        in[v] = fmaf(-d[i][v], in[v], in[v]) + u;
-        o.set(v, in[v]);
-      }
-      if (on && i < n) *reinterpret_cast<Word<T, V> *>(out + (t0 + i) * a.os[1]) = o;
+      in = step_<MODE>(nd[i], in, Lane<T, V>::get(xw[i * kThreads]));
+      if (i < lim) Lane<T, V>::store(token(o, i, a.ot), in);
     }
   }
-  if (on && rank == 0 && warp == 0)
-#pragma unroll
-    for (int v = 0; v < V; ++v) a.hL[(int64_t)b * a.D + c + v] = h[v];
+  if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
+  if (on && rank == 0 && warp == 0) store_state(a.hL + (int64_t)b * a.D + c, h);
 }
 
 // ---------------------------------------------------------------- backward
 // The same walk from the end of the sequence.  The states before each token come from the
-// saved state of the tile and the forward maps of the warps before; the gradient q that
-// flows to earlier tokens is an affine map too (h -> (1 - d) h + Q with the same d).
-struct Map3 {
-  float d, H, Q;
-};
-
+// saved state of the tile and the maps of the warps before; the gradient q that flows to
+// earlier tokens follows an affine map too, q -> a q + Q with the same a.
 template <typename T, int V, int MODE>
-__global__ void __launch_bounds__(kThreads) scan_bwd_kernel(ScanArgs a) {
-  constexpr int C = 32 * V;
-  __shared__ Map3 wmap[2][kWarps][C];
-  __shared__ Map bmap[2][kMaxCluster][C];
+__global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const ScanArgs a) {
+  using F = typename Lane<T, V>::F;
+  constexpr bool EXACT = sizeof(T) == 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto &sh = *reinterpret_cast<ScanSharedBwd<F, EXACT> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
-  const int b = chain / a.tiles_c, c0 = (chain % a.tiles_c) * C;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = c0 + lane * V;
+  const int b = chain / a.tiles_c, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = (chain % a.tiles_c) * 32 * V + lane * V, cc = min(c, a.D - V);
   const bool on = c < a.D;
-  const T *x = static_cast<const T *>(a.x) + b * a.xs[0] + c;
-  const T *gate = static_cast<const T *>(a.gate) + b * a.gs[0] + c;
-  const T *dout = static_cast<const T *>(a.dout) + b * a.os[0] + c;
-  T *dx = static_cast<T *>(a.dx) + (int64_t)b * a.L * a.D + c;
-  T *dg = static_cast<T *>(a.dgate) + (int64_t)b * a.L * a.D + c;
-  float q[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) q[v] = on && a.dhL ? a.dhL[(int64_t)b * a.D + c + v] : 0.f;
+  const T *x = static_cast<const T *>(a.x) + b * a.xb + cc;
+  const T *gate = static_cast<const T *>(a.gate) + b * a.gb + cc;
+  const T *dout = static_cast<const T *>(a.dout) + b * a.ob + cc;
+  T *dx = static_cast<T *>(a.dx) + (int64_t)b * a.L * a.D + cc;
+  T *dg = static_cast<T *>(a.dgate) + (int64_t)b * a.L * a.D + cc;
   const int span = a.cs * kTile, tiles = (a.L + kTile - 1) / kTile;
-  scan_start(a.cs);
-  int buf = 0;
-  for (int64_t base = ((int64_t)(a.L - 1) / span) * span; base >= 0; base -= span, buf ^= 1) {
-    const int64_t tile0 = base + rank * kTile, t0 = tile0 + warp * kTok;
-    const int n = (int)min((int64_t)kTok, max((int64_t)0, (int64_t)a.L - t0));
-    Word<T, V> xw[kTok], gw[kTok], yw[kTok];
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (on && i < n) {
-        xw[i] = *reinterpret_cast<const Word<T, V> *>(x + (t0 + i) * a.xs[1]);
-        gw[i] = *reinterpret_cast<const Word<T, V> *>(gate + (t0 + i) * a.gs[1]);
-        yw[i] = *reinterpret_cast<const Word<T, V> *>(dout + (t0 + i) * a.os[1]);
-      }
-    }
-    float in[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      in[v] = on && tile0 < a.L ? a.saved[((int64_t)b * tiles + tile0 / kTile) * a.D + c + v] : 0.f;
-    float d[kTok][V];
-    Map3 m[V];
-    float dmax[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      m[v] = {0.f, 0.f, 0.f};
-      dmax[v] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (!(on && i < n)) {
-        xw[i] = word_zero<T, V>();
-        yw[i] = word_zero<T, V>();
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        d[i][v] = on && i < n ? drop_of<T, MODE>(gw[i].get(v)) : 0.f;
-        const float xv = xw[i].get(v), u = MODE == DP_SCAN_SIGMOID ? d[i][v] * xv : xv;
-        m[v].H = fmaf(-d[i][v], m[v].H, m[v].H) + u;
-        m[v].d = fmaf(-d[i][v], m[v].d, m[v].d) + d[i][v];
-        dmax[v] = fmaxf(dmax[v], d[i][v]);
-      }
-    }
-#pragma unroll
-    for (int i = kTok - 1; i >= 0; --i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float p = yw[i].get(v) + m[v].Q;
-        m[v].Q = fmaf(-d[i][v], p, p);
-      }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (dmax[v] == 1.f) m[v].d = 1.f;
-      wmap[buf][warp][lane * V + v] = m[v];
-    }
-    __syncthreads();
-    if (warp == 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        Map r = {0.f, 0.f};
-        bool drop = false;
-#pragma unroll
-        for (int j = kWarps - 1; j >= 0; --j) {
-          const Map3 w = wmap[buf][j][lane * V + v];
-          r.H = apply({w.d, w.Q}, r.H);
-          r.d = fmaf(-w.d, r.d, r.d) + w.d;
-          drop |= w.d == 1.f;
-        }
-        if (drop) r.d = 1.f;
-        if (a.cs > 1) {
-          for (int k = 0; k < a.cs; ++k) cg::this_cluster().map_shared_rank(&bmap[buf][rank][lane * V + v], k)[0] = r;
-        } else {
-          bmap[buf][0][lane * V + v] = r;
-        }
-      }
-    }
-    scan_sync(a.cs);
-    float qi[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) qi[v] = q[v];
-    for (int k = a.cs - 1; k >= 0; --k)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (k == rank) qi[v] = q[v];
-        q[v] = apply(bmap[buf][k][lane * V + v], q[v]);
-      }
-    for (int j = kWarps - 1; j > warp; --j)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const Map3 w = wmap[buf][j][lane * V + v];
-        qi[v] = apply({w.d, w.Q}, qi[v]);
-      }
-    for (int j = 0; j < warp; ++j)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const Map3 w = wmap[buf][j][lane * V + v];
-        in[v] = apply({w.d, w.H}, in[v]);
-      }
-    float hb[kTok][V];  // the state before each token
-#pragma unroll
-    for (int i = 0; i < kTok; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        hb[i][v] = in[v];
-        const float xv = xw[i].get(v), u = MODE == DP_SCAN_SIGMOID ? d[i][v] * xv : xv;
-        in[v] = fmaf(-d[i][v], in[v], in[v]) + u;
-      }
+  const int off = rank * kTile + warp * kTok;
+  auto fetch = [&](int64_t base, int buf) {
+    const int64_t t0 = min(base + off, (int64_t)a.L - 1);  // byte offsets from here in 64 bits
+    const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off)));
+    stage<T, V>(&sh.gate[0][threadIdx.x], at(gate, t0, a.gt), a.gt, n);
+    stage<T, V>(&sh.x[0][buf][0][threadIdx.x], at(x, t0, a.xt), a.xt, n);
+    stage<T, V>(&sh.x[1][buf][0][threadIdx.x], at(dout, t0, a.ot), a.ot, n);
+    stage_commit();
+  };
+  const int64_t last = (int64_t)(a.L - 1) / span * span;
+  fetch(last, 0);
+  F q = all_<F>(0.f);
+  if (on && a.dhL) load_state(a.dhL + (int64_t)b * a.D + c, q);
+  cluster_start(sh.bar, a.cs);
+  int buf = 0, phase = 0;
+  bool alive = true;
+  for (int64_t base = last; base >= 0; base -= span, buf ^= 1, ++phase) {
+    const int64_t t0 = base + off;
+    const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - t0));
+    const uint32_t *xw = &sh.x[0][buf][0][threadIdx.x], *yw = &sh.x[1][buf][0][threadIdx.x];
+    F in = all_<F>(0.f);
+    if (on && base + rank * kTile < a.L)
+      load_state(a.saved + ((int64_t)b * tiles + base / kTile + rank) * a.D + c, in);
+    F nd[kTok];
+    stage_wait();
+    load_gates<T, V, MODE>(&sh.gate[0][threadIdx.x], n, nd);
+    if (base > 0) fetch(base - span, buf ^ 1);
+    sh.wmap[buf][warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
+    F Q = all_<F>(0.f);
 #pragma unroll
     for (int i = kTok - 1; i >= 0; --i) {
-      Word<T, V> ox, og;
+      Q = add_(Q, Lane<T, V>::get(yw[i * kThreads]));
+      Q = fma_(nd[i], Q, Q);
+    }
+    sh.wq[buf][warp][lane] = Q;
+    __syncthreads();
+    if (warp == 0) {
+      Map<EXACT, F> r = {sh.wmap[buf][kWarps - 1][lane].a, sh.wq[buf][kWarps - 1][lane]};
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float p = yw[i].get(v) + qi[v];
-        qi[v] = fmaf(-d[i][v], p, p);
-        if (MODE == DP_SCAN_SIGMOID) {
-          ox.set(v, p * d[i][v]);
-          og.set(v, qi[v] * d[i][v] * (hb[i][v] - xw[i].get(v)));
-        } else {
-          ox.set(v, p);
-          og.set(v, qi[v] * hb[i][v]);
-        }
+      for (int j = kWarps - 2; j >= 0; --j) {
+        const Map<EXACT, F> w = {sh.wmap[buf][j][lane].a, sh.wq[buf][j][lane]};
+        r.H = apply(w, r.H);
+        r.a = compose<EXACT>(r.a, w.a);
       }
-      if (on && i < n) {
-        *reinterpret_cast<Word<T, V> *>(dx + (t0 + i) * a.D) = ox;
-        *reinterpret_cast<Word<T, V> *>(dg + (t0 + i) * a.D) = og;
+      if (a.cs > 1) {
+        if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
+        for (int k = 0; k < a.cs; ++k)
+          send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+      } else {
+        sh.bmap[buf][0][lane] = r;
+      }
+    }
+    if (a.cs == 1)
+      __syncthreads();
+    else if (alive && !wait_maps(&sh.bar[buf], phase >> 1 & 1))
+      alive = false;
+    F qi = q;
+    for (int k = a.cs - 1; k >= 0; --k) {
+      if (k == rank) qi = q;
+      q = apply(sh.bmap[buf][k][lane], q);
+    }
+    for (int j = kWarps - 1; j > warp; --j)
+      qi = apply(Map<EXACT, F>{sh.wmap[buf][j][lane].a, sh.wq[buf][j][lane]}, qi);
+    for (int j = 0; j < warp; ++j) in = apply(sh.wmap[buf][j][lane], in);
+    // backwards over the tokens; the states before them are run forwards again, half of the
+    // tokens at a time (registers)
+    constexpr int kHalf = kTok / 2;
+    const int lim = on ? n : 0, st = a.D * (int)sizeof(T);
+    T *px = at(dx, t0, st), *pg = at(dg, t0, st);
+    F mid = in;
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) mid = step_<MODE>(nd[i], mid, Lane<T, V>::get(xw[i * kThreads]));
+#pragma unroll
+    for (int half = 1; half >= 0; --half) {
+      F hb[kHalf];  // the state before each token
+      hb[0] = half ? mid : in;
+#pragma unroll
+      for (int i = 1; i < kHalf; ++i)
+        hb[i] = step_<MODE>(nd[half * kHalf + i - 1], hb[i - 1],
+                            Lane<T, V>::get(xw[(half * kHalf + i - 1) * kThreads]));
+#pragma unroll
+      for (int k = kHalf - 1; k >= 0; --k) {
+        const int i = half * kHalf + k;
+        const F p = add_(qi, Lane<T, V>::get(yw[i * kThreads]));
+        qi = fma_(nd[i], p, p);
+        F ox = p, og = mul_(qi, hb[k]);
+        if constexpr (MODE == DP_SCAN_SIGMOID) {
+          const F d = mul_(nd[i], all_<F>(-1.f));
+          ox = mul_(p, d);
+          og = mul_(mul_(qi, d), fma_(Lane<T, V>::get(xw[i * kThreads]), all_<F>(-1.f), hb[k]));
+        }
+        if (i < lim) {
+          Lane<T, V>::store(token(px, i, st), ox);
+          Lane<T, V>::store(token(pg, i, st), og);
+        }
       }
     }
   }
-  if (on && rank == 0 && warp == 0 && a.dh0)
-#pragma unroll
-    for (int v = 0; v < V; ++v) a.dh0[(int64_t)b * a.D + c + v] = q[v];
+  if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
+  if (on && rank == 0 && warp == 0 && a.dh0) store_state(a.dh0 + (int64_t)b * a.D + c, q);
 }
 
 // ---------------------------------------------------------------- one token
@@ -400,38 +539,48 @@ scan_step_kernel(const float *state, float *state_out, const T *x, const T *gate
   if (i >= n) return;
   const int64_t b = i / D;
   const int c = (int)(i - b * D);
-  const float d = drop_of<float, MODE>(to_f32(gate[b * gs + c])), xv = to_f32(x[b * xs + c]);
-  const float h = state[i];
-  const float r = fmaf(-d, h, h) + (MODE == DP_SCAN_SIGMOID ? d * xv : xv);
+  const float nd = neg_drop<float, MODE>(to_f32(gate[b * gs + c])), xv = to_f32(x[b * xs + c]);
+  const float r = step_<MODE>(nd, state[i], xv);
   state_out[i] = r;
   out[b * os + c] = from_f32<T>(r);
 }
 
-// Blocks of a cluster: as many tiles as the sequence has, up to 16.
-int scan_cluster(int L) {
+// Blocks of a cluster.  Smaller clusters wait less for one another, but a sequence's chain of
+// spans has to be split until about 1.7 blocks an SM run.  Measured (us forward, backward at
+// 2 / 4 / 8 / 16 blocks): 32 chains x 32768 tokens bf16 312, 443 / 168, 240 / 144, 217 /
+// 164, 265; 128 chains x 8192 tokens 129, 201 / 129, 213 / 134, 220 / 152, 261; 4 chains x
+// 65536 tokens 583, 842 / 308, 437 / 164, 232 / 95, 131.
+int scan_cluster(int L, int64_t chains) {
   int cs = 1;
-  while (cs < kMaxCluster && cs * kTile < L) cs *= 2;
+  while (cs < kMaxCluster && cs * kTile < L && chains * cs < 256) cs *= 2;
   return cs;
 }
 
-template <typename Kern>
-int scan_launch(Kern kern, const ScanArgs &a, cudaStream_t st, const char *what) {
-  if (a.cs > 8) {  // a non-portable size: opt in
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return set_error(DP_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+template <void (*KERN)(const ScanArgs), size_t SMEM>
+int scan_launch(const ScanArgs &a, cudaStream_t st, const char *what) {
+  static thread_local bool opted[64] = {};  // shared memory and 16-block clusters: opt in once
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !opted[dev])) {
+    e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(KERN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) opted[dev] = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.tiles_c * a.cs));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.cs;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.tiles_c * a.cs));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.cs;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, KERN, a);
+  }
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(DP_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
@@ -439,11 +588,23 @@ int scan_launch(Kern kern, const ScanArgs &a, cudaStream_t st, const char *what)
   return check_launch(what);
 }
 
+// Fills in the strides ({sb, st} of x, gate and out or dout); false where a token stride does
+// not fit the kernels' 32 bits of bytes.
+bool scan_strides(ScanArgs &a, const int64_t *s, int size) {
+  int64_t t[3];
+  for (int i = 0; i < 3; ++i) {
+    t[i] = s[2 * i + 1] * size;
+    if (s[2 * i + 1] > (1 << 28) || s[2 * i + 1] < -(1 << 28)) return false;
+  }
+  a.xb = s[0], a.gb = s[2], a.ob = s[4], a.xt = (int)t[0], a.gt = (int)t[1], a.ot = (int)t[2];
+  return a.D <= 1 << 28;
+}
+
 // Channel pairs of 16-bit values can be moved as 4-byte words.
 template <typename... P>
-bool scan_pairs(int D, const int64_t *s, int ns, P... ptrs) {
+bool scan_pairs(int D, const int64_t *s, P... ptrs) {
   if (D % 2) return false;
-  for (int i = 0; i < ns; ++i)
+  for (int i = 0; i < 6; ++i)
     if (s[i] % 2) return false;
   const void *ps[] = {ptrs...};
   for (const void *p : ps)
@@ -453,16 +614,22 @@ bool scan_pairs(int D, const int64_t *s, int ns, P... ptrs) {
 
 template <bool BWD, typename T, int V>
 int scan_run(ScanArgs a, int mode, cudaStream_t st, const char *what) {
+  using F = typename Lane<T, V>::F;
   a.tiles_c = (a.D + 32 * V - 1) / (32 * V);
-  a.cs = scan_cluster(a.L);
+  a.cs = scan_cluster(a.L, (int64_t)a.B * a.tiles_c);
+  a.err = device_error_ptr();
+  DP_REQUIRE(a.err, DP_ERR_CUDA, std::string(what) + ": device error word unavailable");
   DP_REQUIRE((int64_t)a.B * a.tiles_c * a.cs < (1ll << 31), DP_ERR_UNSUPPORTED,
              std::string(what) + ": too many channels");
-  if constexpr (BWD)
-    return mode == DP_SCAN_SIGMOID ? scan_launch(scan_bwd_kernel<T, V, DP_SCAN_SIGMOID>, a, st, what)
-                                   : scan_launch(scan_bwd_kernel<T, V, DP_SCAN_DECAY>, a, st, what);
-  else
-    return mode == DP_SCAN_SIGMOID ? scan_launch(scan_fwd_kernel<T, V, DP_SCAN_SIGMOID>, a, st, what)
-                                   : scan_launch(scan_fwd_kernel<T, V, DP_SCAN_DECAY>, a, st, what);
+  if constexpr (BWD) {
+    constexpr size_t kSmem = sizeof(ScanSharedBwd<F, sizeof(T) == 4>);
+    return mode == DP_SCAN_SIGMOID ? scan_launch<scan_bwd_kernel<T, V, DP_SCAN_SIGMOID>, kSmem>(a, st, what)
+                                   : scan_launch<scan_bwd_kernel<T, V, DP_SCAN_DECAY>, kSmem>(a, st, what);
+  } else {
+    constexpr size_t kSmem = sizeof(ScanShared<F, sizeof(T) == 4, 1>);
+    return mode == DP_SCAN_SIGMOID ? scan_launch<scan_fwd_kernel<T, V, DP_SCAN_SIGMOID>, kSmem>(a, st, what)
+                                   : scan_launch<scan_fwd_kernel<T, V, DP_SCAN_DECAY>, kSmem>(a, st, what);
+  }
 }
 
 template <bool BWD>
@@ -497,9 +664,9 @@ extern "C" int dp_scan_fwd(const void *x, const void *gate, int dtype, int mode,
   }
   ScanArgs a = {};
   a.x = x, a.gate = gate, a.h0 = state_in, a.hL = state_out, a.saved = saved, a.out = out;
-  for (int i = 0; i < 2; ++i) a.xs[i] = strides[i], a.gs[i] = strides[2 + i], a.os[i] = strides[4 + i];
   a.B = B, a.L = L, a.D = D;
-  return scan_dispatch<false>(a, dtype, mode, scan_pairs(D, strides, 6, x, gate, (const void *)out), st, "dp_scan_fwd");
+  DP_REQUIRE(scan_strides(a, strides, (int)dtype_size(dtype)), DP_ERR_UNSUPPORTED, "dp_scan_fwd: token stride too large");
+  return scan_dispatch<false>(a, dtype, mode, scan_pairs(D, strides, x, gate, (const void *)out), st, "dp_scan_fwd");
 }
 
 extern "C" int dp_scan_bwd(const void *x, const void *gate, const void *grad_out, int dtype, int mode,
@@ -524,10 +691,10 @@ extern "C" int dp_scan_bwd(const void *x, const void *gate, const void *grad_out
   ScanArgs a = {};
   a.x = x, a.gate = gate, a.dout = grad_out, a.saved = const_cast<float *>(saved), a.dhL = grad_state_out;
   a.dx = grad_x, a.dgate = grad_gate, a.dh0 = grad_state_in;
-  for (int i = 0; i < 2; ++i) a.xs[i] = strides[i], a.gs[i] = strides[2 + i], a.os[i] = strides[4 + i];
   a.B = B, a.L = L, a.D = D;
+  DP_REQUIRE(scan_strides(a, strides, (int)dtype_size(dtype)), DP_ERR_UNSUPPORTED, "dp_scan_bwd: token stride too large");
   return scan_dispatch<true>(a, dtype, mode,
-                             scan_pairs(D, strides, 6, x, gate, grad_out, (const void *)grad_x, (const void *)grad_gate),
+                             scan_pairs(D, strides, x, gate, grad_out, (const void *)grad_x, (const void *)grad_gate),
                              st, "dp_scan_bwd");
 }
 

@@ -15,13 +15,21 @@ from .. import _capi
 
 
 def _rows(t):
-    """(..., n) as (B, L, n): a view wherever the leading dimensions allow it."""
-    if t.dim() == 1:
-        return t.view(1, 1, -1)
-    return t.unsqueeze(0) if t.dim() == 2 else t.reshape(math.prod(t.shape[:-2]), t.shape[-2], t.shape[-1])
+    """Logits (..., V) as the kernel reads them: (tensor, B, L, sb, st) with unit stride over V;
+    in place wherever the leading dimensions are two or fewer, or can be viewed as two."""
+    if t.dim() > 3:
+        t = t.reshape(math.prod(t.shape[:-2]), t.shape[-2], t.shape[-1])
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    if t.dim() == 3:
+        return t, t.shape[0], t.shape[1], t.stride(0), t.stride(1)
+    if t.dim() == 2:
+        return t, 1, t.shape[0], 0, t.stride(0)
+    return t, 1, 1, 0, 0
 
 
-def _prepare(student_logits, teacher_index, teacher_logits, temperature, weight):
+def _check(student_logits, teacher_index, teacher_logits, temperature, weight):
+    """Refuses what the kernel does not take; returns tau and the constants as it takes them."""
     if student_logits.dim() < 1 or student_logits.shape[-1] < 1:
         raise ValueError("student_logits must be (..., V)")
     lead = student_logits.shape[:-1]
@@ -32,33 +40,28 @@ def _prepare(student_logits, teacher_index, teacher_logits, temperature, weight)
         raise TypeError("teacher_index must be int64 or int32")
     _capi.dtype_code(student_logits)
     _capi.dtype_code(teacher_logits)
-    if weight is not None and weight.shape != lead:
-        raise ValueError(f"weight must be {tuple(lead)}, got {tuple(weight.shape)}")
     if isinstance(temperature, torch.Tensor):
         raise TypeError("temperature must be a number")
     tau = float(temperature)
-    if not (tau > 0.0 and math.isfinite(tau)):
+    if not 1e-30 < tau < 1e30:
         raise ValueError("temperature must be positive and finite")
-    _capi.require_cuda(student_logits, teacher_index, teacher_logits, weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (teacher_logits, weight)):
-        raise ValueError("teacher_logits and weight are constants of the loss: detach them")
-    z = _rows(student_logits.detach())
-    if z.shape[-1] > 1 and z.stride(-1) != 1:
-        z = z.contiguous()
-    w = None if weight is None else weight.detach().to(torch.float32).contiguous()
-    return z, _rows(teacher_index).contiguous(), _rows(teacher_logits.detach()).contiguous(), tau, w
+    if weight is not None:
+        if weight.shape != lead:
+            raise ValueError(f"weight must be {tuple(lead)}, got {tuple(weight.shape)}")
+        if weight.dtype != torch.float32 or not weight.is_contiguous():
+            weight = weight.to(torch.float32).contiguous()
+    return tau, teacher_index.contiguous(), teacher_logits.contiguous(), weight
 
 
 class DistillCudaFunction(torch.autograd.Function):
-    """Autograd wrapper of dp_distill: the loss in the forward pass; the backward pass reads the
-    logits again and writes their gradient."""
+    """Autograd wrapper of dp_distill on arguments that distill_loss has checked: the loss in the
+    forward pass; the backward pass reads the logits again and writes their gradient."""
 
     @staticmethod
-    def forward(ctx, student_logits, teacher_index, teacher_logits, temperature, weight):
-        z, idx, t, tau, w = _prepare(student_logits, teacher_index, teacher_logits, temperature, weight)
-        loss = torch.empty(student_logits.shape[:-1], device=z.device, dtype=torch.float32)
-        _capi.distill(z, idx, t, w, None, tau, loss=loss)
-        ctx.save_for_backward(student_logits, teacher_index, teacher_logits, weight)
+    def forward(ctx, student_logits, index, teacher, tau, weight):
+        loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
+        _capi.distill(*_rows(student_logits), index, teacher, weight, None, tau, loss=loss)
+        ctx.save_for_backward(student_logits, index, teacher, weight)
         ctx.tau = tau
         return loss
 
@@ -66,9 +69,8 @@ class DistillCudaFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, index, teacher, weight = ctx.saved_tensors
-        z, idx, t, tau, w = _prepare(logits, index, teacher, ctx.tau, weight)
-        dz = torch.empty(logits.shape, device=z.device, dtype=z.dtype)
-        _capi.distill(z, idx, t, w, grad_loss.to(torch.float32).contiguous(), tau, dz=dz)
+        dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        _capi.distill(*_rows(logits), index, teacher, weight, grad_loss.contiguous(), ctx.tau, dz=dz)
         return dz, None, None, None, None
 
 
@@ -85,13 +87,14 @@ def distill_loss(student_logits, teacher_index, teacher_logits, temperature=1.0,
     loss and gradient 0, whatever its logits are.  Returns (...) float32.  Limits: K <= 1024,
     V times the element size below 1 MiB.
     """
-    if torch.is_grad_enabled() and student_logits.requires_grad:
-        # the constants are looked at here: inside the function gradients are off
-        _prepare(student_logits, teacher_index, teacher_logits, temperature, weight)
-        return DistillCudaFunction.apply(student_logits, teacher_index, teacher_logits, temperature, weight)
-    z, idx, t, tau, w = _prepare(student_logits, teacher_index, teacher_logits, temperature, weight)
-    loss = torch.empty(student_logits.shape[:-1], device=z.device, dtype=torch.float32)
-    _capi.distill(z, idx, t, w, None, tau, loss=loss)
+    recording = torch.is_grad_enabled()
+    if recording and (teacher_logits.requires_grad or (weight is not None and weight.requires_grad)):
+        raise ValueError("teacher_logits and weight are constants of the loss: detach them")
+    tau, index, teacher, w = _check(student_logits, teacher_index, teacher_logits, temperature, weight)
+    if recording and student_logits.requires_grad:
+        return DistillCudaFunction.apply(student_logits, index, teacher, tau, w)
+    loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
+    _capi.distill(*_rows(student_logits), index, teacher, w, None, tau, loss=loss)
     return loss
 
 
@@ -100,8 +103,8 @@ def distill_loss_and_grad(student_logits, teacher_index, teacher_logits, tempera
     logits, in one pass over them: ``(loss (...) float32, grad (..., V) of the logits' dtype)``.
     Nothing is recorded for autograd; ``logits.backward(grad)`` carries the gradient on."""
     with torch.no_grad():
-        z, idx, t, tau, w = _prepare(student_logits, teacher_index, teacher_logits, temperature, weight)
-        loss = torch.empty(student_logits.shape[:-1], device=z.device, dtype=torch.float32)
-        dz = torch.empty(student_logits.shape, device=z.device, dtype=z.dtype)
-        _capi.distill(z, idx, t, w, None, tau, loss=loss, dz=dz)
+        tau, index, teacher, w = _check(student_logits, teacher_index, teacher_logits, temperature, weight)
+        loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
+        dz = torch.empty(student_logits.shape, device=student_logits.device, dtype=student_logits.dtype)
+        _capi.distill(*_rows(student_logits), index, teacher, w, None, tau, loss=loss, dz=dz)
     return loss, dz

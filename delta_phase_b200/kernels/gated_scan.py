@@ -42,14 +42,14 @@ def _check_state(state, B, D, name):
 
 def _forward(x, gate, initial_state, mode, keep):
     B, L, D = x.shape
-    h0 = None if initial_state is None else initial_state.detach().contiguous()
+    h0 = None if initial_state is None else initial_state.contiguous()
     out = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
     final = torch.empty(B, D, device=x.device, dtype=torch.float32)
     saved = None
     if keep:
         tile = _capi.scan_tile()
         saved = torch.empty(B, (L + tile - 1) // tile, D, device=x.device, dtype=torch.float32)
-    _capi.scan_fwd(_unit(x.detach()), _unit(gate.detach()), mode, h0, out, final, saved)
+    _capi.scan_fwd(_unit(x), _unit(gate), mode, h0, out, final, saved)
     return out, final, saved
 
 
@@ -72,10 +72,10 @@ class GatedScanCudaFunction(torch.autograd.Function):
         if grad_out is None and grad_final is None:
             return None, None, None, None
         B, L, D = x.shape
-        go = torch.zeros(B, L, D, device=x.device, dtype=x.dtype) if grad_out is None else _unit(grad_out)
-        gf = None if grad_final is None else grad_final.contiguous()
         dx = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
-        dg = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
+        dg = torch.empty_like(dx)
+        go = torch.zeros_like(dx) if grad_out is None else _unit(grad_out)
+        gf = None if grad_final is None else grad_final.contiguous()
         dh = torch.empty(B, D, device=x.device, dtype=torch.float32) if ctx.needs_input_grad[2] else None
         _capi.scan_bwd(_unit(x), _unit(gate), go, ctx.mode, saved, gf, dx, dg, dh)
         return (dx if ctx.needs_input_grad[0] else None, dg if ctx.needs_input_grad[1] else None, dh, None)
@@ -100,7 +100,6 @@ def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
     _check_inputs(x, gate, 3, "(B, L, D)")
     if initial_state is not None:
         _check_state(initial_state, x.shape[0], x.shape[2], "initial_state")
-    _capi.require_cuda(x, gate, initial_state)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, initial_state)):
         return GatedScanCudaFunction.apply(x, gate, initial_state, mode)
     return _forward(x, gate, initial_state, mode, False)[:2]
@@ -114,7 +113,6 @@ def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None)
     _check_inputs(x, gate, 2, "(B, D)")
     B, D = x.shape
     _check_state(state, B, D, "state")
-    _capi.require_cuda(state, x, gate, state_out, out)
     if state_out is None:
         state_out = torch.empty(B, D, device=x.device, dtype=torch.float32)
     else:
@@ -125,6 +123,5 @@ def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None)
         out = torch.empty(B, D, device=x.device, dtype=x.dtype)
     elif out.dtype != x.dtype or out.shape != x.shape or (D > 1 and out.stride(1) != 1):
         raise ValueError("out must be a (B, D) tensor of x's dtype with unit channel stride")
-    _capi.scan_step(state.detach().contiguous(), state_out.detach(), _unit(x.detach()), _unit(gate.detach()), mode,
-                    out.detach())
+    _capi.scan_step(state.contiguous(), state_out, _unit(x), _unit(gate), mode, out)
     return out, state_out
