@@ -13,13 +13,18 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "dp_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace dp {
+
 namespace {
+
+using namespace ptx;
 
 constexpr int kDiMaxVec = 8;      // 16-byte vectors of a row per thread, at most
 constexpr int kDiMaxThreads = 512;
@@ -36,6 +41,8 @@ struct DistillArgs {
   int64_t rows, sb, st;
   int index64, teacher_dt, L, V, K, cs;
   int group_smem;  // bytes of shared memory of a group
+  int stage_bytes;  // the part of it that holds the group's vectors
+  int regular;  // one row stride, rows (dz's too) of whole vectors on 16 bytes
   float tau, inv_tau, c;  // c = log2(e) / tau
 };
 
@@ -82,10 +89,15 @@ struct Vec<float> {
     (i == 0 ? v.x : v.z) = __float_as_uint(f.x);
     (i == 0 ? v.y : v.w) = __float_as_uint(f.y);
   }
-  static __device__ __forceinline__ float max(const uint4 &v, float m) {
-    return fmaxf(fmaxf(m, fmaxf(__uint_as_float(v.x), __uint_as_float(v.y))),
-                 fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
-  }
+  struct Max {
+    float m;
+    __device__ __forceinline__ void start() { m = -INFINITY; }
+    __device__ __forceinline__ void add(const uint4 &v) {
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                         fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+    }
+    __device__ __forceinline__ float get(float x) const { return fmaxf(x, m); }
+  };
 };
 __device__ __forceinline__ uint32_t &di_word(uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ uint32_t di_word(const uint4 &v, int i) {
@@ -102,11 +114,18 @@ struct Vec<__nv_bfloat16> {
     const __nv_bfloat162 h = __float22bfloat162_rn(f);
     di_word(v, i) = *reinterpret_cast<const uint32_t *>(&h);
   }
-  static __device__ __forceinline__ float max(const uint4 &v, float m) {
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
-    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-    return fmaxf(m, fmaxf(f.x, f.y));
-  }
+  struct Max {  // in pairs until the end
+    __nv_bfloat162 m;
+    __device__ __forceinline__ void start() { m = __float2bfloat162_rn(-INFINITY); }
+    __device__ __forceinline__ void add(const uint4 &v) {
+      const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+      m = __hmax2(m, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    }
+    __device__ __forceinline__ float get(float x) const {
+      const float2 f = __bfloat1622float2(m);
+      return fmaxf(x, fmaxf(f.x, f.y));
+    }
+  };
 };
 template <>
 struct Vec<__half> {
@@ -119,12 +138,30 @@ struct Vec<__half> {
     const __half2 h = __float22half2_rn(f);
     di_word(v, i) = *reinterpret_cast<const uint32_t *>(&h);
   }
-  static __device__ __forceinline__ float max(const uint4 &v, float m) {
-    const __half2 *h = reinterpret_cast<const __half2 *>(&v);
-    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-    return fmaxf(m, fmaxf(f.x, f.y));
-  }
+  struct Max {  // in pairs until the end
+    __half2 m;
+    __device__ __forceinline__ void start() { m = __float2half2_rn(-INFINITY); }
+    __device__ __forceinline__ void add(const uint4 &v) {
+      const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+      m = __hmax2(m, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    }
+    __device__ __forceinline__ float get(float x) const {
+      const float2 f = __half22float2(m);
+      return fmaxf(x, fmaxf(f.x, f.y));
+    }
+  };
 };
+
+// v 2^((m - M) c), for a sum v against the maximum m; against -inf (nothing there) v is 0 or NaN.
+__device__ __forceinline__ float di_scaled(float v, float m, float M, float c) {
+  return m == -INFINITY ? v : v * di_ex2((m - M) * c);
+}
+// The (maximum, sum) of the cluster out of its blocks'.
+__device__ __forceinline__ void di_join(const float2 *part, int cs, float c, float &M, float &S) {
+  for (int r = 0; r < cs; ++r) M = fmaxf(M, part[r].x);
+  S = 0.f;
+  for (int r = 0; r < cs; ++r) S += di_scaled(part[r].y, part[r].x, M, c);
+}
 
 // Shared memory of one group: the teacher's entries (index, logit, the student's logit there)
 // and two bit maps over hashed indices: an entry is there; more than one is (or two indices
@@ -136,35 +173,68 @@ __host__ __device__ inline int di_map_words(int K) {
 }
 inline int di_smem(int K) { return 12 * K + 8 * di_map_words(K); }
 
-// NV vectors per thread; WARP: a warp holds a row, kDiWarpRows rows a block; else a block (or
-// a cluster of a.cs blocks) holds a row.
-template <typename T, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kDiWarpRows : kDiMaxThreads, WARP ? 6 : 2)
-distill_kernel(const DistillArgs a) {
-  using W = Vec<T>;
-  constexpr int E = W::E;
-  __shared__ Part parts[kDiMaxThreads / 32];
-  __shared__ float2 cpart[kDiMaxCluster];
-  extern __shared__ __align__(16) unsigned char dyn[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tid = WARP ? lane : (int)threadIdx.x, n = WARP ? 32 : (int)blockDim.x;
-  const int cs = WARP ? 1 : a.cs, rank = WARP ? 0 : blockIdx.x % cs;
-  const unsigned row = WARP ? blockIdx.x * kDiWarpRows + warp : blockIdx.x / cs;
-  if (WARP && row >= a.rows) return;  // whole warps
-  const float weight = a.weight ? a.weight[row] : 1.f, grad = a.grad ? a.grad[row] : 1.f;
-  const unsigned batch = row / a.L;
-  const T *z = static_cast<const T *>(a.z) + batch * a.sb + (row - batch * a.L) * a.st;
-  T *dz = a.dz ? static_cast<T *>(a.dz) + (int64_t)row * a.V : nullptr;
-  // The row: 16-byte aligned vectors from element `head` on, split over the cluster, and fewer
-  // than 2 E single elements before and behind them, one each for the first block's threads.
-  const int phase = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-  const int head = min(phase ? E - phase : 0, a.V), nvec = (a.V - head) / E, tail = head + nvec * E;
-  const int per = (nvec + cs - 1) / cs, v0 = min(rank * per, nvec), cnt = min(per, nvec - v0);
-  const int edge = rank ? a.V : tid < head ? tid : tail + tid - head;  // this thread's; none: V and on
-  const uint4 *zv = reinterpret_cast<const uint4 *>(z + head) + v0;
-  // dz may lie differently against the 16-byte grid than z
-  const bool vec = (reinterpret_cast<uintptr_t>(dz) & 15) == (reinterpret_cast<uintptr_t>(z) & 15);
-  auto write_zeros = [&] {
+struct Entries {
+  int *index;       // -1: padding
+  float *t, *z;     // teacher's and student's logit there
+  uint32_t *once, *again;
+  int words;
+};
+__device__ __forceinline__ Entries di_entries(unsigned char *mem, int K) {
+  Entries e;
+  e.index = reinterpret_cast<int *>(mem);
+  e.t = reinterpret_cast<float *>(e.index + K), e.z = e.t + K;
+  e.words = di_map_words(K);
+  e.once = reinterpret_cast<uint32_t *>(e.z + K), e.again = e.once + e.words;
+  return e;
+}
+
+// One teacher entry as it is read ahead of its row.
+struct Entry {
+  int64_t index;
+  uint32_t t;
+  __device__ __forceinline__ void read(const DistillArgs &a, unsigned row, int k) {
+    const int64_t o = (int64_t)row * a.K + k;
+    index = a.index64 ? static_cast<const int64_t *>(a.index)[o] : static_cast<const int32_t *>(a.index)[o];
+    t = load_raw_scalar(a.teacher, a.teacher_dt, o);
+  }
+  __device__ __forceinline__ bool ok(const DistillArgs &a) const { return index >= 0 && index < a.V; }
+};
+
+// A row as its group sees it: 16-byte aligned vectors from element `head` on, split over the
+// cluster (this block's: v0 .. v0 + cnt - 1), and fewer than 2 E single elements before and
+// behind them, one each for the threads of the first block (edge; none: V and on).
+template <typename T>
+struct Row {
+  const T *z;
+  T *dz;
+  unsigned row;
+  int head, tail, v0, cnt, edge;
+  bool vec;  // dz lies like z against the 16-byte grid
+  __device__ __forceinline__ Row(const DistillArgs &a, unsigned row_, int rank, int cs, int tid) : row(row_) {
+    constexpr int E = Vec<T>::E;
+    dz = a.dz ? static_cast<T *>(a.dz) + (int64_t)row * a.V : nullptr;
+    int nvec;
+    if (a.regular) {  // every row is vectors from its first element to its last
+      z = static_cast<const T *>(a.z) + row * a.st;
+      head = 0, tail = edge = a.V, nvec = a.V / E;
+      vec = true;
+    } else {
+      const unsigned batch = row / a.L;
+      z = static_cast<const T *>(a.z) + batch * a.sb + (row - batch * a.L) * a.st;
+      const int phase = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+      head = min(phase ? E - phase : 0, a.V);
+      nvec = (a.V - head) / E;
+      tail = head + nvec * E;
+      edge = rank ? a.V : tid < head ? tid : tail + tid - head;
+      vec = (reinterpret_cast<uintptr_t>(dz) & 15) == (reinterpret_cast<uintptr_t>(z) & 15);
+    }
+    const int per = cs == 1 ? nvec : (nvec + cs - 1) / cs;
+    v0 = min(rank * per, nvec), cnt = min(per, nvec - v0);
+  }
+  __device__ __forceinline__ const uint4 *vectors() const { return reinterpret_cast<const uint4 *>(z + head) + v0; }
+  // A row that does not count: loss 0 (by the caller), gradient 0, z not looked at.
+  __device__ __forceinline__ void zeros(const DistillArgs &a, int tid, int n) const {
+    constexpr int E = Vec<T>::E;
     for (int j = tid; j < cnt; j += n) {
       T *p = dz + head + (v0 + j) * E;
       if (vec)
@@ -173,181 +243,306 @@ distill_kernel(const DistillArgs a) {
         for (int k = 0; k < E; ++k) p[k] = from_f32<T>(0.f);
     }
     if (edge < a.V) dz[edge] = from_f32<T>(0.f);
-  };
-  if (weight == 0.f) {  // a padding row: z is not looked at (the same for the whole cluster)
-    if (a.loss && rank == 0 && tid == 0) a.loss[row] = 0.f;
-    if (dz) write_zeros();
-    return;
   }
-  if (cs > 1) cg::this_cluster().sync();  // every block of the cluster runs
-  uint4 raw[NV];
-  if (cnt == NV * n) {
+};
+
+// The threads that hold a row (or a block's slice of it): tid of n, whole warps.
+struct WarpGroup {
+  int tid, n = 32;
+  Part *parts;
+  __device__ __forceinline__ void sync() const { __syncwarp(); }
+};
+struct BlockGroup {
+  int tid, n;
+  Part *parts;
+  __device__ __forceinline__ void sync() const { __syncthreads(); }
+};
+// The i-th vector of a thread, -inf past the end: out of the row's copy in shared memory, or
+// out of the registers it was read into.
+template <typename T>
+__device__ __forceinline__ uint4 di_nothing() {
+  uint4 v;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = zv[tid + i * n];
-  } else {
+  for (int k = 0; k < Vec<T>::E / 2; ++k) Vec<T>::set(v, k, make_float2(-INFINITY, -INFINITY));
+  return v;
+}
+struct FromShared {
+  uint32_t v;  // of this thread
+  int n;
+  // volatile: read again in each pass, not kept in registers between them
+  __device__ __forceinline__ uint4 operator()(int i) const {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(v + i * n * 16));
+    return x;
+  }
+};
+template <int NV>
+struct FromRegisters {
+  uint4 v[NV];
+  __device__ __forceinline__ uint4 operator()(int i) const { return v[i]; }
+};
+
+// Loss and gradient of a row (ze: the thread's single element, -inf if none; first: entry
+// `tid`, read ahead; zt: the student's logit there).  `loaded` runs once all of the group have
+// read their vectors; `join` makes the (maximum, sum) of the cluster out of this block's.
+// KEEP: the exponentials, against the warp's maximum, are kept in float32 registers and the
+// gradient is their multiple; otherwise the gradient's pass computes them again.
+template <typename T, int NV, bool KEEP, class G, class Src, class Join>
+__device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e, int rank,
+                                       float weight, float grad, const Src &src, float ze, const Entry &first,
+                                       float zt, Join join) {
+  using W = Vec<T>;
+  constexpr int E = W::E;
+  const int tid = g.tid, n = g.n, lane = threadIdx.x & 31, warps = n >> 5;
+  const float c = a.c;
+  Part w;
+  typename W::Max vm;
+  vm.start();
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+  for (int i = 0; i < NV; ++i) vm.add(src(i));
+  w.m = di_warp_redux_max(vm.get(ze));
+  // what is masked throughout has the sum 0, not NaN
+  const float m0 = w.m == -INFINITY ? 0.f : w.m;
+  // Exponents z c - m c in one rounding; what the rounding of m c did to all of them alike is
+  // taken back from the sum and the gradient's factor (corr).  Where m c would overflow
+  // -- a row that is masked throughout by the type's lowest value -- values other than m are
+  // further from it than any exponent reaches: 0 for m, -inf for the others.
+  const bool far = fabsf(m0) * c > 1e37f && fabsf(m0) < INFINITY;
+  const float mc = m0 * c, corr = far ? 1.f : di_ex2(-fmaf(m0, c, -mc));
+  const float2 c2 = make_float2(c, c), off = make_float2(-mc, -mc);
+  auto exps = [&](const uint4 &v, int k) {
+    const float2 x = __ffma2_rn(W::pair(v, k), c2, off);
+    return make_float2(di_ex2(x.x), di_ex2(x.y));
+  };
+  auto far_exp = [&](float z) { return z == m0 ? 1.f : z == -INFINITY ? 0.f : z * 0.f; };
+  auto far_exps = [&](const uint4 &v, int k) {
+    const float2 z = W::pair(v, k);
+    return make_float2(far_exp(z.x), far_exp(z.y));
+  };
+  float2 ev[KEEP ? NV * E / 2 : 1];
+  const float ee = far ? far_exp(ze) : di_ex2(fmaf(ze, c, -mc));
+  float2 acc[2] = {make_float2(ee, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int k = 0; k < E / 2; ++k) W::set(raw[i], k, make_float2(-INFINITY, -INFINITY));
-      if (tid + i * n < cnt) raw[i] = zv[tid + i * n];
+  for (int i = 0; i < NV; ++i) {
+    const uint4 v = src(i);
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+      const float2 x = exps(v, k);
+      if (KEEP) ev[i * (E / 2) + k] = x;
+      acc[k & 1] = __fadd2_rn(acc[k & 1], x);
     }
   }
-  const float ze = edge < a.V ? to_f32(z[edge]) : -INFINITY;
-  // the teacher's entries, and the student's logits there
-  int *si = reinterpret_cast<int *>(dyn + (WARP ? warp * a.group_smem : 0));
-  float *st = reinterpret_cast<float *>(si + a.K), *sz = st + a.K;
-  const int words = di_map_words(a.K);
-  uint32_t *once = reinterpret_cast<uint32_t *>(sz + a.K), *again = once + words;
-  float tm = -INFINITY;
-  for (int k = tid; k < a.K; k += n) {
-    const int64_t o = (int64_t)row * a.K + k;
-    const int64_t i = a.index64 ? static_cast<const int64_t *>(a.index)[o] : static_cast<const int32_t *>(a.index)[o];
-    const bool ok = i >= 0 && i < a.V;
-    const float t = ok ? raw_scalar_to_f32(load_raw_scalar(a.teacher, a.teacher_dt, o), a.teacher_dt) : -INFINITY;
-    si[k] = ok ? (int)i : -1;
-    st[k] = t;
-    sz[k] = ok ? to_f32(z[i]) : 0.f;
-    tm = fmaxf(tm, t);
-  }
-  if (dz)
-    for (int k = tid; k < 2 * words; k += n) once[k] = 0;
-  // Exponents: the maximum is taken off before the factor is applied, so masked logits of the
-  // type's lowest value do not overflow; what is masked throughout has the sum 0, not NaN.
-  const float c = a.c;
-  const float2 c2 = make_float2(c, c);
-  Part w;
-  w.m = ze;
+  if (far) {
+    acc[0] = make_float2(ee, 0.f), acc[1] = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) w.m = W::max(raw[i], w.m);
-  w.m = di_warp_redux_max(w.m);
-  const float m0 = w.m == -INFINITY ? 0.f : w.m;
-  {
-    float2 acc[2] = {make_float2(di_ex2((ze - m0) * c), 0.f), make_float2(0.f, 0.f)};
-    const float2 off = make_float2(-m0, -m0);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const uint4 v = src(i);
 #pragma unroll
       for (int k = 0; k < E / 2; ++k) {
-        const float2 x = __fmul2_rn(__fadd2_rn(W::pair(raw[i], k), off), c2);
-        acc[k & 1] = __fadd2_rn(acc[k & 1], make_float2(di_ex2(x.x), di_ex2(x.y)));
+        const float2 x = far_exps(v, k);
+        if (KEEP) ev[i * (E / 2) + k] = x;
+        acc[k & 1] = __fadd2_rn(acc[k & 1], x);
       }
-    acc[0] = __fadd2_rn(acc[0], acc[1]);
-    w.s = di_warp_sum(acc[0].x + acc[0].y);
+    }
   }
+  acc[0] = __fadd2_rn(acc[0], acc[1]);
+  w.s = di_warp_sum(acc[0].x + acc[0].y) * corr;
+  // the teacher's entries
+  const bool entries = tid - lane < a.K;  // a warp that has some
   w.tm = -INFINITY, w.ts = w.d = 0.f;
-  if (tid - lane < a.K) {  // a warp that has entries
+  if (entries) {
+    float tm = -INFINITY;
+    for (int k = tid; k < a.K; k += n) {
+      Entry x = first;
+      if (k != tid) x.read(a, r.row, k);
+      const bool ok = x.ok(a);
+      if (k != tid) zt = ok ? to_f32(r.z[x.index]) : 0.f;
+      const float t = ok ? raw_scalar_to_f32(x.t, a.teacher_dt) : -INFINITY;
+      e.index[k] = ok ? (int)x.index : -1;
+      e.t[k] = t;
+      e.z[k] = zt;
+      tm = fmaxf(tm, t);
+    }
     w.tm = di_warp_redux_max(tm);
     const float t0 = w.tm == -INFINITY ? 0.f : w.tm;
     for (int k = tid; k < a.K; k += n) {
-      const float t = st[k] - t0, e = di_ex2(t * c);
-      w.ts += e;
-      if (e != 0.f && si[k] >= 0) w.d = fmaf(e, t - (sz[k] - m0), w.d);
+      const float t = e.t[k] - t0, x = di_ex2(t * c);
+      w.ts += x;
+      if (x != 0.f && e.index[k] >= 0) w.d = fmaf(x, t - (e.z[k] - m0), w.d);
     }
     w.ts = di_warp_sum(w.ts);
     w.d = di_warp_sum(w.d);
   }
-  // the parts of all warps: maxima, then sums relative to them
+  if (a.dz)
+    for (int k = tid; k < 2 * e.words; k += n) e.once[k] = 0;
+  // the parts of all warps: maxima, then sums relative to them; what the teacher's side gives
+  // is needed where entries are handled and by the thread that writes the loss
   float M = w.m, S = w.s, TM = w.tm, TS = w.ts, D = w.d;
-  const int warps = blockDim.x >> 5;
-  if (WARP) {
-    __syncwarp();  // the entries and the cleared maps are seen by all lanes
-  } else {
-    if (lane == 0) parts[warp] = w;
-    __syncthreads();
+  bool empty = TS == 0.f;
+  if (warps > 1) {
+    if (lane == 0) g.parts[tid >> 5] = w;
+    g.sync();
     Part q = {-INFINITY, 0.f, -INFINITY, 0.f, 0.f};
-    if (lane < warps) q = parts[lane];
+    if (lane < warps) q = g.parts[lane];
     M = di_warp_redux_max(q.m);
-    TM = di_warp_redux_max(q.tm);
-    S = di_warp_sum(q.m == -INFINITY ? q.s : q.s * di_ex2((q.m - M) * c));
-    const float f = q.tm == -INFINITY ? 1.f : di_ex2((q.tm - TM) * c);
-    TS = di_warp_sum(q.ts * f);
-    // d against the common maxima (a part without entries has ts = d = 0)
-    if (q.ts != 0.f) q.d = f * fmaf(q.ts, (q.tm - TM) - ((q.m == -INFINITY ? 0.f : q.m) - (M == -INFINITY ? 0.f : M)), q.d);
-    D = di_warp_sum(q.d);
+    const float qs = di_scaled(q.s, q.m, M, c);
+    S = di_warp_sum(qs);
+    empty = !__any_sync(0xffffffffu, q.ts != 0.f);
+    if (entries) {
+      TM = di_warp_redux_max(q.tm);
+      const float f = q.tm == -INFINITY ? 1.f : di_ex2((q.tm - TM) * c);
+      TS = di_warp_sum(q.ts * f);
+      // d against the common maxima (a part without entries has ts = d = 0)
+      if (q.ts != 0.f)
+        q.d = f * fmaf(q.ts, (q.tm - TM) - ((q.m == -INFINITY ? 0.f : q.m) - (M == -INFINITY ? 0.f : M)), q.d);
+      D = di_warp_sum(q.d);
+    }
+  } else {
+    g.sync();
   }
   // the entries' bits (their maps were cleared before the barrier)
-  if (dz)
+  if (a.dz && entries)
     for (int k = tid; k < a.K; k += n)
-      if (si[k] >= 0) {
-        const uint32_t bit = 1u << (si[k] & 31);
-        uint32_t *word = &once[si[k] >> 5 & (words - 1)];
-        if (atomicOr(word, bit) & bit) atomicOr(word + words, bit);
+      if (e.index[k] >= 0) {
+        const uint32_t bit = 1u << (e.index[k] & 31);
+        uint32_t *word = &e.once[e.index[k] >> 5 & (e.words - 1)];
+        if (atomicOr(word, bit) & bit) atomicOr(word + e.words, bit);
       }
   const float M0 = M;
-  if (cs > 1) {
-    cg::cluster_group cl = cg::this_cluster();
-    if (tid < cs) cl.map_shared_rank(cpart, tid)[rank] = make_float2(M, S);
-    cl.sync();
-    for (int r = 0; r < cs; ++r) M = fmaxf(M, cpart[r].x);
-    S = 0.f;
-    for (int r = 0; r < cs; ++r)
-      S += cpart[r].x == -INFINITY ? cpart[r].y : cpart[r].y * di_ex2((cpart[r].x - M) * c);
-  }
+  join(M, S);
   // masked throughout (or NaN throughout): 0 / 0
   if (M == -INFINITY) S = NAN;
-  const bool empty = TS == 0.f;
   if (a.loss && rank == 0 && tid == 0) {
     // sum p (log p - log q) = sum p ((t - TM) - (z - M)) / tau - log TS + log S
     const float d = D / TS - ((M0 == -INFINITY ? 0.f : M0) - M);
-    a.loss[row] = empty ? 0.f : weight * a.tau * a.tau * (d * a.inv_tau + (logf(S) - logf(TS)));
+    a.loss[r.row] = empty ? 0.f : weight * a.tau * a.tau * (d * a.inv_tau + (logf(S) - logf(TS)));
   }
-  if (!dz) return;
+  if (!a.dz) return;
   if (empty || grad == 0.f) {
-    write_zeros();
+    r.zeros(a, tid, n);
     return;
   }
-  const float cw = weight * a.tau * grad, inv_S = di_rcp(S), scale = cw * inv_S;
-  const float2 off = make_float2(-M, -M), scale2 = make_float2(scale, scale);
-  T *pd = dz + head + (v0 + tid) * E;
+  const float cw = weight * a.tau * grad, inv_S = di_rcp(S);
+  // from the warp's maximum to the row's (a warp that is masked throughout has only zeros)
+  const float scale = di_scaled(cw * inv_S, w.m, M, c) * corr;
+  const float2 scale2 = make_float2(scale, scale);
+  T *pd = r.dz + r.head + (r.v0 + tid) * E;
+  auto write = [&](auto exp_of) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    uint4 o;
+    for (int i = 0; i < NV; ++i) {
+      uint4 o, v;
+      if (!KEEP) v = src(i);
 #pragma unroll
-    for (int k = 0; k < E / 2; ++k) {
-      const float2 x = __fmul2_rn(__fadd2_rn(W::pair(raw[i], k), off), c2);
-      W::set(o, k, __fmul2_rn(make_float2(di_ex2(x.x), di_ex2(x.y)), scale2));
-    }
-    if (tid + i * n < cnt) {
-      T *p = pd + i * n * E;
-      if (vec) {
-        *reinterpret_cast<uint4 *>(p) = o;
-      } else {
-        const T *e = reinterpret_cast<const T *>(&o);
+      for (int k = 0; k < E / 2; ++k)
+        W::set(o, k, __fmul2_rn(KEEP ? ev[i * (E / 2) + k] : exp_of(v, k), scale2));
+      if (tid + i * n < r.cnt) {
+        T *p = pd + i * n * E;
+        if (r.vec) {
+          *reinterpret_cast<uint4 *>(p) = o;
+        } else {
+          const T *x = reinterpret_cast<const T *>(&o);
 #pragma unroll
-        for (int k = 0; k < E; ++k) p[k] = e[k];
+          for (int k = 0; k < E; ++k) p[k] = x[k];
+        }
       }
     }
-  }
-  if (edge < a.V) dz[edge] = from_f32<T>(di_ex2((ze - M) * c) * scale);
-  if (WARP)
-    __syncwarp();
+  };
+  if (!KEEP && far)
+    write(far_exps);
   else
-    __syncthreads();  // the dense values are written and the maps complete: now the teacher's entries
+    write(exps);
+  if (r.edge < a.V) r.dz[r.edge] = from_f32<T>(ee * scale);
+  g.sync();  // the dense values are written and the maps complete: now the teacher's entries
+  if (!entries) return;
   const float inv_TS = di_rcp(TS);
   for (int k0 = tid - lane; k0 < a.K; k0 += n) {  // whole warps
-    const int k = k0 + lane, i = k < a.K ? si[k] : -1;
+    const int k = k0 + lane, i = k < a.K ? e.index[k] : -1;
     // this block's elements (vectors, and the single ones for the first)
-    const bool here = i >= 0 && (i < head || i >= tail ? rank == 0 : i >= head + v0 * E && i < head + (v0 + cnt) * E);
-    float p = here ? di_ex2((st[k] - TM) * c) * inv_TS : 0.f;
-    // an index that occurs more than once: the warp adds up all its entries, in a fixed order,
-    // so each of them writes the same value
-    uint32_t more = __ballot_sync(0xffffffffu, here && (again[i >> 5 & (words - 1)] >> (i & 31) & 1));
+    const bool here = i >= 0 && (i < r.head || i >= r.tail
+                                     ? rank == 0
+                                     : i >= r.head + r.v0 * E && i < r.head + (r.v0 + r.cnt) * E);
+    float p = here ? di_ex2((e.t[k] - TM) * c) * inv_TS : 0.f;
+    // an index that occurs more than once: the warp adds up all its entries, in a fixed
+    // order, so each of them writes the same value
+    uint32_t more = __ballot_sync(0xffffffffu, here && (e.again[i >> 5 & (e.words - 1)] >> (i & 31) & 1));
     while (more) {
-      const int src = __ffs(more) - 1, at = __shfl_sync(0xffffffffu, i, src);
+      const int from = __ffs(more) - 1, at = __shfl_sync(0xffffffffu, i, from);
       more &= more - 1;
       float t = 0.f;
       for (int q = lane; q < a.K; q += 32)
-        if (si[q] == at) t += di_ex2((st[q] - TM) * c) * inv_TS;
+        if (e.index[q] == at) t += di_ex2((e.t[q] - TM) * c) * inv_TS;
       t = di_warp_sum(t);
-      if (lane == src) p = t;
+      if (lane == from) p = t;
     }
-    if (here) dz[i] = from_f32<T>(cw * (di_ex2((sz[k] - M) * c) * inv_S - p));
+    if (here) r.dz[i] = from_f32<T>(cw * (di_ex2((e.z[k] - M) * c) * inv_S - p));
   }
 }
 
-template <typename T, int NV, bool WARP>
+// A block (or a cluster of a.cs blocks) holds a row, or with WARP a warp, kDiWarpRows rows a
+// block; NV vectors per thread.  STAGE: the vectors wait in shared memory, each copied there
+// (cp.async) by the thread that reads it, twice, so that three times as many threads fit on an
+// SM as hold their exponentials in registers: many rows, HBM counts.  Otherwise they are read
+// into registers: few rows, latency counts.
+template <typename T, int NV, bool WARP, bool STAGE>
+__global__ void __launch_bounds__(WARP ? 32 * kDiWarpRows : kDiMaxThreads, (STAGE ? 1536 : 1024) / (WARP ? 32 * kDiWarpRows : kDiMaxThreads))
+distill_kernel(const DistillArgs a) {
+  __shared__ Part parts[kDiMaxThreads / 32];
+  __shared__ float2 cpart[kDiMaxCluster];
+  extern __shared__ __align__(16) unsigned char dyn[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cs = WARP ? 1 : a.cs, rank = WARP ? 0 : blockIdx.x % cs;
+  const unsigned row = WARP ? blockIdx.x * kDiWarpRows + warp : blockIdx.x / cs;
+  if (WARP && row >= a.rows) return;  // whole warps
+  std::conditional_t<WARP, WarpGroup, BlockGroup> g;
+  g.tid = WARP ? lane : (int)threadIdx.x, g.n = WARP ? 32 : (int)blockDim.x, g.parts = parts;
+  const float weight = a.weight ? a.weight[row] : 1.f, grad = a.grad ? a.grad[row] : 1.f;
+  Entry first = {-1, 0};
+  if (g.tid < a.K) first.read(a, row, g.tid);
+  const Row<T> r(a, row, rank, cs, g.tid);
+  if (weight == 0.f) {  // the same for the whole cluster
+    if (a.loss && rank == 0 && g.tid == 0) a.loss[row] = 0.f;
+    if (a.dz) r.zeros(a, g.tid, g.n);
+    return;
+  }
+  unsigned char *mem = dyn + (WARP ? warp * a.group_smem : 0);
+  std::conditional_t<STAGE, FromShared, FromRegisters<NV>> src;
+  if constexpr (STAGE) {
+    uint4 *slot = reinterpret_cast<uint4 *>(mem) + g.tid;
+    const uint32_t s = smem_u32(slot);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (g.tid + i * g.n < r.cnt)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(s + i * g.n * 16),
+                     "l"(r.vectors() + g.tid + i * g.n)
+                     : "memory");
+      else
+        slot[i * g.n] = di_nothing<T>();
+    }
+    mem += a.stage_bytes;
+    src.v = s, src.n = g.n;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      src.v[i] = g.tid + i * g.n < r.cnt ? r.vectors()[g.tid + i * g.n] : di_nothing<T>();
+  }
+  if (cs > 1) cg::this_cluster().sync();  // every block of the cluster runs
+  const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
+  const float zt = first.ok(a) ? to_f32(r.z[first.index]) : 0.f;
+  if constexpr (STAGE) asm volatile("cp.async.wait_all;\n" ::: "memory");
+  di_row<T, NV, !STAGE>(a, g, r, di_entries(mem, a.K), rank, weight, grad, src, ze, first, zt, [&](float &M, float &S) {
+    if (cs == 1) return;
+    cg::cluster_group cl = cg::this_cluster();
+    if (g.tid < cs) cl.map_shared_rank(cpart, g.tid)[rank] = make_float2(M, S);
+    cl.sync();
+    di_join(cpart, cs, a.c, M, S);
+  });
+}
+
+template <typename T, int NV, bool WARP, bool STAGE>
 int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, cudaStream_t st) {
-  auto kern = distill_kernel<T, NV, WARP>;
+  auto kern = distill_kernel<T, NV, WARP, STAGE>;
   cudaError_t e = cudaSuccess;
   if (smem > 40 * 1024)  // beside the static part
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -378,14 +573,20 @@ int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, 
 template <typename T>
 int distill_launch(DistillArgs a, cudaStream_t st) {
   constexpr int E = Vec<T>::E;
+  const int64_t size = sizeof(T);
   const int nvec = a.V / E;  // at most: fewer where a row does not start on 16 bytes
+  a.regular = a.V % E == 0 && (a.rows == a.L || a.sb == a.L * a.st) && a.st * size % 16 == 0 &&
+              ((reinterpret_cast<uintptr_t>(a.z) | reinterpret_cast<uintptr_t>(a.dz)) & 15) == 0;
+  const int entries = (di_smem(a.K) + 15) / 16 * 16;
   a.cs = 1;
   if (nvec <= 32 * kDiMaxVec) {
     const int64_t blocks = (a.rows + kDiWarpRows - 1) / kDiWarpRows;
-    a.group_smem = di_smem(a.K);
+    const bool two = nvec <= 64;
+    a.stage_bytes = 32 * (two ? 2 : kDiMaxVec) * 16;
+    a.group_smem = a.stage_bytes + entries;
     const size_t smem = (size_t)a.group_smem * kDiWarpRows;
-    if (nvec <= 64) return distill_run<T, 2, true>(a, blocks, 32 * kDiWarpRows, smem, st);
-    return distill_run<T, kDiMaxVec, true>(a, blocks, 32 * kDiWarpRows, smem, st);
+    return two ? distill_run<T, 2, true, true>(a, blocks, 32 * kDiWarpRows, smem, st)
+               : distill_run<T, kDiMaxVec, true, true>(a, blocks, 32 * kDiWarpRows, smem, st);
   }
   const int most = kDiMaxThreads * kDiMaxVec;
   while (a.cs < kDiMaxCluster && (int64_t)a.cs * most < nvec) a.cs *= 2;
@@ -394,12 +595,13 @@ int distill_launch(DistillArgs a, cudaStream_t st) {
   while (a.cs < kDiMaxCluster && a.rows * a.cs < kDiSms && nvec / a.cs >= 2 * kDiMaxThreads) a.cs *= 2;
   const int per = (nvec + a.cs - 1) / a.cs;
   const int64_t blocks = a.rows * a.cs;
-  const int nv = blocks >= 2 * kDiSms ? kDiMaxVec : per > 4 * kDiMaxThreads ? kDiMaxVec : per > kDiMaxThreads ? 4 : 1;
+  const int nv = blocks >= 2 * kDiSms || per > 4 * kDiMaxThreads ? kDiMaxVec : per > kDiMaxThreads ? 4 : 1;
   const int threads = std::max(64, ((per + nv - 1) / nv + 31) / 32 * 32);
-  const size_t smem = a.group_smem = di_smem(a.K);
-  if (nv == 1) return distill_run<T, 1, false>(a, blocks, threads, smem, st);
-  if (nv == 4) return distill_run<T, 4, false>(a, blocks, threads, smem, st);
-  return distill_run<T, kDiMaxVec, false>(a, blocks, threads, smem, st);
+  a.stage_bytes = nv == kDiMaxVec ? threads * nv * 16 : 0;
+  a.group_smem = a.stage_bytes + entries;
+  if (nv == 1) return distill_run<T, 1, false, false>(a, blocks, threads, a.group_smem, st);
+  if (nv == 4) return distill_run<T, 4, false, false>(a, blocks, threads, a.group_smem, st);
+  return distill_run<T, kDiMaxVec, false, true>(a, blocks, threads, a.group_smem, st);
 }
 
 }  // namespace

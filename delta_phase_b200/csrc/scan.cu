@@ -27,8 +27,8 @@
 #include <string>
 #include <type_traits>
 
+#include "cluster_msg.cuh"
 #include "dp_common.cuh"
-#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -245,41 +245,6 @@ __device__ __forceinline__ void cluster_start(uint64_t *bar, int cs) {
   }
   cg::this_cluster().sync();  // the barriers exist in every block before the first message
 }
-__device__ __forceinline__ uint32_t peer_addr(const void *p, int rank) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ void send(uint32_t dst, uint32_t bar, float a, float b) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];\n" ::"r"(dst),
-               "f"(a), "f"(b), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void send(uint32_t dst, uint32_t bar, float2 a, float2 b) {
-  asm volatile(
-      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];\n" ::"r"(dst),
-      "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"(bar)
-      : "memory");
-}
-// Waits for the span's maps; a wait that lasts kWaitNs (it cannot, unless a block of the
-// cluster died) is recorded in the device error word and the walk goes on without waiting.
-constexpr uint64_t kWaitNs = 2000000000ull;
-__device__ __forceinline__ bool wait_maps(uint64_t *bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer();
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (globaltimer() - t0 > kWaitNs) return false;
-  }
-}
-
 // The n = -d of a thread's tokens from the staged gates; tokens past the end keep the state.
 template <typename T, int V, int MODE, typename F>
 __device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[kTok]) {
@@ -376,14 +341,14 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanArgs a)
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
-          send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
       } else {
         sh.bmap[buf][0][lane] = r;
       }
     }
     if (a.cs == 1)
       __syncthreads();
-    else if (alive && !wait_maps(&sh.bar[buf], phase >> 1 & 1))
+    else if (alive && !cluster_wait(&sh.bar[buf], phase >> 1 & 1))
       alive = false;
     // the state that reaches this block, this warp, and the next span
     F in = h;
@@ -473,14 +438,14 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const ScanArgs a)
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
-          send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
       } else {
         sh.bmap[buf][0][lane] = r;
       }
     }
     if (a.cs == 1)
       __syncthreads();
-    else if (alive && !wait_maps(&sh.bar[buf], phase >> 1 & 1))
+    else if (alive && !cluster_wait(&sh.bar[buf], phase >> 1 & 1))
       alive = false;
     F qi = q;
     for (int k = a.cs - 1; k >= 0; --k) {
