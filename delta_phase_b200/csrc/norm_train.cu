@@ -9,6 +9,7 @@
 // read and its write, so each pass reads and writes every tensor once and HBM bounds it.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "dp_common.cuh"
 
@@ -150,7 +151,7 @@ __device__ __forceinline__ float ln_group_sum(float v, float *slot) {
 
 // G threads per row, 8 NV columns per thread.
 template <int G, int NV, bool VEC>
-__global__ void __launch_bounds__(G == 32 ? 128 : G) ln_fwd_kernel(LnFwdArgs a) {
+__global__ void __launch_bounds__(G == 32 ? 128 : G, G == 32 ? 6 : 2) ln_fwd_kernel(LnFwdArgs a) {
   __shared__ float slot[2][G / 32];
   const int g = threadIdx.x % G;
   const int64_t r = (int64_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
@@ -188,14 +189,17 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G) ln_fwd_kernel(LnFwdArgs a) 
     a.mean[r] = mean;
     a.rstd[r] = rstd;
   }
-  float w[NV][8], b[NV][8];
-  if (a.w) ln_load_row<G, NV, VEC>(a.w, g, a.d, w);
-  if (a.b) ln_load_row<G, NV, VEC>(a.b, g, a.d, b);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    // the parameters eight columns at a time (L1), not all of them in registers
+    float w[1][8], b[1][8];
+    const int gi = VEC ? g + G * i : g + 8 * G * i;
+    if (a.w) ln_load_row<G, 1, VEC>(a.w, gi, a.d, w);
+    if (a.b) ln_load_row<G, 1, VEC>(a.b, gi, a.d, b);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      v[i][j] = fmaf(v[i][j] * rstd, a.w ? w[i][j] : kNoWeight, a.b ? b[i][j] : 0.f);
+      v[i][j] = fmaf(v[i][j] * rstd, a.w ? w[0][j] : kNoWeight, a.b ? b[0][j] : 0.f);
+  }
   ln_store_row<G, NV, VEC>(a.y, a.y_dt, off, g, a.d, v);
 }
 
@@ -248,54 +252,113 @@ struct LnBwdArgs {
   int64_t rows;
 };
 
-constexpr int kLnRows = 2;  // rows a group of threads handles between two barriers
+// Resident blocks of the backward kernel: all of them run at once and walk over the rows.
+constexpr int ln_bwd_per_sm(int G) { return G <= 256 ? 2 : 1; }
+
+// Eight columns of a row as they lie in memory (vectors, or single values), loaded a row ahead
+// and converted when their turn comes.  WIDE: float32; otherwise a 16-bit type by its code.
+template <int G, bool VEC, bool WIDE>
+struct LnRaw {
+  static constexpr int N = VEC && !WIDE ? 4 : 8;
+  uint32_t r[N];
+  __device__ __forceinline__ void load(const void *p, int64_t off, int g, int d) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) r[j] = 0;
+      if (8 * g < d) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + (off + 8 * g) * (WIDE ? 4 : 2));
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) {
+          const uint4 a = q[j];
+          r[4 * j] = a.x, r[4 * j + 1] = a.y, r[4 * j + 2] = a.z, r[4 * j + 3] = a.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t i = off + g + G * j;
+        r[j] = g + G * j >= d ? 0u
+               : WIDE         ? static_cast<const uint32_t *>(p)[i]
+                              : (uint32_t)static_cast<const unsigned short *>(p)[i];
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int dt, int j) const {
+    if constexpr (WIDE)
+      return __uint_as_float(r[j]);
+    else if constexpr (VEC)
+      return raw_scalar_to_f32(j & 1 ? r[j / 2] >> 16 : r[j / 2] & 0xffffu, dt);
+    else
+      return raw_scalar_to_f32(r[j], dt);
+  }
+};
 
 // G threads per row, eight columns per thread; a block is max(G, 256) threads.  The block
 // walks over the rows (grid-stride), each thread adding up dw and db of its own columns in
 // registers; at the end the block writes one partial row, and ln_bwd_reduce_kernel adds
 // the blocks' rows in a fixed order (the result does not depend on timing).  The two sums
-// of a row cross the block through shared memory, kLnRows rows a barrier.
-template <int G, bool VEC>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) ln_bwd_kernel(LnBwdArgs a) {
-  constexpr int BT = G < 256 ? 256 : G, NG = BT / G, W = G / 32, R = kLnRows;
-  __shared__ float red[2][NG][2 * R][W];
+// of a row cross the block through shared memory, R rows a barrier; the next rows' s and dy are
+// on their way meanwhile.
+template <int G, bool VEC, bool S32, bool D32>
+__global__ void __launch_bounds__(G < 256 ? 256 : G, ln_bwd_per_sm(G)) ln_bwd_kernel(LnBwdArgs a) {
+  constexpr int BT = G < 256 ? 256 : G, NG = BT / G, W = G / 32;
+  constexpr int R = S32 || D32 || G == 1024 ? 1 : 2;  // rows a group handles between two barriers
+  constexpr bool KEEP_W = G < 1024;  // 64 registers a thread: the weight is read again for every row (L1)
+  __shared__ float2 red[2][NG][R][W];
   __shared__ float comb[NG > 1 ? NG : 1][NG > 1 ? G * 8 : 1];
-  const int g = threadIdx.x % G, grp = threadIdx.x / G, wg = g >> 5;
+  const int g = threadIdx.x % G, grp = threadIdx.x / G;
   float w[1][8], aw[8], ab[8];
-  if (a.w) ln_load_row<G, 1, VEC>(a.w, g, a.d, w);
+  auto weight = [&] {
+    if (a.w) {
+      ln_load_row<G, 1, VEC>(a.w, g, a.d, w);
+    } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (!a.w) w[0][j] = kNoWeight;
-    aw[j] = ab[j] = 0.f;
-  }
+      for (int j = 0; j < 8; ++j) w[0][j] = kNoWeight;
+    }
+  };
+  if (KEEP_W) weight();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) aw[j] = ab[j] = 0.f;
   const float inv_d = 1.f / (float)a.d;
-  int buf = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * NG * R; r0 < a.rows; r0 += (int64_t)gridDim.x * NG * R, buf ^= 1) {
-    float n[R][1][8], dy[R][1][8], ds[R][1][8], rs[R], s1[R], s2[R];
+  const int64_t step = (int64_t)gridDim.x * NG * R;
+  int64_t r = ((int64_t)blockIdx.x * NG + grp) * R;
+  LnRaw<G, VEC, S32> rs[R];
+  LnRaw<G, VEC, D32> rd[R];
+  float mean[R], rstd[R];
+  auto fetch = [&](int64_t row0) {  // a row past the end reads zeros
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      const int64_t r = r0 + grp * R + k;
-      const bool on = r < a.rows;
-      const int64_t off = r * a.d;
-      const int dd = on ? a.d : 0;  // a row past the end reads zeros
-      ln_load_row<G, 1, VEC>(a.s, a.s_dt, off, g, dd, n[k]);
-      ln_load_row<G, 1, VEC>(a.dy, a.dy_dt, off, g, dd, dy[k]);
-      if (a.dsum) ln_load_row<G, 1, VEC>(a.dsum + off, g, dd, ds[k]);
-      const float mean = on ? a.mean[r] : 0.f;
-      rs[k] = on ? a.rstd[r] : 0.f;
+      const int64_t row = row0 + k;
+      const bool on = row < a.rows;
+      rs[k].load(a.s, row * a.d, g, on ? a.d : 0);
+      rd[k].load(a.dy, row * a.d, g, on ? a.d : 0);
+      mean[k] = on ? a.mean[row] : 0.f;
+      rstd[k] = on ? a.rstd[row] : 0.f;
+    }
+  };
+  fetch(r);
+  int buf = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * NG * R; r0 < a.rows; r0 += step, r += step, buf ^= 1) {
+    if (!KEEP_W) weight();
+    float n[R][8], gv[R][1][8], rr[R], s1[R], s2[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
       s1[k] = s2[k] = 0.f;
+      rr[k] = rstd[k];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        n[k][0][j] = (n[k][0][j] - mean) * rs[k];
-        const float t = dy[k][0][j];
-        aw[j] = fmaf(t, n[k][0][j], aw[j]);
+        n[k][j] = (rs[k].get(a.s_dt, j) - mean[k]) * rr[k];
+        const float t = rd[k].get(a.dy_dt, j);
+        aw[j] = fmaf(t, n[k][j], aw[j]);
         ab[j] += t;
-        const float gv = t * w[0][j];
-        dy[k][0][j] = gv;
-        s1[k] += gv;
-        s2[k] = fmaf(gv, n[k][0][j], s2[k]);
+        gv[k][0][j] = t * w[0][j];
+        s1[k] += gv[k][0][j];
+        s2[k] = fmaf(gv[k][0][j], n[k][j], s2[k]);
       }
     }
+    float ds[1][8];  // with R = 1 (a residual comes with a float32 s); read in its place otherwise
+    if (R == 1 && a.dsum) ln_load_row<G, 1, VEC>(a.dsum + r * a.d, g, r < a.rows ? a.d : 0, ds);
+    fetch(r + step);
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       s1[k] = ln_warp_sum(s1[k]);
@@ -304,10 +367,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) ln_bwd_kernel(LnBwdArgs a) 
     if (W > 1) {
       if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int k = 0; k < R; ++k) {
-          red[buf][grp][2 * k][wg] = s1[k];
-          red[buf][grp][2 * k + 1][wg] = s2[k];
-        }
+        for (int k = 0; k < R; ++k) red[buf][grp][k][g >> 5] = make_float2(s1[k], s2[k]);
       }
       __syncthreads();
 #pragma unroll
@@ -315,24 +375,26 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) ln_bwd_kernel(LnBwdArgs a) 
         s1[k] = s2[k] = 0.f;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-          s1[k] += red[buf][grp][2 * k][i];
-          s2[k] += red[buf][grp][2 * k + 1][i];
+          const float2 t = red[buf][grp][k][i];
+          s1[k] += t.x;
+          s2[k] += t.y;
         }
       }
     }
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      const int64_t r = r0 + grp * R + k;
-      if (r >= a.rows) continue;
+      if (r + k >= a.rows) continue;
+      const int64_t off = (r + k) * a.d;
       const float c1 = s1[k] * inv_d, c2 = s2[k] * inv_d;
+      if (R > 1 && a.dsum) ln_load_row<G, 1, VEC>(a.dsum + off, g, a.d, ds);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float t = rs[k] * (dy[k][0][j] - c1 - n[k][0][j] * c2);
-        if (a.dsum) t += ds[k][0][j];
-        dy[k][0][j] = t;
+        float t = rr[k] * (gv[k][0][j] - c1 - n[k][j] * c2);
+        if (a.dsum) t += ds[0][j];
+        gv[k][0][j] = t;
       }
-      if (a.dx) ln_store_row<G, 1, VEC>(a.dx, a.dx_dt, r * a.d, g, a.d, dy[k]);
-      if (a.dres) ln_store_row<G, 1, VEC>(a.dres + r * a.d, g, a.d, dy[k]);
+      if (a.dx) ln_store_row<G, 1, VEC>(a.dx, a.dx_dt, off, g, a.d, gv[k]);
+      if (a.dres) ln_store_row<G, 1, VEC>(a.dres + off, g, a.d, gv[k]);
     }
   }
   if (!a.part) return;
@@ -419,9 +481,7 @@ int ln_bwd_blocks(int64_t rows, int d) {
   const int G = ln_bwd_group(d);
   if (G == 0) return (int)std::min<int64_t>(rows, kLnSms);
   const int ng = G < 256 ? 256 / G : 1;
-  const int per_sm = G <= 256 ? 3 : G == 512 ? 2 : 1;
-  const int64_t need = (rows + ng * kLnRows - 1) / (ng * kLnRows);
-  return (int)std::min<int64_t>(need, (int64_t)kLnSms * per_sm);
+  return (int)std::min<int64_t>((rows + ng - 1) / ng, (int64_t)kLnSms * ln_bwd_per_sm(G));
 }
 
 bool ln_al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -502,16 +562,26 @@ extern "C" int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int 
              "dp_layernorm_bwd: the workspace must be 16-byte aligned");
   const bool vec = d % 8 == 0 && ln_al16(s) && ln_al16(dy) && ln_al16(ln_w) && ln_al16(grad_sum) && ln_al16(dx) &&
                    ln_al16(grad_residual);
-  auto launch = [&](auto kern, int G) { kern<<<np, G < 256 ? 256 : G, 0, st>>>(a); };
-  switch (ln_bwd_group(d)) {
-    case 32: vec ? launch(ln_bwd_kernel<32, true>, 32) : launch(ln_bwd_kernel<32, false>, 32); break;
-    case 64: vec ? launch(ln_bwd_kernel<64, true>, 64) : launch(ln_bwd_kernel<64, false>, 64); break;
-    case 128: vec ? launch(ln_bwd_kernel<128, true>, 128) : launch(ln_bwd_kernel<128, false>, 128); break;
-    case 256: vec ? launch(ln_bwd_kernel<256, true>, 256) : launch(ln_bwd_kernel<256, false>, 256); break;
-    case 512: vec ? launch(ln_bwd_kernel<512, true>, 512) : launch(ln_bwd_kernel<512, false>, 512); break;
-    case 1024: vec ? launch(ln_bwd_kernel<1024, true>, 1024) : launch(ln_bwd_kernel<1024, false>, 1024); break;
-    default: ln_bwd_wide_kernel<<<np, 1024, 0, st>>>(a);
-  }
+  auto run = [&](auto s32, auto d32) {
+    constexpr bool S = decltype(s32)::value, D = decltype(d32)::value;
+    auto launch = [&](auto kern, int G) { kern<<<np, G < 256 ? 256 : G, 0, st>>>(a); };
+    switch (ln_bwd_group(d)) {
+      case 32: vec ? launch(ln_bwd_kernel<32, true, S, D>, 32) : launch(ln_bwd_kernel<32, false, S, D>, 32); break;
+      case 64: vec ? launch(ln_bwd_kernel<64, true, S, D>, 64) : launch(ln_bwd_kernel<64, false, S, D>, 64); break;
+      case 128: vec ? launch(ln_bwd_kernel<128, true, S, D>, 128) : launch(ln_bwd_kernel<128, false, S, D>, 128); break;
+      case 256: vec ? launch(ln_bwd_kernel<256, true, S, D>, 256) : launch(ln_bwd_kernel<256, false, S, D>, 256); break;
+      case 512: vec ? launch(ln_bwd_kernel<512, true, S, D>, 512) : launch(ln_bwd_kernel<512, false, S, D>, 512); break;
+      case 1024:
+        vec ? launch(ln_bwd_kernel<1024, true, S, D>, 1024) : launch(ln_bwd_kernel<1024, false, S, D>, 1024);
+        break;
+      default: ln_bwd_wide_kernel<<<np, 1024, 0, st>>>(a);
+    }
+  };
+  const bool s32 = s_dtype == DP_F32, d32 = dy_dtype == DP_F32;
+  if (s32)
+    d32 ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
+  else
+    d32 ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
   const int rc = check_launch("dp_layernorm_bwd");
   if (rc != DP_OK || !sums) return rc;
   return pdl_status(launch_pdl(ln_bwd_reduce_kernel, dim3((d + 31) / 32, 2), dim3(1024), 0, st, a.part, np, d, grad_w,
