@@ -29,6 +29,7 @@
 
 #include "cluster_msg.cuh"
 #include "dp_common.cuh"
+#include "tmap.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -209,14 +210,14 @@ __device__ __forceinline__ void stage(uint32_t *slot, const T *p, int st, int n)
     const uint32_t s = (uint32_t)__cvta_generic_to_shared(slot);
     if (n == kTok) {
 #pragma unroll
-      for (int i = 0; i < kTok; ++i) copy_word<4>(s + i * kThreads * 4, token(p, i, st));
+      for (int i = 0; i < kTok; ++i) copy_word<4>(s + i * 128, token(p, i, st));
     } else {
 #pragma unroll 1
       for (int i = 0; i < kTok; ++i) {
         if (i < n)
-          copy_word<4>(s + i * kThreads * 4, token(p, i, st));
+          copy_word<4>(s + i * 128, token(p, i, st));
         else
-          copy_word<0>(s + i * kThreads * 4, p);
+          copy_word<0>(s + i * 128, p);
       }
     }
   } else {
@@ -224,11 +225,31 @@ __device__ __forceinline__ void stage(uint32_t *slot, const T *p, int st, int n)
 #pragma unroll
     for (int i = 0; i < kTok; ++i) w[i] = i < n ? *reinterpret_cast<const unsigned short *>(token(p, i, st)) : 0;
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) slot[i * kThreads] = w[i];
+    for (int i = 0; i < kTok; ++i) slot[i * 32] = w[i];
   }
 }
 __device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
+
+// Bulk tensor copies of a warp's box (kTok tokens of 32 words) where the tensors allow them:
+// one instruction a box for one lane instead of a copy, its address and its bounds a word for
+// every lane.  Tokens past L and channels past D arrive as zeros and are not stored.
+struct ScanMaps {
+  CUtensorMap x, gate, out;  // out: out, or dout
+  CUtensorMap dx, dgate;
+};
+__device__ __forceinline__ void box_load(void *dst, const CUtensorMap *m, int c, int t, int b, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];\n" ::"r"(smem_u32(dst)),
+      "l"(m), "r"(c), "r"(t), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void box_store(const CUtensorMap *m, const void *src, int c, int t, int b) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(m), "r"(c),
+               "r"(t), "r"(b), "r"(smem_u32(src))
+               : "memory");
+}
 
 // The exchange of the blocks' maps inside a cluster: each block sends its map to every block
 // (st.async, counted in bytes on the receiver's mbarrier) and waits for the maps of all; there
@@ -236,20 +257,27 @@ __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group
 // warps have left the span before (__syncthreads), so whoever has received the maps of span s
 // may send those of span s + 1 into the buffer of span s - 1.  No message is left when a block
 // ends: it has received all that is sent to it.
-__device__ __forceinline__ void cluster_start(uint64_t *bar, int cs) {
-  if (cs == 1) return;
+template <typename Shared>
+__device__ __forceinline__ void scan_start(Shared &sh, int cs) {
   if (threadIdx.x == 0) {
-    mbar_init(&bar[0], 1);
-    mbar_init(&bar[1], 1);
+    mbar_init(&sh.bar[0], 1);
+    mbar_init(&sh.bar[1], 1);
+    for (int w = 0; w < kWarps; ++w) {
+      mbar_init(&sh.gate_bar[w], 1);
+      mbar_init(&sh.x_bar[w], 1);
+    }
     fence_mbar_init();
   }
-  cg::this_cluster().sync();  // the barriers exist in every block before the first message
+  if (cs > 1)
+    cg::this_cluster().sync();  // the barriers exist in every block before the first message
+  else
+    __syncthreads();
 }
 // The n = -d of a thread's tokens from the staged gates; tokens past the end keep the state.
 template <typename T, int V, int MODE, typename F>
 __device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[kTok]) {
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) nd[i] = neg_drop<T, MODE>(Lane<T, V>::get(slot[i * kThreads]));
+  for (int i = 0; i < kTok; ++i) nd[i] = neg_drop<T, MODE>(Lane<T, V>::get(slot[i * 32]));
   if (n < kTok) {
 #pragma unroll
     for (int i = 0; i < kTok; ++i)
@@ -264,7 +292,7 @@ __device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *
   Map<EXACT, F> m = {all_<F>(EXACT ? 0.f : 1.f), all_<F>(0.f)};
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {
-    m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(xw[i * kThreads]));
+    m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(xw[i * 32]));
     m.a = fma_(nd[i], m.a, m.a);
     if constexpr (EXACT) m.a = add_(m.a, nd[i]);
   }
@@ -279,11 +307,12 @@ __device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *
 
 template <typename F, bool EXACT, int NX>
 struct ScanShared {
-  uint32_t gate[kTok][kThreads];
-  uint32_t x[NX][2][kTok][kThreads];        // x, and dout in the backward pass
+  uint32_t gate[kWarps][kTok][32];
+  uint32_t x[NX][2][kWarps][kTok][32];      // x, and dout in the backward pass
   Map<EXACT, F> wmap[2][kWarps][32];        // the warps' maps
   Map<EXACT, F> bmap[2][kMaxCluster][32];   // the blocks' maps
   uint64_t bar[2];                          // one per buffer of bmap
+  uint64_t gate_bar[kWarps], x_bar[kWarps];  // the warps' bulk copies
 };
 template <typename F, bool EXACT>
 struct ScanSharedBwd : ScanShared<F, EXACT, 2> {
@@ -291,43 +320,78 @@ struct ScanSharedBwd : ScanShared<F, EXACT, 2> {
 };
 
 // ---------------------------------------------------------------- forward
-template <typename T, int V, int MODE>
-__global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanArgs a) {
+template <typename T, int V, int MODE, bool TMA>
+__global__ void __launch_bounds__(kThreads, 3)
+scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   using F = typename Lane<T, V>::F;
   constexpr bool EXACT = sizeof(T) == 4;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   auto &sh = *reinterpret_cast<ScanShared<F, EXACT, 1> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
   const int b = chain / a.tiles_c, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = (chain % a.tiles_c) * 32 * V + lane * V, cc = min(c, a.D - V);
+  const int c0 = (chain % a.tiles_c) * 32 * V, c = c0 + lane * V, cc = min(c, a.D - V);
   const bool on = c < a.D;  // D is a multiple of V
   const T *x = static_cast<const T *>(a.x) + b * a.xb + cc;
   const T *gate = static_cast<const T *>(a.gate) + b * a.gb + cc;
   T *out = static_cast<T *>(a.out) + b * a.ob + cc;
   const int span = a.cs * kTile, tiles = (a.L + kTile - 1) / kTile;
   const int off = rank * kTile + warp * kTok;
-  auto fetch = [&](int64_t base, int buf) {
-    const int64_t t0 = min(base + off, (int64_t)a.L - 1);  // byte offsets from here in 64 bits
-    const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off)));
-    stage<T, V>(&sh.gate[0][threadIdx.x], at(gate, t0, a.gt), a.gt, n);
-    stage<T, V>(&sh.x[0][buf][0][threadIdx.x], at(x, t0, a.xt), a.xt, n);
-    stage_commit();
+  uint32_t *gw = &sh.gate[warp][0][lane];
+  constexpr uint32_t kBox = sizeof(sh.gate[0]);
+  auto fetch_gate = [&](int64_t base) {
+    const int64_t t0 = min(base + off, (int64_t)a.L - 1);
+    if constexpr (TMA) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sh.gate_bar[warp], kBox);
+        box_load(gw, &maps.gate, c0, (int)min(base + off, (int64_t)a.L), b, &sh.gate_bar[warp]);
+      }
+    } else {
+      stage<T, V>(gw, at(gate, t0, a.gt), a.gt, (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off))));
+    }
   };
-  fetch(0, 0);
+  auto fetch_x = [&](int64_t base, int buf) {
+    const int64_t t0 = min(base + off, (int64_t)a.L - 1);
+    if constexpr (TMA) {
+      if (lane == 0) {
+        bulk_wait_read_all();  // the outputs staged in these slots have been read
+        mbar_arrive_expect_tx(&sh.x_bar[warp], kBox);
+        box_load(&sh.x[0][buf][warp][0][0], &maps.x, c0, (int)min(base + off, (int64_t)a.L), b, &sh.x_bar[warp]);
+      }
+    } else {
+      stage<T, V>(&sh.x[0][buf][warp][0][lane], at(x, t0, a.xt), a.xt,
+                  (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off))));
+      stage_commit();
+    }
+  };
   F h = all_<F>(0.f);
   if (on && a.h0) load_state(a.h0 + (int64_t)b * a.D + c, h);
-  cluster_start(sh.bar, a.cs);
+  scan_start(sh, a.cs);
+  fetch_gate(0);
+  fetch_x(0, 0);
   int buf = 0, phase = 0;
   bool alive = true;
   for (int64_t base = 0; base < a.L; base += span, buf ^= 1, ++phase) {
     const int64_t t0 = base + off;
     const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - t0));
-    const uint32_t *xw = &sh.x[0][buf][0][threadIdx.x];
+    uint32_t *xw = &sh.x[0][buf][warp][0][lane];
     F nd[kTok];
-    stage_wait();
-    load_gates<T, V, MODE>(&sh.gate[0][threadIdx.x], n, nd);
-    if (base + span < a.L) fetch(base + span, buf ^ 1);
+    const bool more = base + span < a.L;
+    if constexpr (TMA) {
+      if (alive) alive = mbar_wait(&sh.gate_bar[warp], phase & 1, kWaitNs);
+    } else {
+      stage_wait();
+    }
+    load_gates<T, V, MODE>(gw, n, nd);
+    if constexpr (TMA) {
+      __syncwarp();  // every lane has its gates
+      if (more) fetch_gate(base + span);
+      if (alive) alive = mbar_wait(&sh.x_bar[warp], phase & 1, kWaitNs);
+    } else if (more) {
+      fetch_gate(base + span);
+      fetch_x(base + span, buf ^ 1);
+    }
     sh.wmap[buf][warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
+    if (TMA && more) fetch_x(base + span, buf ^ 1);
     __syncthreads();
     // the block's map, by its last warp, to every block of the cluster
     if (warp == kWarps - 1) {
@@ -363,10 +427,22 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanArgs a)
     T *o = at(out, t0, a.ot);
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      in = step_<MODE>(nd[i], in, Lane<T, V>::get(xw[i * kThreads]));
-      if (i < lim) Lane<T, V>::store(token(o, i, a.ot), in);
+      in = step_<MODE>(nd[i], in, Lane<T, V>::get(xw[i * 32]));
+      if constexpr (TMA)
+        Lane<T, V>::store(reinterpret_cast<T *>(xw + i * 32), in);  // over the x that it took
+      else if (i < lim)
+        Lane<T, V>::store(token(o, i, a.ot), in);
+    }
+    if constexpr (TMA) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && n > 0) {
+        box_store(&maps.out, &sh.x[0][buf][warp][0][0], c0, (int)t0, b);
+        bulk_commit_group();
+      }
     }
   }
+  if (TMA && lane == 0) bulk_wait_all();
   if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
   if (on && rank == 0 && warp == 0) store_state(a.hL + (int64_t)b * a.D + c, h);
 }
@@ -375,15 +451,16 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanArgs a)
 // The same walk from the end of the sequence.  The states before each token come from the
 // saved state of the tile and the maps of the warps before; the gradient q that flows to
 // earlier tokens follows an affine map too, q -> a q + Q with the same a.
-template <typename T, int V, int MODE>
-__global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const ScanArgs a) {
+template <typename T, int V, int MODE, bool TMA>
+__global__ void __launch_bounds__(kThreads, 2)
+scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   using F = typename Lane<T, V>::F;
   constexpr bool EXACT = sizeof(T) == 4;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   auto &sh = *reinterpret_cast<ScanSharedBwd<F, EXACT> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
   const int b = chain / a.tiles_c, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = (chain % a.tiles_c) * 32 * V + lane * V, cc = min(c, a.D - V);
+  const int c0 = (chain % a.tiles_c) * 32 * V, c = c0 + lane * V, cc = min(c, a.D - V);
   const bool on = c < a.D;
   const T *x = static_cast<const T *>(a.x) + b * a.xb + cc;
   const T *gate = static_cast<const T *>(a.gate) + b * a.gb + cc;
@@ -392,40 +469,76 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const ScanArgs a)
   T *dg = static_cast<T *>(a.dgate) + (int64_t)b * a.L * a.D + cc;
   const int span = a.cs * kTile, tiles = (a.L + kTile - 1) / kTile;
   const int off = rank * kTile + warp * kTok;
-  auto fetch = [&](int64_t base, int buf) {
-    const int64_t t0 = min(base + off, (int64_t)a.L - 1);  // byte offsets from here in 64 bits
-    const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off)));
-    stage<T, V>(&sh.gate[0][threadIdx.x], at(gate, t0, a.gt), a.gt, n);
-    stage<T, V>(&sh.x[0][buf][0][threadIdx.x], at(x, t0, a.xt), a.xt, n);
-    stage<T, V>(&sh.x[1][buf][0][threadIdx.x], at(dout, t0, a.ot), a.ot, n);
-    stage_commit();
+  uint32_t *gw = &sh.gate[warp][0][lane];
+  constexpr uint32_t kBox = sizeof(sh.gate[0]);
+  auto fetch_gate = [&](int64_t base) {
+    const int64_t t0 = min(base + off, (int64_t)a.L - 1);
+    if constexpr (TMA) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sh.gate_bar[warp], kBox);
+        box_load(gw, &maps.gate, c0, (int)min(base + off, (int64_t)a.L), b, &sh.gate_bar[warp]);
+      }
+    } else {
+      stage<T, V>(gw, at(gate, t0, a.gt), a.gt, (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off))));
+    }
+  };
+  auto fetch_x = [&](int64_t base, int buf) {
+    const int64_t t0 = min(base + off, (int64_t)a.L - 1);
+    if constexpr (TMA) {
+      if (lane == 0) {
+        const int t = (int)min(base + off, (int64_t)a.L);
+        bulk_wait_read_all();  // the gradients staged in these slots have been read
+        mbar_arrive_expect_tx(&sh.x_bar[warp], 2 * kBox);
+        box_load(&sh.x[0][buf][warp][0][0], &maps.x, c0, t, b, &sh.x_bar[warp]);
+        box_load(&sh.x[1][buf][warp][0][0], &maps.out, c0, t, b, &sh.x_bar[warp]);
+      }
+    } else {
+      const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - (base + off)));
+      stage<T, V>(&sh.x[0][buf][warp][0][lane], at(x, t0, a.xt), a.xt, n);
+      stage<T, V>(&sh.x[1][buf][warp][0][lane], at(dout, t0, a.ot), a.ot, n);
+      stage_commit();
+    }
   };
   const int64_t last = (int64_t)(a.L - 1) / span * span;
-  fetch(last, 0);
   F q = all_<F>(0.f);
   if (on && a.dhL) load_state(a.dhL + (int64_t)b * a.D + c, q);
-  cluster_start(sh.bar, a.cs);
+  scan_start(sh, a.cs);
+  fetch_gate(last);
+  fetch_x(last, 0);
   int buf = 0, phase = 0;
   bool alive = true;
   for (int64_t base = last; base >= 0; base -= span, buf ^= 1, ++phase) {
     const int64_t t0 = base + off;
     const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - t0));
-    const uint32_t *xw = &sh.x[0][buf][0][threadIdx.x], *yw = &sh.x[1][buf][0][threadIdx.x];
+    uint32_t *xw = &sh.x[0][buf][warp][0][lane], *yw = &sh.x[1][buf][warp][0][lane];
     F in = all_<F>(0.f);
     if (on && base + rank * kTile < a.L)
       load_state(a.saved + ((int64_t)b * tiles + base / kTile + rank) * a.D + c, in);
     F nd[kTok];
-    stage_wait();
-    load_gates<T, V, MODE>(&sh.gate[0][threadIdx.x], n, nd);
-    if (base > 0) fetch(base - span, buf ^ 1);
+    const bool more = base > 0;
+    if constexpr (TMA) {
+      if (alive) alive = mbar_wait(&sh.gate_bar[warp], phase & 1, kWaitNs);
+    } else {
+      stage_wait();
+    }
+    load_gates<T, V, MODE>(gw, n, nd);
+    if constexpr (TMA) {
+      __syncwarp();  // every lane has its gates
+      if (more) fetch_gate(base - span);
+      if (alive) alive = mbar_wait(&sh.x_bar[warp], phase & 1, kWaitNs);
+    } else if (more) {
+      fetch_gate(base - span);
+      fetch_x(base - span, buf ^ 1);
+    }
     sh.wmap[buf][warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
     F Q = all_<F>(0.f);
 #pragma unroll
     for (int i = kTok - 1; i >= 0; --i) {
-      Q = add_(Q, Lane<T, V>::get(yw[i * kThreads]));
+      Q = add_(Q, Lane<T, V>::get(yw[i * 32]));
       Q = fma_(nd[i], Q, Q);
     }
     sh.wq[buf][warp][lane] = Q;
+    if (TMA && more) fetch_x(base - span, buf ^ 1);
     __syncthreads();
     if (warp == 0) {
       Map<EXACT, F> r = {sh.wmap[buf][kWarps - 1][lane].a, sh.wq[buf][kWarps - 1][lane]};
@@ -462,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const ScanArgs a)
     T *px = at(dx, t0, st), *pg = at(dg, t0, st);
     F mid = in;
 #pragma unroll
-    for (int i = 0; i < kHalf; ++i) mid = step_<MODE>(nd[i], mid, Lane<T, V>::get(xw[i * kThreads]));
+    for (int i = 0; i < kHalf; ++i) mid = step_<MODE>(nd[i], mid, Lane<T, V>::get(xw[i * 32]));
 #pragma unroll
     for (int half = 1; half >= 0; --half) {
       F hb[kHalf];  // the state before each token
@@ -470,25 +583,38 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const ScanArgs a)
 #pragma unroll
       for (int i = 1; i < kHalf; ++i)
         hb[i] = step_<MODE>(nd[half * kHalf + i - 1], hb[i - 1],
-                            Lane<T, V>::get(xw[(half * kHalf + i - 1) * kThreads]));
+                            Lane<T, V>::get(xw[(half * kHalf + i - 1) * 32]));
 #pragma unroll
       for (int k = kHalf - 1; k >= 0; --k) {
         const int i = half * kHalf + k;
-        const F p = add_(qi, Lane<T, V>::get(yw[i * kThreads]));
+        const F p = add_(qi, Lane<T, V>::get(yw[i * 32]));
         qi = fma_(nd[i], p, p);
         F ox = p, og = mul_(qi, hb[k]);
         if constexpr (MODE == DP_SCAN_SIGMOID) {
           const F d = mul_(nd[i], all_<F>(-1.f));
           ox = mul_(p, d);
-          og = mul_(mul_(qi, d), fma_(Lane<T, V>::get(xw[i * kThreads]), all_<F>(-1.f), hb[k]));
+          og = mul_(mul_(qi, d), fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k]));
         }
-        if (i < lim) {
+        if constexpr (TMA) {  // over the dout and the x that they took
+          Lane<T, V>::store(reinterpret_cast<T *>(yw + i * 32), ox);
+          Lane<T, V>::store(reinterpret_cast<T *>(xw + i * 32), og);
+        } else if (i < lim) {
           Lane<T, V>::store(token(px, i, st), ox);
           Lane<T, V>::store(token(pg, i, st), og);
         }
       }
     }
+    if constexpr (TMA) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && n > 0) {
+        box_store(&maps.dx, &sh.x[1][buf][warp][0][0], c0, (int)t0, b);
+        box_store(&maps.dgate, &sh.x[0][buf][warp][0][0], c0, (int)t0, b);
+        bulk_commit_group();
+      }
+    }
   }
+  if (TMA && lane == 0) bulk_wait_all();
   if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
   if (on && rank == 0 && warp == 0 && a.dh0) store_state(a.dh0 + (int64_t)b * a.D + c, q);
 }
@@ -521,8 +647,8 @@ int scan_cluster(int L, int64_t chains) {
   return cs;
 }
 
-template <void (*KERN)(const ScanArgs), size_t SMEM>
-int scan_launch(const ScanArgs &a, cudaStream_t st, const char *what) {
+template <void (*KERN)(const ScanArgs, const ScanMaps), size_t SMEM>
+int scan_launch(const ScanArgs &a, const ScanMaps &maps, cudaStream_t st, const char *what) {
   static thread_local bool opted[64] = {};  // shared memory and 16-block clusters: opt in once
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -544,7 +670,7 @@ int scan_launch(const ScanArgs &a, cudaStream_t st, const char *what) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, KERN, a);
+    e = cudaLaunchKernelEx(&cfg, KERN, a, maps);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -577,24 +703,58 @@ bool scan_pairs(int D, const int64_t *s, P... ptrs) {
   return true;
 }
 
+// The map of a (B, L, D) tensor with byte strides sb, st and unit channel stride: boxes of kTok
+// tokens by 32 words.  False where its alignment does not allow bulk tensor copies.
+template <typename T>
+bool scan_map(CUtensorMap *m, const void *p, const ScanArgs &a, int64_t sb, int64_t st) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (a.B == 1) sb = st * a.L;
+  if (!enc || reinterpret_cast<uintptr_t>(p) % 16 || sb % 16 || st % 16 || st < a.D * (int64_t)sizeof(T) || sb < st ||
+      sb >= (1ll << 40))
+    return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.L, (cuuint64_t)a.B};
+  const cuuint64_t strides[2] = {(cuuint64_t)st, (cuuint64_t)sb};
+  const cuuint32_t box[3] = {128 / sizeof(T), kTok, 1}, one[3] = {1, 1, 1};
+  const CUtensorMapDataType type = std::is_same_v<T, float>            ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(m, type, 3, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BWD, typename T, int V, bool TMA>
+int scan_run_mode(const ScanArgs &a, const ScanMaps &maps, int mode, cudaStream_t st, const char *what) {
+  using F = typename Lane<T, V>::F;
+  if constexpr (BWD) {
+    constexpr size_t kSmem = sizeof(ScanSharedBwd<F, sizeof(T) == 4>);
+    return mode == DP_SCAN_SIGMOID ? scan_launch<scan_bwd_kernel<T, V, DP_SCAN_SIGMOID, TMA>, kSmem>(a, maps, st, what)
+                                   : scan_launch<scan_bwd_kernel<T, V, DP_SCAN_DECAY, TMA>, kSmem>(a, maps, st, what);
+  } else {
+    constexpr size_t kSmem = sizeof(ScanShared<F, sizeof(T) == 4, 1>);
+    return mode == DP_SCAN_SIGMOID ? scan_launch<scan_fwd_kernel<T, V, DP_SCAN_SIGMOID, TMA>, kSmem>(a, maps, st, what)
+                                   : scan_launch<scan_fwd_kernel<T, V, DP_SCAN_DECAY, TMA>, kSmem>(a, maps, st, what);
+  }
+}
+
 template <bool BWD, typename T, int V>
 int scan_run(ScanArgs a, int mode, cudaStream_t st, const char *what) {
-  using F = typename Lane<T, V>::F;
   a.tiles_c = (a.D + 32 * V - 1) / (32 * V);
   a.cs = scan_cluster(a.L, (int64_t)a.B * a.tiles_c);
   a.err = device_error_ptr();
   DP_REQUIRE(a.err, DP_ERR_CUDA, std::string(what) + ": device error word unavailable");
   DP_REQUIRE((int64_t)a.B * a.tiles_c * a.cs < (1ll << 31), DP_ERR_UNSUPPORTED,
              std::string(what) + ": too many channels");
-  if constexpr (BWD) {
-    constexpr size_t kSmem = sizeof(ScanSharedBwd<F, sizeof(T) == 4>);
-    return mode == DP_SCAN_SIGMOID ? scan_launch<scan_bwd_kernel<T, V, DP_SCAN_SIGMOID>, kSmem>(a, st, what)
-                                   : scan_launch<scan_bwd_kernel<T, V, DP_SCAN_DECAY>, kSmem>(a, st, what);
-  } else {
-    constexpr size_t kSmem = sizeof(ScanShared<F, sizeof(T) == 4, 1>);
-    return mode == DP_SCAN_SIGMOID ? scan_launch<scan_fwd_kernel<T, V, DP_SCAN_SIGMOID>, kSmem>(a, st, what)
-                                   : scan_launch<scan_fwd_kernel<T, V, DP_SCAN_DECAY>, kSmem>(a, st, what);
+  ScanMaps maps = {};
+  if constexpr (sizeof(T) * V == 4) {
+    const int64_t e = sizeof(T), dense = a.D * e;
+    bool tma = scan_map<T>(&maps.x, a.x, a, a.xb * e, a.xt) && scan_map<T>(&maps.gate, a.gate, a, a.gb * e, a.gt) &&
+               scan_map<T>(&maps.out, BWD ? a.dout : a.out, a, a.ob * e, a.ot);
+    if (BWD) tma = tma && scan_map<T>(&maps.dx, a.dx, a, dense * a.L, dense) &&
+                   scan_map<T>(&maps.dgate, a.dgate, a, dense * a.L, dense);
+    if (tma) return scan_run_mode<BWD, T, V, true>(a, maps, mode, st, what);
   }
+  return scan_run_mode<BWD, T, V, false>(a, maps, mode, st, what);
 }
 
 template <bool BWD>
