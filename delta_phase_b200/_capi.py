@@ -487,7 +487,7 @@ def layernorm_bwd(s, dy, ln_w, stats, grad_sum=None, dx=None, grad_residual=None
     ws, nbytes = None, 0
     if grad_w is not None or grad_b is not None:
         nbytes = (_lib or lib()).dp_layernorm_bwd_workspace_size(rows, d)
-        ws = torch.empty(nbytes, device=s.device, dtype=torch.uint8)
+        ws = stats.new_empty(nbytes // 4)
     mean = stats.data_ptr()
     _call("dp_layernorm_bwd", idx, s.data_ptr(), dtype_code(s), dy.data_ptr(), dtype_code(dy), _addr(ln_w), mean,
           mean + 4 * rows, _addr(grad_sum), _addr(dx), DP_F32 if dx is None else dtype_code(dx),

@@ -28,6 +28,11 @@ def _rows(t):
     return t, 1, 1, 0, 0
 
 
+def _like(t):
+    """An empty contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def _check(student_logits, teacher_index, teacher_logits, temperature, weight):
     """Refuses what the kernel does not take; returns tau and the constants as it takes them."""
     if student_logits.dim() < 1 or student_logits.shape[-1] < 1:
@@ -66,12 +71,20 @@ class DistillCudaFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, index, teacher, weight = ctx.saved_tensors
-        dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        _capi.distill(*_rows(logits), index, teacher, weight, grad_loss.contiguous(), ctx.tau, dz=dz)
-        return dz, None, None, None, None
+        if torch.is_grad_enabled():  # create_graph: the gradient is not differentiable itself
+            return _backward_once(ctx, grad_loss)
+        return _backward(ctx, grad_loss)
+
+
+def _backward(ctx, grad_loss):
+    logits, index, teacher, weight = ctx.saved_tensors
+    dz = _like(logits)
+    _capi.distill(*_rows(logits), index, teacher, weight, grad_loss.contiguous(), ctx.tau, dz=dz)
+    return dz, None, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def distill_loss(student_logits, teacher_index, teacher_logits, temperature=1.0, weight=None):
@@ -105,6 +118,6 @@ def distill_loss_and_grad(student_logits, teacher_index, teacher_logits, tempera
     with torch.no_grad():
         tau, index, teacher, w = _check(student_logits, teacher_index, teacher_logits, temperature, weight)
         loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
-        dz = torch.empty(student_logits.shape, device=student_logits.device, dtype=student_logits.dtype)
+        dz = _like(student_logits)
         _capi.distill(*_rows(student_logits), index, teacher, w, None, tau, loss=loss, dz=dz)
     return loss, dz

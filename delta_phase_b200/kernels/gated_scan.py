@@ -20,6 +20,11 @@ def _mode(gate_mode):
         raise ValueError(f"gate_mode must be one of {sorted(_MODES)}, got {gate_mode!r}") from None
 
 
+def _like(t):
+    """An empty contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def _unit(t):
     """t with unit channel stride (a copy only where it has none)."""
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
@@ -43,12 +48,12 @@ def _check_state(state, B, D, name):
 def _forward(x, gate, initial_state, mode, keep):
     B, L, D = x.shape
     h0 = None if initial_state is None else initial_state.contiguous()
-    out = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
-    final = torch.empty(B, D, device=x.device, dtype=torch.float32)
+    out = _like(x)
+    final = torch.empty((B, D), device=x.device, dtype=torch.float32)
     saved = None
     if keep:
         tile = _capi.scan_tile()
-        saved = torch.empty(B, (L + tile - 1) // tile, D, device=x.device, dtype=torch.float32)
+        saved = final.new_empty((B, (L + tile - 1) // tile, D))
     _capi.scan_fwd(_unit(x), _unit(gate), mode, h0, out, final, saved)
     return out, final, saved
 
@@ -66,19 +71,26 @@ class GatedScanCudaFunction(torch.autograd.Function):
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out, grad_final):
-        x, gate, saved = ctx.saved_tensors
-        if grad_out is None and grad_final is None:
-            return None, None, None, None
-        B, L, D = x.shape
-        dx = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
-        dg = torch.empty_like(dx)
-        go = torch.zeros_like(dx) if grad_out is None else _unit(grad_out)
-        gf = None if grad_final is None else grad_final.contiguous()
-        dh = torch.empty(B, D, device=x.device, dtype=torch.float32) if ctx.needs_input_grad[2] else None
-        _capi.scan_bwd(_unit(x), _unit(gate), go, ctx.mode, saved, gf, dx, dg, dh)
-        return (dx if ctx.needs_input_grad[0] else None, dg if ctx.needs_input_grad[1] else None, dh, None)
+        if torch.is_grad_enabled():  # create_graph: the gradients are not differentiable themselves
+            return _backward_once(ctx, grad_out, grad_final)
+        return _backward(ctx, grad_out, grad_final)
+
+
+def _backward(ctx, grad_out, grad_final):
+    x, gate, saved = ctx.saved_tensors
+    if grad_out is None and grad_final is None:
+        return None, None, None, None
+    need_x, need_gate, need_state, _ = ctx.needs_input_grad
+    dx, dg = _like(x), _like(x)
+    go = torch.zeros_like(dx) if grad_out is None else _unit(grad_out)
+    gf = None if grad_final is None else grad_final.contiguous()
+    dh = saved.new_empty((x.shape[0], x.shape[2])) if need_state else None
+    _capi.scan_bwd(_unit(x), _unit(gate), go, ctx.mode, saved, gf, dx, dg, dh)
+    return dx if need_x else None, dg if need_gate else None, dh, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
@@ -114,13 +126,13 @@ def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None)
     B, D = x.shape
     _check_state(state, B, D, "state")
     if state_out is None:
-        state_out = torch.empty(B, D, device=x.device, dtype=torch.float32)
+        state_out = _like(state)
     else:
         _check_state(state_out, B, D, "state_out")
         if not state_out.is_contiguous():
             raise ValueError("state_out must be contiguous")
     if out is None:
-        out = torch.empty(B, D, device=x.device, dtype=x.dtype)
+        out = _like(x)
     elif out.dtype != x.dtype or out.shape != x.shape or (D > 1 and out.stride(1) != 1):
         raise ValueError("out must be a (B, D) tensor of x's dtype with unit channel stride")
     _capi.scan_step(state.contiguous(), state_out, _unit(x), _unit(gate), mode, out)

@@ -31,12 +31,12 @@ class LayerNormCudaFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual, out_dtype):
         xc = _dense(x)
-        y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+        y = torch.empty_like(xc) if out_dtype == x.dtype else torch.empty_like(xc, dtype=out_dtype)
         stats = torch.empty((2, x.numel() // x.shape[-1]), device=x.device, dtype=torch.float32)
         res = s = None
         if residual is not None:
             res = _dense(residual)
-            s = torch.empty(x.shape, device=x.device, dtype=torch.float32)
+            s = torch.empty_like(res)
         _capi.layernorm_fwd(xc, _f32(weight), _f32(bias), eps, y, stats, residual=res, sum_out=s)
         ctx.set_materialize_grads(False)
         ctx.x_dtype = x.dtype
@@ -46,40 +46,49 @@ class LayerNormCudaFunction(torch.autograd.Function):
         return y if s is None else (y, s)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_s=None):
-        if grad_y is None and grad_s is None:
-            return None, None, None, None, None, None
-        s, weight, stats = ctx.saved_tensors
-        need_x, need_w, need_b, _, need_res, _ = ctx.needs_input_grad
-        gw = gb = dx = dres = None
-        if grad_y is None:  # s alone was used
-            d = s.shape[-1]
-            gw = torch.zeros(d, device=s.device) if need_w else None
-            gb = torch.zeros(d, device=s.device) if need_b else None
-            dx = grad_s.to(ctx.x_dtype) if need_x else None
-            dres = grad_s if need_res else None
-        else:
-            if need_w:
-                gw = torch.empty(s.shape[-1], device=s.device, dtype=torch.float32)
-            if need_b:
-                gb = torch.empty(s.shape[-1], device=s.device, dtype=torch.float32)
-            if need_res:
-                dres = torch.empty_like(s)
-            # a float32 x has the residual's gradient
-            shared = need_x and need_res and ctx.x_dtype == torch.float32
-            if need_x and not shared:
-                dx = torch.empty_like(s, dtype=ctx.x_dtype)
-            _capi.layernorm_bwd(s, _dense(grad_y), _f32(weight), stats,
-                                grad_sum=None if grad_s is None else _dense(grad_s), dx=dx, grad_residual=dres,
-                                grad_w=gw, grad_b=gb)
-            if shared:
-                dx = dres
-        if gw is not None and weight.dtype != torch.float32:
-            gw = gw.to(weight.dtype)
-        if gb is not None and ctx.bias_dtype != torch.float32:
-            gb = gb.to(ctx.bias_dtype)
-        return dx, gw, gb, None, dres, None
+        if torch.is_grad_enabled():  # create_graph: the gradients are not differentiable themselves
+            return _backward_once(ctx, grad_y, grad_s)
+        return _backward(ctx, grad_y, grad_s)
+
+
+def _backward(ctx, grad_y, grad_s):
+    if grad_y is None and grad_s is None:
+        return None, None, None, None, None, None
+    s, weight, stats = ctx.saved_tensors
+    need_x, need_w, need_b, _, need_res, _ = ctx.needs_input_grad
+    gw = gb = dx = dres = None
+    if need_w:
+        gw = stats.new_empty(s.shape[-1])
+    if need_b:
+        gb = stats.new_empty(s.shape[-1])
+    if grad_y is None:  # s alone was used
+        if need_w:
+            gw.zero_()
+        if need_b:
+            gb.zero_()
+        dx = grad_s.to(ctx.x_dtype) if need_x else None
+        dres = grad_s if need_res else None
+    else:
+        if need_res:
+            dres = torch.empty_like(s)
+        # a float32 x has the residual's gradient
+        shared = need_x and need_res and ctx.x_dtype == torch.float32
+        if need_x and not shared:
+            dx = torch.empty_like(s) if s.dtype == ctx.x_dtype else torch.empty_like(s, dtype=ctx.x_dtype)
+        _capi.layernorm_bwd(s, _dense(grad_y), _f32(weight), stats,
+                            grad_sum=None if grad_s is None else _dense(grad_s), dx=dx, grad_residual=dres,
+                            grad_w=gw, grad_b=gb)
+        if shared:
+            dx = dres
+    if gw is not None and weight.dtype != torch.float32:
+        gw = gw.to(weight.dtype)
+    if gb is not None and ctx.bias_dtype != torch.float32:
+        gb = gb.to(ctx.bias_dtype)
+    return dx, gw, gb, None, dres, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, out_dtype=None):
