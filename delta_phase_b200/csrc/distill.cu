@@ -4,11 +4,20 @@
 //   dz_v = grad weight tau (q_v - sum_{k: i_k = v} p_k)
 // for the head of DeltaPhaseModel (delta_phase/model.py:60-66, 101).
 //
-// The logits are by far the largest tensors of a training step and HBM bounds the pass:
-// a row is read once into the registers of a block (or of a cluster of blocks, for wide
-// rows and for few rows), its maximum and sum of exponentials are reduced there, and the
-// gradient is written from the same registers, so loss and gradient together move 2 V
-// values a row.  Statistics and products are float32; the gradient is rounded once.
+// The logits are by far the largest tensors of a training step, and HBM bounds the pass: a row
+// (a block's slice of it, for rows above 64 KB and for few rows; the slices meet in one exchange
+// over distributed shared memory) is read once, into shared memory; its maximum, its sum of
+// exponentials and the gradient come from there, so loss and gradient move 2 V values a row.
+// The exponentials are taken twice, not kept: kept in float32 they fill the registers, one block
+// an SM remains, and its phases (load, reduce, write) follow one another instead of overlapping
+// with those of two others (582 against 406 us below).  What a block does per row besides its
+// 64 elements a thread is kept short: one exchange of maxima and sums, teacher entries by the
+// warps that have some.  Statistics and products are float32; the gradient is rounded once.
+//
+// Measured (B200, K = 64, copy rate 6540 GB/s): loss and gradient of 16384 x 32768 bf16 logits
+// 405 us (5.3 TB/s, 81% of the copy rate), 2048 rows 64 us (64%; 4.6 waves of blocks); loss alone
+// 235 us (70%: the exponentials and the reductions show); 4096 x 32768 float32 213 us (77%);
+// 4096 x 32767 bf16 (rows off the 16-byte grid) 118 us (69%).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -21,7 +30,6 @@
 namespace cg = cooperative_groups;
 
 namespace dp {
-
 namespace {
 
 using namespace ptx;
@@ -40,9 +48,9 @@ struct DistillArgs {
   void *dz;
   int64_t rows, sb, st;
   int index64, teacher_dt, L, V, K, cs;
-  int group_smem;  // bytes of shared memory of a group
+  int group_smem;   // bytes of shared memory of a group
   int stage_bytes;  // the part of it that holds the group's vectors
-  int regular;  // one row stride, rows (dz's too) of whole vectors on 16 bytes
+  int regular;      // one row stride, rows (dz's too) of whole vectors on 16 bytes
   float tau, inv_tau, c;  // c = log2(e) / tau
 };
 
@@ -257,15 +265,16 @@ struct BlockGroup {
   Part *parts;
   __device__ __forceinline__ void sync() const { __syncthreads(); }
 };
-// The i-th vector of a thread, -inf past the end: out of the row's copy in shared memory, or
-// out of the registers it was read into.
+
 template <typename T>
-__device__ __forceinline__ uint4 di_nothing() {
+__device__ __forceinline__ uint4 di_nothing() {  // a vector of -inf
   uint4 v;
 #pragma unroll
   for (int k = 0; k < Vec<T>::E / 2; ++k) Vec<T>::set(v, k, make_float2(-INFINITY, -INFINITY));
   return v;
 }
+// The i-th vector of a thread, -inf past the end: out of the row's copy in shared memory, or
+// out of the registers it was read into.
 struct FromShared {
   uint32_t v;  // of this thread
   int n;
@@ -285,8 +294,8 @@ struct FromRegisters {
 };
 
 // Loss and gradient of a row (ze: the thread's single element, -inf if none; first: entry
-// `tid`, read ahead; zt: the student's logit there).  `loaded` runs once all of the group have
-// read their vectors; `join` makes the (maximum, sum) of the cluster out of this block's.
+// `tid`, read ahead; zt: the student's logit there).  `join` makes the (maximum, sum) of the
+// cluster out of this block's.
 // KEEP: the exponentials, against the warp's maximum, are kept in float32 registers and the
 // gradient is their multiple; otherwise the gradient's pass computes them again.
 template <typename T, int NV, bool KEEP, class G, class Src, class Join>
@@ -484,9 +493,10 @@ __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const R
 // block; NV vectors per thread.  STAGE: the vectors wait in shared memory, each copied there
 // (cp.async) by the thread that reads it, twice, so that three times as many threads fit on an
 // SM as hold their exponentials in registers: many rows, HBM counts.  Otherwise they are read
-// into registers: few rows, latency counts.
+// into registers: few rows, latency counts (16 x 32768 bf16, loss: 4 blocks a row, 15 us a call
+// with 12 us of it on the host).
 template <typename T, int NV, bool WARP, bool STAGE>
-__global__ void __launch_bounds__(WARP ? 32 * kDiWarpRows : kDiMaxThreads, (STAGE ? 1536 : 1024) / (WARP ? 32 * kDiWarpRows : kDiMaxThreads))
+__global__ void __launch_bounds__(WARP ? 32 * kDiWarpRows : kDiMaxThreads, WARP ? 8 : STAGE ? 3 : 2)
 distill_kernel(const DistillArgs a) {
   __shared__ Part parts[kDiMaxThreads / 32];
   __shared__ float2 cpart[kDiMaxCluster];
@@ -543,11 +553,17 @@ distill_kernel(const DistillArgs a) {
 template <typename T, int NV, bool WARP, bool STAGE>
 int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, cudaStream_t st) {
   auto kern = distill_kernel<T, NV, WARP, STAGE>;
-  cudaError_t e = cudaSuccess;
-  if (smem > 40 * 1024)  // beside the static part
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && a.cs > 8)  // a non-portable size: opt in
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  // more than 48 KB of shared memory and 16-block clusters (a non-portable size): opt in once
+  static thread_local bool opted[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !opted[dev])) {
+    constexpr int groups = WARP ? kDiWarpRows : 1, n = WARP ? 32 : kDiMaxThreads;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             groups * ((STAGE ? n * NV * 16 : 0) + di_smem(kDiMaxK)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) opted[dev] = true;
+  }
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -591,7 +607,10 @@ int distill_launch(DistillArgs a, cudaStream_t st) {
   const int most = kDiMaxThreads * kDiMaxVec;
   while (a.cs < kDiMaxCluster && (int64_t)a.cs * most < nvec) a.cs *= 2;
   DP_REQUIRE((int64_t)a.cs * most >= nvec, DP_ERR_UNSUPPORTED, "dp_distill: V too large");
-  // few rows: split each over more blocks, down to a vector per thread
+  // few rows: split each over more blocks, down to a vector per thread (one row of 131072
+  // float32 logits: 16 blocks); enough rows to fill the GPU are split only as far as they must
+  // (16384 x 32768 bf16, loss and gradient: 1 / 2 / 4 blocks a row 498 / 558 / 591 us, measured
+  // on the version before this one)
   while (a.cs < kDiMaxCluster && a.rows * a.cs < kDiSms && nvec / a.cs >= 2 * kDiMaxThreads) a.cs *= 2;
   const int per = (nvec + a.cs - 1) / a.cs;
   const int64_t blocks = a.rows * a.cs;

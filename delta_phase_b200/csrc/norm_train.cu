@@ -5,8 +5,18 @@
 //   dp_layernorm_bwd : n = (s - m) r, g = w dy,
 //                      ds = r (g - mean(g) - n mean(g n)) (+ the gradient that reaches s),
 //                      dw = sum_rows dy n, db = sum_rows dy
-// All statistics, products and sums are float32; a row is held in registers between its
-// read and its write, so each pass reads and writes every tensor once and HBM bounds it.
+// All statistics, products and sums are float32.  HBM bounds both passes: a row is held in
+// registers between its read and its write, so each pass moves every tensor once.
+//   forward : a warp a row up to d = 1024 (no barrier), a block of 256 up to 8192; parameters in
+//             pieces from L1, so that 24 warps an SM fit their rows into registers.
+//   backward: eight columns a thread, so that dw and db of a thread's columns stay in registers
+//             while its block walks over the rows; the next rows are loaded meanwhile.  Two
+//             resident blocks of 256 threads without spills beat three with (183 against 222 us
+//             below); 16-bit rows, half as large, go two at a time (90 against 132 us).
+// Measured (B200, copy rate 6540 GB/s), forward and backward: 65536 x 1024 bf16 with the float32
+// residual 138 us (89% of the copy rate) and 183 us (90%), without 78 us (52%) and 90 us (69%);
+// 16384 x 2048 float32 with residual 91 us (91%) and 109 us (94%); 8192 x 4096 bf16 44 us (47%) and
+// 56 us (55%); 32768 x 1000 bf16 with residual 76 us (79%) and 100 us (80%).
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -475,8 +485,8 @@ int ln_bwd_group(int d) {
   return 0;
 }
 
-// Blocks of the backward kernel (and partial rows in its workspace): two waves' worth of
-// 256-thread blocks, fewer when there are fewer rows.
+// Blocks of the backward kernel (and partial rows in its workspace): those that are resident at
+// once, fewer when there are fewer rows.
 int ln_bwd_blocks(int64_t rows, int d) {
   const int G = ln_bwd_group(d);
   if (G == 0) return (int)std::min<int64_t>(rows, kLnSms);

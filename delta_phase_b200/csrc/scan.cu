@@ -15,12 +15,21 @@
 // float32 arithmetic, or one float), a warp kTok consecutive tokens of its 32 words, a block
 // kWarps warps (kTile tokens), and a thread-block cluster up to 16 consecutive tiles of one
 // sequence.  Each warp reduces its tokens to an affine map of the state, the maps are combined
-// through shared memory inside the block and through distributed shared memory inside the
-// cluster (one cluster barrier per span), and each warp then runs the recurrence over its
-// tokens again from the exact state that reaches it: every input is read from HBM once and
-// the order of all sums is fixed.  A cluster walks over a long sequence in steps of its span;
-// the next span's words are on their way to shared memory (cp.async) while one is computed.
-// Every thread copies the words it reads itself, so staging needs no barrier.
+// through shared memory inside the block and by messages inside the cluster, and each warp then
+// runs the recurrence over its tokens again from the exact state that reaches it: every input
+// is read from HBM once and the order of all sums is fixed.  A cluster walks over a long
+// sequence in steps of its span; the next span is on its way to shared memory while one is
+// computed, and the outputs leave from the slots of the inputs they replace: by bulk tensor
+// copies of a warp's box (kTok tokens of 32 words) where the tensors' alignment allows them,
+// else by cp.async of single words and plain stores.  No warp waits for another one's copies.
+//
+// HBM bounds it where enough channels and tokens run at once (about 1.7 blocks an SM), the chain
+// of spans (2.5 to 3 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
+// and backward: 2 x 32768 x 1024 bf16 97 us (64% of the copy rate) and 130 us (79%), 8 x 8192 x
+// 1024 bf16 89 us (70%) and 123 us (83%), 4 x 8192 x 512 float32 52 us (60%) and 64 us (80%),
+// 1 x 65536 x 256 bf16 (4 chains) 78 us (20%) and 97 us (27%).  With single words instead of boxes
+// the first was 144 and 216 us (address arithmetic: 1048 instead of 769 instructions a warp and
+// span), with a cluster barrier instead of messages 179 and 321 us (its fence).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -637,10 +646,10 @@ scan_step_kernel(const float *state, float *state_out, const T *x, const T *gate
 }
 
 // Blocks of a cluster.  Smaller clusters wait less for one another, but a sequence's chain of
-// spans has to be split until about 1.7 blocks an SM run.  Measured (us forward, backward at
-// 2 / 4 / 8 / 16 blocks): 32 chains x 32768 tokens bf16 312, 443 / 168, 240 / 144, 217 /
-// 164, 265; 128 chains x 8192 tokens 129, 201 / 129, 213 / 134, 220 / 152, 261; 4 chains x
-// 65536 tokens 583, 842 / 308, 437 / 164, 232 / 95, 131.
+// spans has to be split until about 1.7 blocks an SM run; sizes that are no power of two pack
+// badly into the GPU's processor clusters.  Measured (us forward, backward at 2 / 4 / 8 / 9 / 16
+// blocks): 32 chains x 32768 tokens bf16 236, 308 / 123, 160 / 97, 130 / 115, 183 / 117, 175;
+// 128 chains x 8192 tokens bf16 89, 123 / 90, 133 / 96, 144 / 101, 156 / 95, 144.
 int scan_cluster(int L, int64_t chains) {
   int cs = 1;
   while (cs < kMaxCluster && cs * kTile < L && chains * cs < 256) cs *= 2;

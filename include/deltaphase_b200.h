@@ -396,6 +396,8 @@ DP_API int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int dy_d
  *   strides[6]   : {sb, st} of x, gate, out
  * The state is float32 throughout; the order of all sums is fixed by L.  Any L >= 0.  The
  * kernels compute h - (1 - a) h for a h: a state that has become infinite continues as NaN.
+ * Made for 0 <= a <= 1; larger a are computed too, but a product of a over 128 tokens that
+ * overflows float32 may turn a zero state into NaN.  Token strides up to 2^28 elements.
  */
 enum dp_scan_mode { DP_SCAN_DECAY = 0, DP_SCAN_SIGMOID = 1 };
 DP_API int dp_scan_tile(void);

@@ -790,3 +790,50 @@ def test_saved_inputs_changed_in_place_are_noticed():
     y.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         out.sum().backward()
+
+
+# ---------------------------------------------------------------- sizes past 32 bits
+def test_layer_norm_offsets_past_32_bits():
+    rows, d = (1 << 31) // 1024 + 5000, 1024
+    x = torch.empty(rows, d, device="cuda", dtype=BF16).normal_(generator=gen(60)).requires_grad_(True)
+    w = torch.ones(d, device="cuda", requires_grad=True)
+    y = layer_norm(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), y.detach())
+    tail = x.detach()[-300:].clone().requires_grad_(True)
+    yt = layer_norm(tail, w)
+    dxt, = torch.autograd.grad(yt, tail, yt.detach())
+    assert torch.equal(y[-300:], yt) and torch.equal(dx[-300:], dxt)
+    # dw = sum of y^2 over the rows where w = 1: d on average over the columns
+    assert abs(float(dw.mean()) / rows - 1) < 1e-2
+
+
+def test_scan_offsets_past_32_bits():
+    """2.2e9 elements: the end of the sequence from the state before it, forward and backward."""
+    B, L, D, cut = 1, (1 << 31) // 4096 + 20000, 4096, 4096
+    x = torch.empty(B, L, D, device="cuda", dtype=BF16).normal_(generator=gen(61))
+    gate = torch.full((1, 1, D), -0.05, device="cuda", dtype=BF16).expand(B, L, D)
+    leaf = x.requires_grad_(True)
+    out, fin = gated_scan(leaf, gate)
+    dx, = torch.autograd.grad((out, fin), leaf, (leaf.detach(), fin.detach()))
+    with torch.no_grad():
+        _, before = gated_scan(x[:, :-cut], gate[:, :-cut])
+    tail = x.detach()[:, -cut:].clone().requires_grad_(True)
+    out_t, fin_t = gated_scan(tail, gate[:, -cut:], before)
+    dx_t, = torch.autograd.grad((out_t, fin_t), tail, (tail.detach(), fin_t.detach()))
+    # both round nearly the same values: each by half a bf16 step, 2^-8 of the value, together 2^-7
+    # (the larger of the two, hence the second term); the recurrences add 80 U x 20 tokens x 30 = 3e-3
+    for a, b in ((out[:, -cut:], out_t), (dx[:, -cut:], dx_t)):
+        err = (a.float() - b.float()).abs()
+        assert bool((err <= 2.0 ** -7 * b.float().abs() + 4e-3).all())
+    assert float((fin.detach() - fin_t.detach()).abs().max()) < 4e-3
+
+
+def test_distill_offsets_past_32_bits():
+    N, V, K = (1 << 31) // 32768 + 700, 32768, 8
+    z = torch.empty(N, V, device="cuda", dtype=BF16).normal_(generator=gen(62))
+    index = torch.randint(0, V, (N, K), generator=gen(63), device="cuda")
+    teacher = torch.randn(N, K, generator=gen(64), device="cuda")
+    loss, dz = dp.distill_loss_and_grad(z, index, teacher)
+    rl, el, rd, ed = distill_ref(z[-64:], index[-64:], teacher[-64:], 1.0, None)
+    check(loss[-64:], rl, el, "loss")
+    check(dz[-64:], rd, ed, "dz")
