@@ -482,8 +482,7 @@ def layernorm_bwd(s, dy, ln_w, stats, grad_sum=None, dx=None, grad_residual=None
     """dp_layernorm_bwd: the gradients asked for (tensors that are not None) of layernorm_fwd;
     s is its sum_out, or x where there was no residual."""
     idx = _device_index(s, dy, ln_w, stats, grad_sum, dx, grad_residual, grad_w, grad_b)
-    d = s.shape[-1]
-    rows = s.numel() // d
+    rows, d = stats.shape[1], s.shape[-1]
     ws, nbytes = None, 0
     if grad_w is not None or grad_b is not None:
         nbytes = (_lib or lib()).dp_layernorm_bwd_workspace_size(rows, d)

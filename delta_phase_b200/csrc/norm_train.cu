@@ -14,7 +14,7 @@
 //             resident blocks of 256 threads without spills beat three with (183 against 222 us
 //             below); 16-bit rows, half as large, go two at a time (90 against 132 us).
 // Measured (B200, copy rate 6540 GB/s), forward and backward: 65536 x 1024 bf16 with the float32
-// residual 138 us (89% of the copy rate) and 183 us (90%), without 78 us (52%) and 90 us (69%);
+// residual 132 us (94% of the copy rate) and 183 us (90%), without 78 us (52%) and 90 us (69%);
 // 16384 x 2048 float32 with residual 91 us (91%) and 109 us (94%); 8192 x 4096 bf16 44 us (47%) and
 // 56 us (55%); 32768 x 1000 bf16 with residual 76 us (79%) and 100 us (80%).
 #include <algorithm>
@@ -167,11 +167,11 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G, G == 32 ? 6 : 2) ln_fwd_ker
   const int64_t r = (int64_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
   if (r >= a.rows) return;  // a whole warp (G = 32) or never (one row per block)
   const int64_t off = r * a.d;
-  float v[NV][8];
+  float v[NV][8], t[NV][8];
+  // the residual first: x is converted, and waited for, where it is loaded (132 against 138 us)
+  if (a.res) ln_load_row<G, NV, VEC>(a.res + off, g, a.d, t);
   ln_load_row<G, NV, VEC>(a.x, a.x_dt, off, g, a.d, v);
   if (a.res) {
-    float t[NV][8];
-    ln_load_row<G, NV, VEC>(a.res + off, g, a.d, t);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll

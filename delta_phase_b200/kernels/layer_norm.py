@@ -38,12 +38,14 @@ class LayerNormCudaFunction(torch.autograd.Function):
             res = _dense(residual)
             s = torch.empty_like(res)
         _capi.layernorm_fwd(xc, _f32(weight), _f32(bias), eps, y, stats, residual=res, sum_out=s)
-        ctx.set_materialize_grads(False)
-        ctx.x_dtype = x.dtype
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.dtypes = x.dtype, None if bias is None else bias.dtype
         # x itself where it is contiguous, so that a change of x before the backward pass is noticed
-        ctx.save_for_backward(xc if s is None else s, weight, stats)
-        return y if s is None else (y, s)
+        if s is None:
+            ctx.save_for_backward(xc, weight, stats)
+            return y
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(s, weight, stats)
+        return y, s
 
     @staticmethod
     def backward(ctx, grad_y, grad_s=None):
@@ -56,6 +58,7 @@ def _backward(ctx, grad_y, grad_s):
     if grad_y is None and grad_s is None:
         return None, None, None, None, None, None
     s, weight, stats = ctx.saved_tensors
+    x_dtype, bias_dtype = ctx.dtypes
     need_x, need_w, need_b, _, need_res, _ = ctx.needs_input_grad
     gw = gb = dx = dres = None
     if need_w:
@@ -67,24 +70,26 @@ def _backward(ctx, grad_y, grad_s):
             gw.zero_()
         if need_b:
             gb.zero_()
-        dx = grad_s.to(ctx.x_dtype) if need_x else None
+        dx = grad_s.to(x_dtype) if need_x else None
         dres = grad_s if need_res else None
     else:
         if need_res:
             dres = torch.empty_like(s)
         # a float32 x has the residual's gradient
-        shared = need_x and need_res and ctx.x_dtype == torch.float32
+        shared = need_x and need_res and x_dtype == torch.float32
         if need_x and not shared:
-            dx = torch.empty_like(s) if s.dtype == ctx.x_dtype else torch.empty_like(s, dtype=ctx.x_dtype)
-        _capi.layernorm_bwd(s, _dense(grad_y), _f32(weight), stats,
-                            grad_sum=None if grad_s is None else _dense(grad_s), dx=dx, grad_residual=dres,
-                            grad_w=gw, grad_b=gb)
+            dx = torch.empty_like(s) if s.dtype == x_dtype else torch.empty_like(s, dtype=x_dtype)
+        if not grad_y.is_contiguous():
+            grad_y = grad_y.contiguous()
+        if grad_s is not None and not grad_s.is_contiguous():
+            grad_s = grad_s.contiguous()
+        _capi.layernorm_bwd(s, grad_y, _f32(weight), stats, grad_s, dx, dres, gw, gb)
         if shared:
             dx = dres
     if gw is not None and weight.dtype != torch.float32:
         gw = gw.to(weight.dtype)
-    if gb is not None and ctx.bias_dtype != torch.float32:
-        gb = gb.to(ctx.bias_dtype)
+    if gb is not None and bias_dtype != torch.float32:
+        gb = gb.to(bias_dtype)
     return dx, gw, gb, None, dres, None
 
 
