@@ -3,7 +3,8 @@
 Drop-in for the hot-path API of mcarbonell/delta-phase v1.3.0 (``delta_phase``):
 the chunkwise complex delta-rule core, its decode step, the LaplacePhaseCore and the
 spectral Lerp FFN, on hand-written CUDA kernels behind the C ABI of
-``include/deltaphase_b200.h``.
+``include/deltaphase_b200.h``; and training-step operators beside them (layer norm, gated
+linear recurrence, distillation loss, each with its backward pass).
 """
 from .kernels import (
     DeltaPhaseCudaFunction,
