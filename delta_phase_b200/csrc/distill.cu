@@ -645,7 +645,8 @@ extern "C" int dp_distill(const void *z, int z_dtype, const void *index, int ind
   DP_REQUIRE(rows * kDiMaxCluster < (1ll << 31), DP_ERR_UNSUPPORTED, "dp_distill: too many rows");
   DistillArgs a = {};
   a.z = z, a.sb = strides[0], a.st = strides[1], a.index = index, a.index64 = index_bytes == 8, a.teacher = teacher;
-  a.teacher_dt = teacher_dtype, a.weight = weight, a.grad = grad, a.tau = tau, a.inv_tau = 1.f / tau, a.c = 1.4426950408889634f / tau, a.loss = loss, a.dz = dz;
+  a.teacher_dt = teacher_dtype, a.weight = weight, a.grad = grad, a.loss = loss, a.dz = dz;
+  a.tau = tau, a.inv_tau = 1.f / tau, a.c = 1.4426950408889634f / tau;
   a.rows = rows, a.L = L, a.V = V, a.K = K;
   cudaStream_t st = as_stream(stream);
   return dispatch_dtype(z_dtype, [&](auto t) { return distill_launch<decltype(t)>(a, st); });

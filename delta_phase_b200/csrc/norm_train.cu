@@ -566,8 +566,8 @@ extern "C" int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int 
   const bool sums = grad_w || grad_b;
   DP_REQUIRE(!sums || (workspace && workspace_bytes >= dp_layernorm_bwd_workspace_size(rows, d)), DP_ERR_WORKSPACE,
              "dp_layernorm_bwd: workspace too small");
-  LnBwdArgs a{s,  dy,      ln_w,    mean,  rstd, grad_sum, dx, grad_residual, sums ? static_cast<float *>(workspace) : nullptr,
-              s_dtype, dy_dtype, dx_dtype, d, rows};
+  float *part = sums ? static_cast<float *>(workspace) : nullptr;
+  LnBwdArgs a{s, dy, ln_w, mean, rstd, grad_sum, dx, grad_residual, part, s_dtype, dy_dtype, dx_dtype, d, rows};
   DP_REQUIRE(!sums || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, DP_ERR_MISALIGNED,
              "dp_layernorm_bwd: the workspace must be 16-byte aligned");
   const bool vec = d % 8 == 0 && ln_al16(s) && ln_al16(dy) && ln_al16(ln_w) && ln_al16(grad_sum) && ln_al16(dx) &&

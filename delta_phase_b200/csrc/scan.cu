@@ -799,7 +799,8 @@ extern "C" int dp_scan_fwd(const void *x, const void *gate, int dtype, int mode,
   ScanArgs a = {};
   a.x = x, a.gate = gate, a.h0 = state_in, a.hL = state_out, a.saved = saved, a.out = out;
   a.B = B, a.L = L, a.D = D;
-  DP_REQUIRE(scan_strides(a, strides, (int)dtype_size(dtype)), DP_ERR_UNSUPPORTED, "dp_scan_fwd: token stride too large");
+  DP_REQUIRE(scan_strides(a, strides, (int)dtype_size(dtype)), DP_ERR_UNSUPPORTED,
+             "dp_scan_fwd: token stride too large");
   return scan_dispatch<false>(a, dtype, mode, scan_pairs(D, strides, x, gate, (const void *)out), st, "dp_scan_fwd");
 }
 
@@ -826,7 +827,8 @@ extern "C" int dp_scan_bwd(const void *x, const void *gate, const void *grad_out
   a.x = x, a.gate = gate, a.dout = grad_out, a.saved = const_cast<float *>(saved), a.dhL = grad_state_out;
   a.dx = grad_x, a.dgate = grad_gate, a.dh0 = grad_state_in;
   a.B = B, a.L = L, a.D = D;
-  DP_REQUIRE(scan_strides(a, strides, (int)dtype_size(dtype)), DP_ERR_UNSUPPORTED, "dp_scan_bwd: token stride too large");
+  DP_REQUIRE(scan_strides(a, strides, (int)dtype_size(dtype)), DP_ERR_UNSUPPORTED,
+             "dp_scan_bwd: token stride too large");
   return scan_dispatch<true>(a, dtype, mode,
                              scan_pairs(D, strides, x, gate, grad_out, (const void *)grad_x, (const void *)grad_gate),
                              st, "dp_scan_bwd");

@@ -437,7 +437,8 @@ def distill_ref(z, index, teacher, tau, weight, grad=None):
     mag = torch.where(p > 0, p * (logp.abs() + lq.abs() + 4), 0.0).sum(-1)
     xk = (t - t.amax(-1, keepdim=True)).abs().clamp(max=200)
     e_p = p * (2 * U * (3 + 1.2 * xk) + 96 * U)
-    e_loss = torch.where(on, w.abs() * tau * tau * (e_lse + 16 * U * mag + (e_p * (logp - lq).abs().nan_to_num(0, 0, 0)).sum(-1)), 0.0)
+    e_ent = (e_p * (logp - lq).abs().nan_to_num(0, 0, 0)).sum(-1)
+    e_loss = torch.where(on, w.abs() * tau * tau * (e_lse + 16 * U * mag + e_ent), 0.0)
     c = w * tau * (1.0 if grad is None else grad.double())
     pd = torch.zeros_like(z).scatter_add_(-1, index.long().clamp(0, V - 1), p)
     epd = torch.zeros_like(z).scatter_add_(-1, index.long().clamp(0, V - 1), e_p)
@@ -781,6 +782,41 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(ga, want[0]))
     assert all(torch.equal(x, y) for x, y in zip(gb, want[1]))
+
+
+def test_without_autograd_and_in_inference_mode():
+    """The same results without a graph; nothing requires grad."""
+    ins = _pass_inputs(70)
+    with torch.no_grad():
+        want = _pass(*ins)
+    with torch.inference_mode():
+        got = _pass(*ins)
+    assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(want, got))
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 6, 8, device="cuda", requires_grad=True)
+    idx, t = torch.zeros(4, 6, 2, dtype=torch.long, device="cuda"), torch.zeros(4, 6, 2, device="cuda")
+    for f in (lambda: layer_norm(x), lambda: gated_scan(x, torch.zeros_like(x))[0], lambda: dp.distill_loss(x, idx, t)):
+        g, = torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_other_stream_than_the_default():
+    """Forward and backward on a side stream, with work of the default stream still pending."""
+    ins = _pass_inputs(71)
+    leaf = ins[0].clone().requires_grad_(True)
+    ref, = torch.autograd.grad(gated_scan(leaf, ins[1], gate_mode="sigmoid")[0].float().square().sum(), leaf)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    big = torch.randn(4096, 4096, device="cuda")
+    for _ in range(5):
+        big = big @ big * 1e-3
+    with torch.cuda.stream(side):
+        got, = torch.autograd.grad(gated_scan(leaf, ins[1], gate_mode="sigmoid")[0].float().square().sum(), leaf)
+    torch.cuda.synchronize()
+    assert torch.equal(got, ref)
 
 
 def test_saved_inputs_changed_in_place_are_noticed():
