@@ -57,6 +57,11 @@ def test_scan_arguments():
     assert fwd(x=None) == 1 and fwd(out=None) == 1 and fwd(hL=None) == 1 and fwd(h0=P) == 1
     assert fwd(B=0, x=None) == 0
 
+    far = _strides(6)
+    far[1] = (1 << 28) + 1  # tokens further apart than the kernels' 32 bits of bytes
+    assert L.dp_scan_fwd(P, P, 0, 0, None, P, P, None, 1, 4, 8, far, None) == 2
+    assert L.dp_scan_bwd(P, P, P, 0, 0, P, None, P, P, None, 1, 4, 8, far, None) == 2
+
     def bwd(x=P, dt=0, mode=0, saved=P, dx=P, B=1, T=4, D=8):
         return L.dp_scan_bwd(x, P, P, dt, mode, saved, None, dx, P, None, B, T, D, st, None)
 
