@@ -162,6 +162,10 @@ struct __align__(2 * sizeof(F)) Map {
   F a, H;
 };
 template <bool EXACT, typename F>
+__device__ __forceinline__ Map<EXACT, F> identity() {
+  return {all_<F>(EXACT ? 0.f : 1.f), all_<F>(0.f)};
+}
+template <bool EXACT, typename F>
 __device__ __forceinline__ F apply(const Map<EXACT, F> &m, F h) {
   return EXACT ? add_(fma_(m.a, h, h), m.H) : fma_(m.a, h, m.H);
 }
@@ -260,11 +264,13 @@ __device__ __forceinline__ void box_store(const CUtensorMap *m, const void *src,
                : "memory");
 }
 
-// The exchange of the blocks' maps inside a cluster: each block sends its map to every block
-// (st.async, counted in bytes on the receiver's mbarrier) and waits for the maps of all; there
-// is no cluster-wide barrier.  The buffers alternate: a block sends a span's map after all its
-// warps have left the span before (__syncthreads), so whoever has received the maps of span s
-// may send those of span s + 1 into the buffer of span s - 1.  No message is left when a block
+// The combination of the maps is the work of one warp of a block, between two barriers: it
+// composes the warps' maps, leaving in each one's place the map of the warps before it, sends
+// the block's map to every block of the cluster (st.async, counted in bytes on the receiver's
+// mbarrier), waits for the maps of all, and leaves the state that reaches the block.  There is
+// no cluster-wide barrier.  The buffers of the blocks' maps alternate: a block sends a span's map
+// after it has used those of the span before, so whoever has received the maps of span s may
+// send those of span s + 1 into the buffer of span s - 1.  No message is left when a block
 // ends: it has received all that is sent to it.
 template <typename Shared>
 __device__ __forceinline__ void scan_start(Shared &sh, int cs) {
@@ -298,7 +304,7 @@ __device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[
 template <typename T, int V, int MODE, typename F>
 __device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok]) {
   constexpr bool EXACT = sizeof(T) == 4;
-  Map<EXACT, F> m = {all_<F>(EXACT ? 0.f : 1.f), all_<F>(0.f)};
+  Map<EXACT, F> m = identity<EXACT, F>();
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {
     m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(xw[i * 32]));
@@ -318,14 +324,15 @@ template <typename F, bool EXACT, int NX>
 struct ScanShared {
   uint32_t gate[kWarps][kTok][32];
   uint32_t x[NX][2][kWarps][kTok][32];      // x, and dout in the backward pass
-  Map<EXACT, F> wmap[2][kWarps][32];        // the warps' maps
+  Map<EXACT, F> wmap[kWarps][32];           // the warps' maps, then those of the warps before each
   Map<EXACT, F> bmap[2][kMaxCluster][32];   // the blocks' maps
+  F carry[32];                              // the state (gradient) that reaches the block
   uint64_t bar[2];                          // one per buffer of bmap
   uint64_t gate_bar[kWarps], x_bar[kWarps];  // the warps' bulk copies
 };
 template <typename F, bool EXACT>
 struct ScanSharedBwd : ScanShared<F, EXACT, 2> {
-  F wq[2][kWarps][32];  // H of the warps' gradient maps
+  F wq[kWarps][32];  // H of the warps' gradient maps
 };
 
 // ---------------------------------------------------------------- forward
@@ -399,39 +406,38 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       fetch_gate(base + span);
       fetch_x(base + span, buf ^ 1);
     }
-    sh.wmap[buf][warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
+    sh.wmap[warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
     if (TMA && more) fetch_x(base + span, buf ^ 1);
     __syncthreads();
-    // the block's map, by its last warp, to every block of the cluster
     if (warp == kWarps - 1) {
-      Map<EXACT, F> r = sh.wmap[buf][0][lane];
+      Map<EXACT, F> r = identity<EXACT, F>();
 #pragma unroll
-      for (int j = 1; j < kWarps; ++j) {
-        const Map<EXACT, F> w = sh.wmap[buf][j][lane];
+      for (int j = 0; j < kWarps; ++j) {
+        const Map<EXACT, F> w = sh.wmap[j][lane];
+        sh.wmap[j][lane] = r;
         r.H = apply(w, r.H);
         r.a = compose<EXACT>(r.a, w.a);
       }
+      F in = h;
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
           cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+        if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
+#pragma unroll 4
+        for (int k = 0; k < a.cs; ++k) {
+          if (k == rank) in = h;
+          h = apply(sh.bmap[buf][k][lane], h);
+        }
       } else {
-        sh.bmap[buf][0][lane] = r;
+        h = apply(r, h);
       }
+      sh.carry[lane] = in;
+      const int64_t tile = base / kTile + rank;
+      if (a.saved && on && tile < tiles) store_state(a.saved + ((int64_t)b * tiles + tile) * a.D + c, in);
     }
-    if (a.cs == 1)
-      __syncthreads();
-    else if (alive && !cluster_wait(&sh.bar[buf], phase >> 1 & 1))
-      alive = false;
-    // the state that reaches this block, this warp, and the next span
-    F in = h;
-    for (int k = 0; k < a.cs; ++k) {
-      if (k == rank) in = h;
-      h = apply(sh.bmap[buf][k][lane], h);
-    }
-    if (warp == 0 && a.saved && on && n > 0)
-      store_state(a.saved + ((int64_t)b * tiles + t0 / kTile) * a.D + c, in);
-    for (int j = 0; j < warp; ++j) in = apply(sh.wmap[buf][j][lane], in);
+    __syncthreads();
+    F in = apply(sh.wmap[warp][lane], sh.carry[lane]);
     const int lim = on ? n : 0;
     T *o = at(out, t0, a.ot);
 #pragma unroll
@@ -453,7 +459,7 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   }
   if (TMA && lane == 0) bulk_wait_all();
   if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
-  if (on && rank == 0 && warp == 0) store_state(a.hL + (int64_t)b * a.D + c, h);
+  if (on && rank == 0 && warp == kWarps - 1) store_state(a.hL + (int64_t)b * a.D + c, h);
 }
 
 // ---------------------------------------------------------------- backward
@@ -520,8 +526,8 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     const int64_t t0 = base + off;
     const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - t0));
     uint32_t *xw = &sh.x[0][buf][warp][0][lane], *yw = &sh.x[1][buf][warp][0][lane];
-    F in = all_<F>(0.f);
-    if (on && base + rank * kTile < a.L)
+    F in = all_<F>(0.f);  // the state before the tile
+    if (warp == 0 && on && base + rank * kTile < a.L)
       load_state(a.saved + ((int64_t)b * tiles + base / kTile + rank) * a.D + c, in);
     F nd[kTok];
     const bool more = base > 0;
@@ -539,44 +545,52 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       fetch_gate(base - span);
       fetch_x(base - span, buf ^ 1);
     }
-    sh.wmap[buf][warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
+    sh.wmap[warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
     F Q = all_<F>(0.f);
 #pragma unroll
     for (int i = kTok - 1; i >= 0; --i) {
       Q = add_(Q, Lane<T, V>::get(yw[i * 32]));
       Q = fma_(nd[i], Q, Q);
     }
-    sh.wq[buf][warp][lane] = Q;
+    sh.wq[warp][lane] = Q;
     if (TMA && more) fetch_x(base - span, buf ^ 1);
     __syncthreads();
     if (warp == 0) {
-      Map<EXACT, F> r = {sh.wmap[buf][kWarps - 1][lane].a, sh.wq[buf][kWarps - 1][lane]};
+      // in the place of each warp's maps the state before it and the map of the warps behind it
 #pragma unroll
-      for (int j = kWarps - 2; j >= 0; --j) {
-        const Map<EXACT, F> w = {sh.wmap[buf][j][lane].a, sh.wq[buf][j][lane]};
+      for (int j = 0; j < kWarps; ++j) {
+        const Map<EXACT, F> w = sh.wmap[j][lane];
+        sh.wmap[j][lane].H = in;
+        in = apply(w, in);
+      }
+      Map<EXACT, F> r = identity<EXACT, F>();
+#pragma unroll
+      for (int j = kWarps - 1; j >= 0; --j) {
+        const Map<EXACT, F> w = {sh.wmap[j][lane].a, sh.wq[j][lane]};
+        sh.wmap[j][lane].a = r.a;
+        sh.wq[j][lane] = r.H;
         r.H = apply(w, r.H);
         r.a = compose<EXACT>(r.a, w.a);
       }
+      F qin = q;
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
           cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+        if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
+#pragma unroll 4
+        for (int k = a.cs - 1; k >= 0; --k) {
+          if (k == rank) qin = q;
+          q = apply(sh.bmap[buf][k][lane], q);
+        }
       } else {
-        sh.bmap[buf][0][lane] = r;
+        q = apply(r, q);
       }
+      sh.carry[lane] = qin;
     }
-    if (a.cs == 1)
-      __syncthreads();
-    else if (alive && !cluster_wait(&sh.bar[buf], phase >> 1 & 1))
-      alive = false;
-    F qi = q;
-    for (int k = a.cs - 1; k >= 0; --k) {
-      if (k == rank) qi = q;
-      q = apply(sh.bmap[buf][k][lane], q);
-    }
-    for (int j = kWarps - 1; j > warp; --j)
-      qi = apply(Map<EXACT, F>{sh.wmap[buf][j][lane].a, sh.wq[buf][j][lane]}, qi);
-    for (int j = 0; j < warp; ++j) in = apply(sh.wmap[buf][j][lane], in);
+    __syncthreads();
+    F qi = apply(Map<EXACT, F>{sh.wmap[warp][lane].a, sh.wq[warp][lane]}, sh.carry[lane]);
+    in = sh.wmap[warp][lane].H;
     // backwards over the tokens; the states before them are run forwards again, half of the
     // tokens at a time (registers)
     constexpr int kHalf = kTok / 2;
