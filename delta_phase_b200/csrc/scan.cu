@@ -24,12 +24,13 @@
 // else by cp.async of single words and plain stores.  No warp waits for another one's copies.
 //
 // HBM bounds it where enough channels and tokens run at once (about 1.7 blocks an SM), the chain
-// of spans (2.5 to 3 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
-// and backward: 2 x 32768 x 1024 bf16 97 us (64% of the copy rate) and 130 us (79%), 8 x 8192 x
-// 1024 bf16 89 us (70%) and 123 us (83%), 4 x 8192 x 512 float32 52 us (60%) and 64 us (80%),
-// 1 x 65536 x 256 bf16 (4 chains) 78 us (20%) and 97 us (27%).  With single words instead of boxes
-// the first was 144 and 216 us (address arithmetic: 1048 instead of 769 instructions a warp and
-// span), with a cluster barrier instead of messages 179 and 321 us (its fence).
+// of spans (2.2 to 2.8 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
+// and backward: 2 x 32768 x 1024 bf16 88 us (70% of the copy rate) and 123 us (83%), 8 x 8192 x
+// 1024 bf16 86 us (71%) and 121 us (85%), 4 x 8192 x 512 float32 48 us (65%) and 62 us (83%),
+// 1 x 65536 x 256 bf16 (4 chains) 72 us (21%) and 91 us (28%).  With every warp combining the maps
+// the first was 97 and 130 us (769 instead of 637 instructions a warp and span forward); before
+// that with single words instead of boxes 144 and 216 us (address arithmetic: 1048 instructions),
+// and with a cluster barrier instead of messages 179 and 321 us (its fence).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -300,14 +301,17 @@ __device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[
   }
 }
 
-// The map of a thread's tokens.
-template <typename T, int V, int MODE, typename F>
-__device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok]) {
+// The map of a thread's tokens.  KEEP: their words stay in registers for the second pass.
+template <typename T, int V, int MODE, bool KEEP = false, typename F>
+__device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok],
+                                                                uint32_t *kept = nullptr) {
   constexpr bool EXACT = sizeof(T) == 4;
   Map<EXACT, F> m = identity<EXACT, F>();
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {
-    m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(xw[i * 32]));
+    const uint32_t word = xw[i * 32];
+    if constexpr (KEEP) kept[i] = word;
+    m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(word));
     m.a = fma_(nd[i], m.a, m.a);
     if constexpr (EXACT) m.a = add_(m.a, nd[i]);
   }
@@ -341,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 3)
 scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   using F = typename Lane<T, V>::F;
   constexpr bool EXACT = sizeof(T) == 4;
+  constexpr bool kKeep = V == 1;  // word pairs have no registers left for it (spills: 89 -> 109 us)
   extern __shared__ __align__(128) unsigned char smem[];
   auto &sh = *reinterpret_cast<ScanShared<F, EXACT, 1> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
@@ -406,7 +411,8 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       fetch_gate(base + span);
       fetch_x(base + span, buf ^ 1);
     }
-    sh.wmap[warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
+    uint32_t kept[kKeep ? kTok : 1];
+    sh.wmap[warp][lane] = reduce_tokens<T, V, MODE, kKeep>(xw, nd, kept);
     if (TMA && more) fetch_x(base + span, buf ^ 1);
     __syncthreads();
     if (warp == kWarps - 1) {
@@ -442,7 +448,7 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     T *o = at(out, t0, a.ot);
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      in = step_<MODE>(nd[i], in, Lane<T, V>::get(xw[i * 32]));
+      in = step_<MODE>(nd[i], in, Lane<T, V>::get(kKeep ? kept[i] : xw[i * 32]));
       if constexpr (TMA)
         Lane<T, V>::store(reinterpret_cast<T *>(xw + i * 32), in);  // over the x that it took
       else if (i < lim)
@@ -662,8 +668,9 @@ scan_step_kernel(const float *state, float *state_out, const T *x, const T *gate
 // Blocks of a cluster.  Smaller clusters wait less for one another, but a sequence's chain of
 // spans has to be split until about 1.7 blocks an SM run; sizes that are no power of two pack
 // badly into the GPU's processor clusters.  Measured (us forward, backward at 2 / 4 / 8 / 9 / 16
-// blocks): 32 chains x 32768 tokens bf16 236, 308 / 123, 160 / 97, 130 / 115, 183 / 117, 175;
-// 128 chains x 8192 tokens bf16 89, 123 / 90, 133 / 96, 144 / 101, 156 / 95, 144.
+// blocks): 32 chains x 32768 tokens bf16 215, 289 / 113, 154 / 88, 123 / 115, 183 / 103, 164;
+// 128 chains x 8192 tokens bf16 86, 121 / 86, 128 / 96, 144 / 101, 156 / 105, 175 (the 9 and the
+// second 8 taken with every warp combining the maps).
 int scan_cluster(int L, int64_t chains) {
   int cs = 1;
   while (cs < kMaxCluster && cs * kTile < L && chains * cs < 256) cs *= 2;
