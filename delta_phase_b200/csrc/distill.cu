@@ -51,7 +51,7 @@ struct DistillArgs {
   int group_smem;   // bytes of shared memory of a group
   int stage_bytes;  // the part of it that holds the group's vectors
   int regular;      // one row stride, rows (dz's too) of whole vectors on 16 bytes
-  float tau, inv_tau, c;  // c = log2(e) / tau
+  float tau, c;  // c = log2(e) / tau
 };
 
 __device__ __forceinline__ float di_warp_sum(float v) {
@@ -315,10 +315,11 @@ __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const R
   // what is masked throughout has the sum 0, not NaN
   const float m0 = w.m == -INFINITY ? 0.f : w.m;
   // Exponents z c - m c in one rounding; what the rounding of m c did to all of them alike is
-  // taken back from the sum and the gradient's factor (corr).  Where m c would overflow
-  // -- a row that is masked throughout by the type's lowest value -- values other than m are
-  // further from it than any exponent reaches: 0 for m, -inf for the others.
-  const bool far = fabsf(m0) * c > 1e37f && fabsf(m0) < INFINITY;
+  // taken back from the sum and the gradient's factor (corr).  From |m c| = 2^31 on -- a small
+  // tau, or a row that is masked throughout by the type's lowest value -- that rounding would
+  // leave the exponents' range (m c might overflow), but there the float32 next to m is 2^-24 |m c|
+  // = 128 or more away in the exponent: 1 for m, 0 for all others.
+  const bool far = fabsf(m0) * c >= 2147483648.f && fabsf(m0) < INFINITY;
   const float mc = m0 * c, corr = far ? 1.f : di_ex2(-fmaf(m0, c, -mc));
   const float2 c2 = make_float2(c, c), off = make_float2(-mc, -mc);
   auto exps = [&](const uint4 &v, int k) {
@@ -424,9 +425,10 @@ __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const R
   // masked throughout (or NaN throughout): 0 / 0
   if (M == -INFINITY) S = NAN;
   if (a.loss && rank == 0 && tid == 0) {
-    // sum p (log p - log q) = sum p ((t - TM) - (z - M)) / tau - log TS + log S
+    // sum p (log p - log q) = sum p ((t - TM) - (z - M)) / tau - log TS + log S; times tau^2
+    // without tau^2 or 1 / tau, which may leave the float32 range
     const float d = D / TS - ((M0 == -INFINITY ? 0.f : M0) - M);
-    a.loss[r.row] = empty ? 0.f : weight * a.tau * a.tau * (d * a.inv_tau + (logf(S) - logf(TS)));
+    a.loss[r.row] = empty ? 0.f : weight * (a.tau * (d + a.tau * (logf(S) - logf(TS))));
   }
   if (!a.dz) return;
   if (empty || grad == 0.f) {
@@ -646,7 +648,7 @@ extern "C" int dp_distill(const void *z, int z_dtype, const void *index, int ind
   DistillArgs a = {};
   a.z = z, a.sb = strides[0], a.st = strides[1], a.index = index, a.index64 = index_bytes == 8, a.teacher = teacher;
   a.teacher_dt = teacher_dtype, a.weight = weight, a.grad = grad, a.loss = loss, a.dz = dz;
-  a.tau = tau, a.inv_tau = 1.f / tau, a.c = 1.4426950408889634f / tau;
+  a.tau = tau, a.c = 1.4426950408889634f / tau;
   a.rows = rows, a.L = L, a.V = V, a.K = K;
   cudaStream_t st = as_stream(stream);
   return dispatch_dtype(z_dtype, [&](auto t) { return distill_launch<decltype(t)>(a, st); });

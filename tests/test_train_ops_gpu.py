@@ -444,7 +444,10 @@ def distill_ref(z, index, teacher, tau, weight, grad=None):
     epd = torch.zeros_like(z).scatter_add_(-1, index.long().clamp(0, V - 1), e_p)
     on2 = (on & (c != 0))[..., None]
     dz = torch.where(on2, c[..., None] * (q - pd), 0.0)
-    e_dz = torch.where(on2, c.abs()[..., None] * (q * (e_exp + e_lse[..., None] + 8 * U) + epd + 8 * U * pd), 0.0)
+    # an exponential below 2^-126, the smallest normal float32, counts as 0: with the sum of all
+    # at least 1 (the maximum's own) q and p are then off by less than 2^-126 each
+    e_dz = torch.where(on2, c.abs()[..., None] * (q * (e_exp + e_lse[..., None] + 8 * U) + epd + 8 * U * pd +
+                                                  2 * 2.0 ** -126), 0.0)
     return loss, e_loss, dz, e_dz
 
 
@@ -500,6 +503,16 @@ def test_distill_types_and_temperatures(tau):
         for idt in (torch.int32, torch.int64):
             z, index, teacher, _ = distill_inputs(6, 301, 9, BF16, 3, tdt, idt)
             distill_case(z, index, teacher, tau, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tau", [2.0 ** -9, 2.0 ** -20, 2.0 ** -24, 2.0 ** -28, 2.0 ** -31, 2.0 ** -60, 2.0 ** -90, 2.0 ** 40])
+def test_distill_extreme_temperatures(tau, dtype):
+    # powers of two, so that the kernel's float32 temperature is the definition's; the quotients
+    # logit / tau reach from 2^-40 to past the float32 range
+    for V in (7, 301, 9001, 131072):
+        z, index, teacher, weight = distill_inputs(4, V, 5, dtype, V)
+        distill_case(z, index, teacher, tau, weight)
 
 
 def test_distill_repeated_indices():
