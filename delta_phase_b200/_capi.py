@@ -447,6 +447,13 @@ def _device_index(*tensors):
     return idx
 
 
+def check_sizes(*sizes):
+    """Refuses sizes that the entry points' 32-bit arguments (and their kernels' sums of them)
+    do not hold; ctypes would cut them off."""
+    if max(sizes) > 1 << 30:
+        raise ValueError(f"sizes above 2**30 are not supported, got {sizes}")
+
+
 def _addr(t):
     return None if t is None else t.data_ptr()
 

@@ -511,6 +511,7 @@ extern "C" int dp_layernorm_fwd(const void *x, int x_dtype, const float *residua
   DP_REQUIRE(!residual == !sum_out, DP_ERR_INVALID_ARGUMENT,
              "dp_layernorm_fwd: residual and sum_out come together");
   DP_REQUIRE(rows < (1ll << 31), DP_ERR_UNSUPPORTED, "dp_layernorm_fwd: too many rows");
+  DP_REQUIRE(d <= 1 << 30, DP_ERR_UNSUPPORTED, "dp_layernorm_fwd: d must be <= 2^30");
   LnFwdArgs a{x, residual, ln_w, ln_b, sum_out, mean, rstd, y, x_dtype, y_dtype, d, rows, eps};
   cudaStream_t st = as_stream(stream);
   const bool vec = d % 8 == 0 && ln_al16(x) && ln_al16(residual) && ln_al16(ln_w) && ln_al16(ln_b) &&
@@ -552,6 +553,7 @@ extern "C" int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int 
   DP_REQUIRE(valid_dtype(s_dtype) && valid_dtype(dy_dtype) && valid_dtype(dx_dtype), DP_ERR_INVALID_ARGUMENT,
              "dp_layernorm_bwd: unknown dtype code");
   DP_REQUIRE(rows < (1ll << 31), DP_ERR_UNSUPPORTED, "dp_layernorm_bwd: too many rows");
+  DP_REQUIRE(d <= 1 << 30, DP_ERR_UNSUPPORTED, "dp_layernorm_bwd: d must be <= 2^30");
   cudaStream_t st = as_stream(stream);
   if (rows == 0) {  // the sums over no rows
     cudaError_t e = cudaSuccess;

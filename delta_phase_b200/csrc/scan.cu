@@ -817,6 +817,7 @@ extern "C" int dp_scan_fwd(const void *x, const void *gate, int dtype, int mode,
                                    : cudaMemsetAsync(state_out, 0, bytes, st);
     return e == cudaSuccess ? (int)DP_OK : set_error(DP_ERR_CUDA, std::string("dp_scan_fwd: ") + cudaGetErrorString(e));
   }
+  DP_REQUIRE(L <= 1 << 30, DP_ERR_UNSUPPORTED, "dp_scan_fwd: L must be <= 2^30");
   ScanArgs a = {};
   a.x = x, a.gate = gate, a.h0 = state_in, a.hL = state_out, a.saved = saved, a.out = out;
   a.B = B, a.L = L, a.D = D;
@@ -844,6 +845,7 @@ extern "C" int dp_scan_bwd(const void *x, const void *gate, const void *grad_out
   }
   DP_REQUIRE(x && gate && grad_out && saved && grad_x && grad_gate && strides, DP_ERR_INVALID_ARGUMENT,
              "dp_scan_bwd: null pointer");
+  DP_REQUIRE(L <= 1 << 30, DP_ERR_UNSUPPORTED, "dp_scan_bwd: L must be <= 2^30");
   ScanArgs a = {};
   a.x = x, a.gate = gate, a.dout = grad_out, a.saved = const_cast<float *>(saved), a.dhL = grad_state_out;
   a.dx = grad_x, a.dgate = grad_gate, a.dh0 = grad_state_in;

@@ -41,6 +41,7 @@ def _check(student_logits, teacher_index, teacher_logits, temperature, weight):
     if teacher_index.dim() < 1 or teacher_index.shape != teacher_logits.shape or \
             teacher_index.shape[:-1] != lead or teacher_index.shape[-1] < 1:
         raise ValueError(f"teacher_index and teacher_logits must both be {tuple(lead)} + (K,)")
+    _capi.check_sizes(math.prod(lead), student_logits.shape[-1], teacher_index.shape[-1])
     if teacher_index.dtype not in (torch.int64, torch.int32):
         raise TypeError("teacher_index must be int64 or int32")
     _capi.dtype_code(student_logits)

@@ -33,6 +33,7 @@ def _unit(t):
 def _check_inputs(x, gate, dims, what):
     if x.dim() != dims or gate.shape != x.shape or x.shape[-1] < 1:
         raise ValueError(f"x and gate must both be {what}")
+    _capi.check_sizes(*x.shape)
     _capi.dtype_code(x)
     if gate.dtype != x.dtype:
         raise TypeError("x and gate must share one dtype")
@@ -101,7 +102,7 @@ def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
     * ``gate_mode="sigmoid"``: h_t = sigmoid(gate_t) h_{t-1} + (1 - sigmoid(gate_t)) x_t
 
     x, gate (B, L, D) of one dtype (float32 / bfloat16 / float16; any strides, without a copy
-    where the channel stride is 1); initial_state (B, D) float32 or None, never modified.  Any L.
+    where the channel stride is 1); initial_state (B, D) float32 or None, never modified.  Any L up to 2^30.
     Returns ``(out (B, L, D) of x's dtype, h_L (B, D) float32)``; the state is float32
     throughout and the order of all sums depends on L alone.  A value that is not finite stays in
     its channel, from its token on (an infinite state continues as NaN).  Differentiable once when autograd
@@ -133,7 +134,8 @@ def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None)
             raise ValueError("state_out must be contiguous")
     if out is None:
         out = _like(x)
-    elif out.dtype != x.dtype or out.shape != x.shape or (D > 1 and out.stride(1) != 1):
-        raise ValueError("out must be a (B, D) tensor of x's dtype with unit channel stride")
+    elif out.dtype != x.dtype or out.shape != x.shape or (D > 1 and out.stride(1) != 1) or \
+            (B > 1 and out.stride(0) < D):
+        raise ValueError("out must be a (B, D) tensor of x's dtype with unit channel stride and rows apart")
     _capi.scan_step(state.contiguous(), state_out, _unit(x), _unit(gate), mode, out)
     return out, state_out

@@ -109,6 +109,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, out_dtype=Non
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have a last dimension of at least 1")
     d = x.shape[-1]
+    _capi.check_sizes(d)
     _capi.dtype_code(x)
     if out_dtype is None:
         out_dtype = x.dtype

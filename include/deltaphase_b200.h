@@ -359,7 +359,7 @@ DP_API int dp_layernorm(const void *x, int x_dtype, const float *residual, const
  *   x : (rows, d) of x_dtype;  residual, sum_out (= s) : (rows, d) float32, both or neither
  *   ln_w, ln_b : (d) float32 or NULL (1 and 0);  y : (rows, d) of y_dtype
  *   mean, rstd : (rows) float32, written
- * All tensors contiguous; any d >= 1.  sum_out may be residual (the sum in place).
+ * All tensors contiguous; 1 <= d <= 2^30.  sum_out may be residual (the sum in place).
  */
 DP_API int dp_layernorm_fwd(const void *x, int x_dtype, const float *residual, const float *ln_w,
                         const float *ln_b, float eps, float *sum_out, void *y, int y_dtype, float *mean,
@@ -394,8 +394,8 @@ DP_API int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int dy_d
  *   saved        : (B, ceil(L / dp_scan_tile()), D) float32, the state before each tile, for
  *                  dp_scan_bwd; or NULL
  *   strides[6]   : {sb, st} of x, gate, out
- * The state is float32 throughout; the order of all sums is fixed by L.  Any L >= 0.  The
- * kernels compute h - (1 - a) h for a h: a state that has become infinite continues as NaN.
+ * The state is float32 throughout; the order of all sums is fixed by L.  0 <= L <= 2^30.
+ * The kernels compute h - (1 - a) h for a h: a state that has become infinite continues as NaN.
  * Made for 0 <= a <= 1; larger a are computed too, but a product of a over 128 tokens that
  * overflows float32 may turn a zero state into NaN.  Token strides up to 2^28 elements.
  */

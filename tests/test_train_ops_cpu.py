@@ -25,7 +25,7 @@ def test_layernorm_fwd_arguments():
     assert call(rows=-1) == 1 and call(d=0) == 1 and call(xd=7) == 1 and call(yd=-1) == 1
     assert call(x=None) == 1 and call(y=None) == 1 and call(mean=None) == 1 and call(rstd=None) == 1
     assert call(res=P) == 1 and call(s=P) == 1  # residual and sum_out come together
-    assert call(rows=1 << 31) == 2
+    assert call(rows=1 << 31) == 2 and call(d=(1 << 30) + 1) == 2
     assert call(rows=0, x=None) == 0
 
 
@@ -39,7 +39,7 @@ def test_layernorm_bwd_arguments():
     assert call(rows=-1) == 1 and call(d=0) == 1 and call(sd=3) == 1 and call(dyd=3) == 1 and call(dxd=3) == 1
     assert call(s=None) == 1 and call(dy=None) == 1
     assert call(ws=None) == 6 and call(nbytes=3) == 6 and call(ws=P + 4) == 3
-    assert call(rows=1 << 31) == 2
+    assert call(rows=1 << 31) == 2 and call(d=(1 << 30) + 1) == 2
     assert L.dp_layernorm_bwd_workspace_size(0, 8) == 0
     for rows, d in ((1, 1), (5, 257), (1 << 20, 8192), (3, 9000)):
         assert L.dp_layernorm_bwd_workspace_size(rows, d) >= 8 * d
@@ -56,6 +56,7 @@ def test_scan_arguments():
     assert fwd(B=-1) == 1 and fwd(T=-1) == 1 and fwd(D=0) == 1 and fwd(dt=5) == 1 and fwd(mode=2) == 1
     assert fwd(x=None) == 1 and fwd(out=None) == 1 and fwd(hL=None) == 1 and fwd(h0=P) == 1
     assert fwd(B=0, x=None) == 0
+    assert fwd(T=(1 << 30) + 1) == 2
 
     far = _strides(6)
     far[1] = (1 << 28) + 1  # tokens further apart than the kernels' 32 bits of bytes
@@ -67,6 +68,7 @@ def test_scan_arguments():
 
     assert bwd(B=-1) == 1 and bwd(D=0) == 1 and bwd(dt=5) == 1 and bwd(mode=-1) == 1
     assert bwd(x=None) == 1 and bwd(saved=None) == 1 and bwd(dx=None) == 1
+    assert bwd(T=(1 << 30) + 1) == 2
     assert bwd(B=0, x=None) == 0 and bwd(T=0, x=None) == 0
 
     def step(h=P, x=P, dt=0, mode=0, B=1, D=8):
@@ -153,3 +155,26 @@ def test_python_refusals():
     model = dp.DeltaPhaseModel(dp.DeltaPhaseConfig(dim=16, emb_dim=8, n_layers=1, n_heads=2, vocab_size=32))
     with torch.no_grad(), pytest.raises(RuntimeError, match="gradients enabled"):
         model.distill_step(torch.zeros(1, 4, dtype=torch.long), idx[:1], t[:1])
+
+
+def test_sizes_past_the_c_interface_are_refused():
+    # the entry points take 32-bit sizes; one value, expanded, stands for the large tensors
+    one, n = torch.zeros(1), (1 << 32) + 8
+    idx = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        dp.layer_norm(one.expand(2, n))
+    for shape in ((1, n, 1), (n, 1, 1), (1, 1, n)):
+        with pytest.raises(ValueError, match="2\\*\\*30"):
+            dp.gated_scan(one.expand(shape), one.expand(shape))
+    for shape in ((n, 1), (1, n)):
+        with pytest.raises(ValueError, match="2\\*\\*30"):
+            dp.gated_scan_step(one.expand(shape), one.expand(shape), one.expand(shape))
+    for lead, V, K in (((1, n), 1, 1), ((n, 1), 1, 1), ((1, 1), n, 1), ((1, 1), 1, n), ((n,), 1, 1), ((1 << 16, 1, 1 << 16), 1, 1)):
+        with pytest.raises(ValueError, match="2\\*\\*30"):
+            dp.distill_loss(one.expand(*lead, V), idx.expand(*lead, K), one.expand(*lead, K))
+
+
+def test_step_output_rows_must_not_share_memory():
+    z = torch.zeros
+    with pytest.raises(ValueError, match="out"):
+        dp.gated_scan_step(z(2, 8), z(2, 8), z(2, 8), out=z(1, 8).expand(2, 8))
