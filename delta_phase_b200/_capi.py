@@ -58,7 +58,8 @@ _SIG = {
     "dp_scan_fwd": (_I, [_P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I64P, _P]),
     "dp_scan_bwd": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I64P, _P]),
     "dp_scan_step": (_I, [_P, _P, _P, _P, _I, _I, _P, _I, _I, _I64P, _P]),
-    "dp_distill": (_I, [_P, _I, _P, _I, _P, _I, _P, _P, ctypes.c_float, _P, _P, _I, _I, _I, _I, _I64P, _P]),
+    "dp_distill": (_I, [_P, _I, _P, _I, _P, _I, _P, ctypes.c_float, _P, _P, _P, _I, _I, _I, _I, _I64P, _P]),
+    "dp_distill_bwd": (_I, [_P, _I, _P, _I, _P, _I, _P, _P, _P, ctypes.c_float, _P, _I, _I, _I, _I, _I64P, _P]),
     "dp_layernorm": (_I, [_P, _I, _P, _P, _P, ctypes.c_float, _P, _P, _I, ctypes.c_int64, _I, _P]),
 }
 
@@ -541,11 +542,19 @@ def scan_step(state_in, state_out, x, gate, mode, out):
           dtype_code(x), mode, out.data_ptr(), B, D, _I64x3(x.stride(0), gate.stride(0), out.stride(0)))
 
 
-def distill(z, B, L, sb, st, index, teacher, weight, grad, tau, loss=None, dz=None):
+def distill(z, B, L, sb, st, index, teacher, weight, tau, loss, stats=None, dz=None):
     """dp_distill: z read as (B, L, V) with strides sb, st and unit stride over V = its last
-    dimension; index (int64 or int32), teacher (B, L, K), weight, grad, loss (B, L) and dz
-    (B, L, V) contiguous; loss and / or dz."""
-    idx = _device_index(z, index, teacher, weight, grad, loss, dz)
+    dimension; index (int64 or int32), teacher (B, L, K), weight, loss (B, L), dz (B, L, V) and
+    stats (B, L, 4) contiguous."""
+    idx = _device_index(z, index, teacher, weight, loss, stats, dz)
     _call("dp_distill", idx, z.data_ptr(), dtype_code(z), index.data_ptr(), index.element_size(), teacher.data_ptr(),
-          dtype_code(teacher), _addr(weight), _addr(grad), tau, _addr(loss), _addr(dz), B, L, z.shape[-1],
+          dtype_code(teacher), _addr(weight), tau, loss.data_ptr(), _addr(stats), _addr(dz), B, L, z.shape[-1],
           index.shape[-1], _I64x2(sb, st))
+
+
+def distill_bwd(z, B, L, sb, st, index, teacher, weight, stats, grad, tau, dz):
+    """dp_distill_bwd: the gradient from the stats that distill left; grad (B, L) contiguous."""
+    idx = _device_index(z, index, teacher, weight, stats, grad, dz)
+    _call("dp_distill_bwd", idx, z.data_ptr(), dtype_code(z), index.data_ptr(), index.element_size(),
+          teacher.data_ptr(), dtype_code(teacher), _addr(weight), stats.data_ptr(), _addr(grad), tau, dz.data_ptr(),
+          B, L, z.shape[-1], index.shape[-1], _I64x2(sb, st))

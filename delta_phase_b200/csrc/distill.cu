@@ -4,20 +4,28 @@
 //   dz_v = grad weight tau (q_v - sum_{k: i_k = v} p_k)
 // for the head of DeltaPhaseModel (delta_phase/model.py:60-66, 101).
 //
-// The logits are by far the largest tensors of a training step, and HBM bounds the pass: a row
-// (a block's slice of it, for rows above 64 KB and for few rows; the slices meet in one exchange
-// over distributed shared memory) is read once, into shared memory; its maximum, its sum of
-// exponentials and the gradient come from there, so loss and gradient move 2 V values a row.
-// The exponentials are taken twice, not kept: kept in float32 they fill the registers, one block
-// an SM remains, and its phases (load, reduce, write) follow one another instead of overlapping
-// with those of two others (582 against 406 us below).  What a block does per row besides its
-// 64 elements a thread is kept short: one exchange of maxima and sums, teacher entries by the
-// warps that have some.  Statistics and products are float32; the gradient is rounded once.
+// The logits are by far the largest tensors of a training step, and HBM bounds every pass.
+//   loss and gradient at once: a row (a block's slice of it, for rows above 64 KB and for few
+//     rows; the slices meet in one exchange over distributed shared memory) is read once, into
+//     shared memory; its maximum, its sum of exponentials and the gradient come from there, so
+//     2 V values a row move.  The exponentials are taken twice, not kept: kept in float32 they
+//     fill the registers, one block an SM remains, and its phases (load, reduce, write) follow one
+//     another instead of overlapping with those of two others (582 against 406 us).  What a
+//     block does per row besides its 64 elements a thread is kept short: one exchange of maxima
+//     and sums, teacher entries by the warps that have some.
+//   loss alone: the row is read once, against running maxima, and its sums are kept for
+//   the backward pass: with them every value of the gradient is a function of its logit.
+// Statistics and products are float32; the gradient is rounded once.
 //
-// Measured (B200, K = 64, copy rate 6540 GB/s): loss and gradient of 16384 x 32768 bf16 logits
-// 405 us (5.3 TB/s, 81% of the copy rate), 2048 rows 64 us (64%; 4.6 waves of blocks); loss alone
-// 235 us (70%: the exponentials and the reductions show); 4096 x 32768 float32 213 us (77%);
-// 4096 x 32767 bf16 (rows off the 16-byte grid) 118 us (69%).
+// Measured (B200, K = 64, copy rate 6540 GB/s):
+//                          loss and gradient     loss alone          gradient from the sums
+//   16384 x 32768 bf16     387 us (85% of rate)  192 us (86%)        346 us (95%)
+//   2048 x 32768 bf16      59 us (70%; 4.6 waves of blocks)  36 us (57%)  50 us (83%)
+//   4096 x 32768 float32   215 us (76%)          98 us (84%)         164 us (100%)
+//   4096 x 32767 bf16 (rows off the 16-byte grid)  113 us (72%)  61 us (67%)  96 us (86%)
+//   20000 x 8192 bf16      140 us (72%)          72 us (70%)         116 us (87%)
+// Loss alone through the staged rows was 235 us (70%) and 140 us (59%) for the first and third,
+// their backward pass without sums 405 and 213 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -34,24 +42,28 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kDiMaxVec = 8;      // 16-byte vectors of a row per thread, at most
+constexpr int kDiMaxVec = 8;  // 16-byte vectors of a row per thread, at most
 constexpr int kDiMaxThreads = 512;
 constexpr int kDiMaxK = 1024;
 constexpr int kDiMaxCluster = 16;
+constexpr int kDiMaxSlices = 32;  // blocks a row in any launch, at most
 constexpr int kDiSms = 148;
 constexpr int kDiWarpRows = 4;    // rows of a block where a warp holds a row
+constexpr int kDiStream = 2;      // loss alone: vectors a thread reads at a time
+constexpr int kDiGradThreads = 512;  // gradient from the sums, at most
 
 struct DistillArgs {
   const void *z, *index, *teacher;
   const float *weight, *grad;
   float *loss;
+  float4 *stats;  // per row M, S, TM, TS: written by the loss (or null), read by the backward pass
   void *dz;
   int64_t rows, sb, st;
   int index64, teacher_dt, L, V, K, cs;
   int group_smem;   // bytes of shared memory of a group
   int stage_bytes;  // the part of it that holds the group's vectors
   int regular;      // one row stride, rows (dz's too) of whole vectors on 16 bytes
-  float tau, c;  // c = log2(e) / tau
+  float tau, c;     // c = log2(e) / tau
 };
 
 __device__ __forceinline__ float di_warp_sum(float v) {
@@ -186,6 +198,8 @@ struct Entries {
   float *t, *z;     // teacher's and student's logit there
   uint32_t *once, *again;
   int words;
+  __device__ __forceinline__ void clear(int tid, int n) const;                       // the bit maps
+  __device__ __forceinline__ void mark(const DistillArgs &a, int tid, int n) const;  // the entries' bits
 };
 __device__ __forceinline__ Entries di_entries(unsigned char *mem, int K) {
   Entries e;
@@ -194,6 +208,17 @@ __device__ __forceinline__ Entries di_entries(unsigned char *mem, int K) {
   e.words = di_map_words(K);
   e.once = reinterpret_cast<uint32_t *>(e.z + K), e.again = e.once + e.words;
   return e;
+}
+__device__ __forceinline__ void Entries::clear(int tid, int n) const {
+  for (int k = tid; k < 2 * words; k += n) once[k] = 0;
+}
+__device__ __forceinline__ void Entries::mark(const DistillArgs &a, int tid, int n) const {
+  for (int k = tid; k < a.K; k += n)
+    if (index[k] >= 0) {
+      const uint32_t bit = 1u << (index[k] & 31);
+      uint32_t *word = &once[index[k] >> 5 & (words - 1)];
+      if (atomicOr(word, bit) & bit) atomicOr(word + words, bit);
+    }
 }
 
 // One teacher entry as it is read ahead of its row.
@@ -206,6 +231,18 @@ struct Entry {
     t = load_raw_scalar(a.teacher, a.teacher_dt, o);
   }
   __device__ __forceinline__ bool ok(const DistillArgs &a) const { return index >= 0 && index < a.V; }
+};
+// The same with the student's logit there; index -1: padding.
+struct Seen {
+  int index;
+  float t, z;
+  template <typename T>
+  __device__ __forceinline__ Seen(const DistillArgs &a, const T *row, const Entry &x) {
+    const bool ok = x.ok(a);
+    index = ok ? (int)x.index : -1;
+    t = ok ? raw_scalar_to_f32(x.t, a.teacher_dt) : -INFINITY;
+    z = ok ? to_f32(row[x.index]) : 0.f;
+  }
 };
 
 // A row as its group sees it: 16-byte aligned vectors from element `head` on, split over the
@@ -240,6 +277,11 @@ struct Row {
     v0 = min(rank * per, nvec), cnt = min(per, nvec - v0);
   }
   __device__ __forceinline__ const uint4 *vectors() const { return reinterpret_cast<const uint4 *>(z + head) + v0; }
+  // Element i lies in this block's part: its vectors, and the single elements for the first.
+  __device__ __forceinline__ bool has(int i, int rank) const {
+    constexpr int E = Vec<T>::E;
+    return i < head || i >= tail ? rank == 0 : i >= head + v0 * E && i < head + (v0 + cnt) * E;
+  }
   // A row that does not count: loss 0 (by the caller), gradient 0, z not looked at.
   __device__ __forceinline__ void zeros(const DistillArgs &a, int tid, int n) const {
     constexpr int E = Vec<T>::E;
@@ -293,87 +335,63 @@ struct FromRegisters {
   __device__ __forceinline__ uint4 operator()(int i) const { return v[i]; }
 };
 
-// Loss and gradient of a row (ze: the thread's single element, -inf if none; first: entry
-// `tid`, read ahead; zt: the student's logit there).  `join` makes the (maximum, sum) of the
-// cluster out of this block's.
-// KEEP: the exponentials, against the warp's maximum, are kept in float32 registers and the
-// gradient is their multiple; otherwise the gradient's pass computes them again.
-template <typename T, int NV, bool KEEP, class G, class Src, class Join>
-__device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e, int rank,
-                                       float weight, float grad, const Src &src, float ze, const Entry &first,
-                                       float zt, Join join) {
-  using W = Vec<T>;
-  constexpr int E = W::E;
-  const int tid = g.tid, n = g.n, lane = threadIdx.x & 31, warps = n >> 5;
-  const float c = a.c;
-  Part w;
-  typename W::Max vm;
-  vm.start();
-#pragma unroll
-  for (int i = 0; i < NV; ++i) vm.add(src(i));
-  w.m = di_warp_redux_max(vm.get(ze));
-  // what is masked throughout has the sum 0, not NaN
-  const float m0 = w.m == -INFINITY ? 0.f : w.m;
-  // Exponents z c - m c in one rounding; what the rounding of m c did to all of them alike is
-  // taken back from the sum and the gradient's factor (corr).  From |m c| = 2^31 on -- a small
-  // tau, or a row that is masked throughout by the type's lowest value -- that rounding would
-  // leave the exponents' range (m c might overflow), but there the float32 next to m is 2^-24 |m c|
-  // = 128 or more away in the exponent: 1 for m, 0 for all others.
-  const bool far = fabsf(m0) * c >= 2147483648.f && fabsf(m0) < INFINITY;
-  const float mc = m0 * c, corr = far ? 1.f : di_ex2(-fmaf(m0, c, -mc));
-  const float2 c2 = make_float2(c, c), off = make_float2(-mc, -mc);
-  auto exps = [&](const uint4 &v, int k) {
-    const float2 x = __ffma2_rn(W::pair(v, k), c2, off);
+__device__ __forceinline__ void di_no_loss(const DistillArgs &a, unsigned row) {
+  a.loss[row] = 0.f;
+  if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 0.f, 0.f);
+}
+
+// Exponentials of logits against a maximum m: z c - m c in one rounding; what the rounding of m c
+// did to all of them alike is taken back from their sums (corr).  From |m c| = 2^31 on -- a small
+// tau, or a row that is masked throughout by the type's lowest value -- that rounding would
+// leave the exponents' range (m c might overflow), but there the float32 next to m is 2^-24 |m c|
+// = 128 or more away in the exponent: 1 for m, 0 for all others (far).
+struct Exps {
+  float m0, c, mc, corr;  // m0: what is masked throughout has the sum 0, not NaN
+  bool far;
+  __device__ __forceinline__ Exps(float m, float c_) : c(c_) {
+    m0 = m == -INFINITY ? 0.f : m;
+    far = fabsf(m0) * c >= 2147483648.f && fabsf(m0) < INFINITY;
+    mc = m0 * c, corr = far ? 1.f : di_ex2(-fmaf(m0, c, -mc));
+  }
+  __device__ __forceinline__ float near1(float z) const { return di_ex2(fmaf(z, c, -mc)); }
+  __device__ __forceinline__ float2 near2(float2 z) const {
+    const float2 x = __ffma2_rn(z, make_float2(c, c), make_float2(-mc, -mc));
     return make_float2(di_ex2(x.x), di_ex2(x.y));
-  };
-  auto far_exp = [&](float z) { return z == m0 ? 1.f : z == -INFINITY ? 0.f : z * 0.f; };
-  auto far_exps = [&](const uint4 &v, int k) {
-    const float2 z = W::pair(v, k);
-    return make_float2(far_exp(z.x), far_exp(z.y));
-  };
-  float2 ev[KEEP ? NV * E / 2 : 1];
-  const float ee = far ? far_exp(ze) : di_ex2(fmaf(ze, c, -mc));
-  float2 acc[2] = {make_float2(ee, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint4 v = src(i);
-#pragma unroll
-    for (int k = 0; k < E / 2; ++k) {
-      const float2 x = exps(v, k);
-      if (KEEP) ev[i * (E / 2) + k] = x;
-      acc[k & 1] = __fadd2_rn(acc[k & 1], x);
-    }
   }
-  if (far) {
-    acc[0] = make_float2(ee, 0.f), acc[1] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint4 v = src(i);
-#pragma unroll
-      for (int k = 0; k < E / 2; ++k) {
-        const float2 x = far_exps(v, k);
-        if (KEEP) ev[i * (E / 2) + k] = x;
-        acc[k & 1] = __fadd2_rn(acc[k & 1], x);
-      }
-    }
-  }
-  acc[0] = __fadd2_rn(acc[0], acc[1]);
-  w.s = di_warp_sum(acc[0].x + acc[0].y) * corr;
-  // the teacher's entries
+  __device__ __forceinline__ float far1(float z) const { return z == m0 ? 1.f : z == -INFINITY ? 0.f : z * 0.f; }
+  __device__ __forceinline__ float2 far2(float2 z) const { return make_float2(far1(z.x), far1(z.y)); }
+  __device__ __forceinline__ float one(float z) const { return far ? far1(z) : near1(z); }
+};
+
+// What a row's sums are: the maximum and the sum of its logits' exponentials, those of the
+// teacher's, and whether it has no teacher entries.
+struct Sums {
+  float M, S, TM, TS;
+  bool empty;
+};
+
+// The group's entries into shared memory, their sums, the sums of the row out of the warps' (w.m
+// and w.s are there), and its loss.  TM and TS are valid in the warps that handle entries.
+// first: entry `tid`, read ahead.  `join` makes the (maximum, sum)
+// of the cluster out of this block's.
+template <typename T, class G, class Join>
+__device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e, int rank,
+                                        float weight, Part w, const Seen &first, Join join) {
+  const int tid = g.tid, n = g.n, lane = threadIdx.x & 31, warps = n >> 5;
+  const float c = a.c, m0 = w.m == -INFINITY ? 0.f : w.m;
   const bool entries = tid - lane < a.K;  // a warp that has some
   w.tm = -INFINITY, w.ts = w.d = 0.f;
   if (entries) {
     float tm = -INFINITY;
-    for (int k = tid; k < a.K; k += n) {
-      Entry x = first;
-      if (k != tid) x.read(a, r.row, k);
-      const bool ok = x.ok(a);
-      if (k != tid) zt = ok ? to_f32(r.z[x.index]) : 0.f;
-      const float t = ok ? raw_scalar_to_f32(x.t, a.teacher_dt) : -INFINITY;
-      e.index[k] = ok ? (int)x.index : -1;
-      e.t[k] = t;
-      e.z[k] = zt;
-      tm = fmaxf(tm, t);
+    auto put = [&](int k, const Seen &x) {
+      e.index[k] = x.index, e.t[k] = x.t, e.z[k] = x.z;
+      tm = fmaxf(tm, x.t);
+    };
+    if (tid < a.K) put(tid, first);
+    for (int k = tid + n; k < a.K; k += n) {
+      Entry x;
+      x.read(a, r.row, k);
+      put(k, Seen(a, r.z, x));
     }
     w.tm = di_warp_redux_max(tm);
     const float t0 = w.tm == -INFINITY ? 0.f : w.tm;
@@ -385,59 +403,144 @@ __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const R
     w.ts = di_warp_sum(w.ts);
     w.d = di_warp_sum(w.d);
   }
-  if (a.dz)
-    for (int k = tid; k < 2 * e.words; k += n) e.once[k] = 0;
+  if (a.dz) e.clear(tid, n);
   // the parts of all warps: maxima, then sums relative to them; what the teacher's side gives
   // is needed where entries are handled and by the thread that writes the loss
-  float M = w.m, S = w.s, TM = w.tm, TS = w.ts, D = w.d;
-  bool empty = TS == 0.f;
+  float D = w.d;
+  Sums q = {w.m, w.s, w.tm, w.ts, w.ts == 0.f};
   if (warps > 1) {
     if (lane == 0) g.parts[tid >> 5] = w;
     g.sync();
-    Part q = {-INFINITY, 0.f, -INFINITY, 0.f, 0.f};
-    if (lane < warps) q = g.parts[lane];
-    M = di_warp_redux_max(q.m);
-    const float qs = di_scaled(q.s, q.m, M, c);
-    S = di_warp_sum(qs);
-    empty = !__any_sync(0xffffffffu, q.ts != 0.f);
+    Part o = {-INFINITY, 0.f, -INFINITY, 0.f, 0.f};
+    if (lane < warps) o = g.parts[lane];
+    q.M = di_warp_redux_max(o.m);
+    const float os = di_scaled(o.s, o.m, q.M, c);
+    q.S = di_warp_sum(os);
+    q.empty = !__any_sync(0xffffffffu, o.ts != 0.f);
     if (entries) {
-      TM = di_warp_redux_max(q.tm);
-      const float f = q.tm == -INFINITY ? 1.f : di_ex2((q.tm - TM) * c);
-      TS = di_warp_sum(q.ts * f);
+      q.TM = di_warp_redux_max(o.tm);
+      const float f = o.tm == -INFINITY ? 1.f : di_ex2((o.tm - q.TM) * c);
+      q.TS = di_warp_sum(o.ts * f);
       // d against the common maxima (a part without entries has ts = d = 0)
-      if (q.ts != 0.f)
-        q.d = f * fmaf(q.ts, (q.tm - TM) - ((q.m == -INFINITY ? 0.f : q.m) - (M == -INFINITY ? 0.f : M)), q.d);
-      D = di_warp_sum(q.d);
+      if (o.ts != 0.f)
+        o.d = f * fmaf(o.ts, (o.tm - q.TM) - ((o.m == -INFINITY ? 0.f : o.m) - (q.M == -INFINITY ? 0.f : q.M)), o.d);
+      D = di_warp_sum(o.d);
     }
   } else {
     g.sync();
   }
-  // the entries' bits (their maps were cleared before the barrier)
-  if (a.dz && entries)
-    for (int k = tid; k < a.K; k += n)
-      if (e.index[k] >= 0) {
-        const uint32_t bit = 1u << (e.index[k] & 31);
-        uint32_t *word = &e.once[e.index[k] >> 5 & (e.words - 1)];
-        if (atomicOr(word, bit) & bit) atomicOr(word + e.words, bit);
-      }
-  const float M0 = M;
-  join(M, S);
+  if (a.dz && entries) e.mark(a, tid, n);  // the maps were cleared before the barrier
+  const float M0 = q.M;
+  join(q.M, q.S);
   // masked throughout (or NaN throughout): 0 / 0
-  if (M == -INFINITY) S = NAN;
-  if (a.loss && rank == 0 && tid == 0) {
+  if (q.M == -INFINITY) q.S = NAN;
+  if (rank == 0 && tid == 0) {
     // sum p (log p - log q) = sum p ((t - TM) - (z - M)) / tau - log TS + log S; times tau^2
     // without tau^2 or 1 / tau, which may leave the float32 range
-    const float d = D / TS - ((M0 == -INFINITY ? 0.f : M0) - M);
-    a.loss[r.row] = empty ? 0.f : weight * (a.tau * (d + a.tau * (logf(S) - logf(TS))));
+    const float d = D / q.TS - ((M0 == -INFINITY ? 0.f : M0) - q.M);
+    a.loss[r.row] = q.empty ? 0.f : weight * (a.tau * (d + a.tau * (logf(q.S) - logf(q.TS))));
+    if (a.stats) a.stats[r.row] = make_float4(q.M, q.S, q.TM, q.TS);
   }
+  return q;
+}
+
+// The gradients at the teacher's entries, over the dense values written there (a barrier and the
+// completed bit maps before).  cw = weight tau grad.
+template <typename T, class G>
+__device__ __forceinline__ void di_entry_grads(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e,
+                                               int rank, const Sums &q, float cw) {
+  const int tid = g.tid, n = g.n, lane = threadIdx.x & 31;
+  const float c = a.c, inv_S = di_rcp(q.S), inv_TS = di_rcp(q.TS);
+  for (int k0 = tid - lane; k0 < a.K; k0 += n) {  // whole warps
+    const int k = k0 + lane, i = k < a.K ? e.index[k] : -1;
+    const bool here = i >= 0 && r.has(i, rank);
+    float p = here ? di_ex2((e.t[k] - q.TM) * c) * inv_TS : 0.f;
+    // an index that occurs more than once: the warp adds up all its entries, in a fixed
+    // order, so each of them writes the same value
+    uint32_t more = __ballot_sync(0xffffffffu, here && (e.again[i >> 5 & (e.words - 1)] >> (i & 31) & 1));
+    while (more) {
+      const int from = __ffs(more) - 1, at = __shfl_sync(0xffffffffu, i, from);
+      more &= more - 1;
+      float t = 0.f;
+      for (int j = lane; j < a.K; j += 32)
+        if (e.index[j] == at) t += di_ex2((e.t[j] - q.TM) * c) * inv_TS;
+      t = di_warp_sum(t);
+      if (lane == from) p = t;
+    }
+    if (here) r.dz[i] = from_f32<T>(cw * (di_ex2((e.z[k] - q.M) * c) * inv_S - p));
+  }
+}
+
+// A vector of a row's gradient at p.
+template <typename T>
+__device__ __forceinline__ void di_store(const Row<T> &r, T *p, const uint4 &o) {
+  constexpr int E = Vec<T>::E;
+  if (r.vec) {
+    *reinterpret_cast<uint4 *>(p) = o;
+  } else {
+    const T *x = reinterpret_cast<const T *>(&o);
+#pragma unroll
+    for (int k = 0; k < E; ++k) p[k] = x[k];
+  }
+}
+
+// Loss and gradient of a row (ze: the thread's single element, -inf if none).
+// KEEP: the exponentials, against the warp's maximum, are kept in float32 registers and the
+// gradient is their multiple; otherwise the gradient's pass computes them again, against the
+// row's.
+template <typename T, int NV, bool KEEP, class G, class Src, class Join>
+__device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e, int rank,
+                                       float weight, const Src &src, float ze, const Seen &first,
+                                       Join join) {
+  using W = Vec<T>;
+  constexpr int E = W::E;
+  const int tid = g.tid, n = g.n, lane = threadIdx.x & 31;
+  Part w;
+  typename W::Max vm;
+  vm.start();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) vm.add(src(i));
+  w.m = di_warp_redux_max(vm.get(ze));
+  const Exps x(w.m, a.c);
+  float2 ev[KEEP ? NV * E / 2 : 1];
+  const float ee = x.one(ze);
+  float2 acc[2] = {make_float2(ee, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint4 v = src(i);
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+      const float2 y = x.near2(W::pair(v, k));
+      if (KEEP) ev[i * (E / 2) + k] = y;
+      acc[k & 1] = __fadd2_rn(acc[k & 1], y);
+    }
+  }
+  if (x.far) {
+    acc[0] = make_float2(ee, 0.f), acc[1] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint4 v = src(i);
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) {
+        const float2 y = x.far2(W::pair(v, k));
+        if (KEEP) ev[i * (E / 2) + k] = y;
+        acc[k & 1] = __fadd2_rn(acc[k & 1], y);
+      }
+    }
+  }
+  acc[0] = __fadd2_rn(acc[0], acc[1]);
+  w.s = di_warp_sum(acc[0].x + acc[0].y) * x.corr;
+  const Sums q = di_sums(a, g, r, e, rank, weight, w, first, join);
   if (!a.dz) return;
-  if (empty || grad == 0.f) {
+  if (q.empty) {
     r.zeros(a, tid, n);
     return;
   }
-  const float cw = weight * a.tau * grad, inv_S = di_rcp(S);
-  // from the warp's maximum to the row's (a warp that is masked throughout has only zeros)
-  const float scale = di_scaled(cw * inv_S, w.m, M, c) * corr;
+  const bool entries = tid - lane < a.K;
+  const float cw = weight * a.tau;
+  // KEEP: from the warp's maximum to the row's (a warp that is masked throughout has only zeros)
+  const Exps y(KEEP ? w.m : q.M, a.c);
+  const float scale = (KEEP ? di_scaled(cw * di_rcp(q.S), w.m, q.M, a.c) : cw * di_rcp(q.S)) * y.corr;
   const float2 scale2 = make_float2(scale, scale);
   T *pd = r.dz + r.head + (r.v0 + tid) * E;
   auto write = [&](auto exp_of) {
@@ -447,50 +550,20 @@ __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const R
       if (!KEEP) v = src(i);
 #pragma unroll
       for (int k = 0; k < E / 2; ++k)
-        W::set(o, k, __fmul2_rn(KEEP ? ev[i * (E / 2) + k] : exp_of(v, k), scale2));
-      if (tid + i * n < r.cnt) {
-        T *p = pd + i * n * E;
-        if (r.vec) {
-          *reinterpret_cast<uint4 *>(p) = o;
-        } else {
-          const T *x = reinterpret_cast<const T *>(&o);
-#pragma unroll
-          for (int k = 0; k < E; ++k) p[k] = x[k];
-        }
-      }
+        W::set(o, k, __fmul2_rn(KEEP ? ev[i * (E / 2) + k] : exp_of(W::pair(v, k)), scale2));
+      if (tid + i * n < r.cnt) di_store(r, pd + i * n * E, o);
     }
   };
-  if (!KEEP && far)
-    write(far_exps);
+  if (!KEEP && y.far)
+    write([&](float2 z) { return y.far2(z); });
   else
-    write(exps);
-  if (r.edge < a.V) r.dz[r.edge] = from_f32<T>(ee * scale);
+    write([&](float2 z) { return y.near2(z); });
+  if (r.edge < a.V) r.dz[r.edge] = from_f32<T>(y.one(ze) * scale);
   g.sync();  // the dense values are written and the maps complete: now the teacher's entries
-  if (!entries) return;
-  const float inv_TS = di_rcp(TS);
-  for (int k0 = tid - lane; k0 < a.K; k0 += n) {  // whole warps
-    const int k = k0 + lane, i = k < a.K ? e.index[k] : -1;
-    // this block's elements (vectors, and the single ones for the first)
-    const bool here = i >= 0 && (i < r.head || i >= r.tail
-                                     ? rank == 0
-                                     : i >= r.head + r.v0 * E && i < r.head + (r.v0 + r.cnt) * E);
-    float p = here ? di_ex2((e.t[k] - TM) * c) * inv_TS : 0.f;
-    // an index that occurs more than once: the warp adds up all its entries, in a fixed
-    // order, so each of them writes the same value
-    uint32_t more = __ballot_sync(0xffffffffu, here && (e.again[i >> 5 & (e.words - 1)] >> (i & 31) & 1));
-    while (more) {
-      const int from = __ffs(more) - 1, at = __shfl_sync(0xffffffffu, i, from);
-      more &= more - 1;
-      float t = 0.f;
-      for (int q = lane; q < a.K; q += 32)
-        if (e.index[q] == at) t += di_ex2((e.t[q] - TM) * c) * inv_TS;
-      t = di_warp_sum(t);
-      if (lane == from) p = t;
-    }
-    if (here) r.dz[i] = from_f32<T>(cw * (di_ex2((e.z[k] - M) * c) * inv_S - p));
-  }
+  if (entries) di_entry_grads(a, g, r, e, rank, q, cw);
 }
 
+// Loss and gradient, and the loss alone of short or few rows.
 // A block (or a cluster of a.cs blocks) holds a row, or with WARP a warp, kDiWarpRows rows a
 // block; NV vectors per thread.  STAGE: the vectors wait in shared memory, each copied there
 // (cp.async) by the thread that reads it, twice, so that three times as many threads fit on an
@@ -509,12 +582,12 @@ distill_kernel(const DistillArgs a) {
   if (WARP && row >= a.rows) return;  // whole warps
   std::conditional_t<WARP, WarpGroup, BlockGroup> g;
   g.tid = WARP ? lane : (int)threadIdx.x, g.n = WARP ? 32 : (int)blockDim.x, g.parts = parts;
-  const float weight = a.weight ? a.weight[row] : 1.f, grad = a.grad ? a.grad[row] : 1.f;
+  const float weight = a.weight ? a.weight[row] : 1.f;
   Entry first = {-1, 0};
   if (g.tid < a.K) first.read(a, row, g.tid);
   const Row<T> r(a, row, rank, cs, g.tid);
   if (weight == 0.f) {  // the same for the whole cluster
-    if (a.loss && rank == 0 && g.tid == 0) a.loss[row] = 0.f;
+    if (rank == 0 && g.tid == 0) di_no_loss(a, row);
     if (a.dz) r.zeros(a, g.tid, g.n);
     return;
   }
@@ -541,9 +614,9 @@ distill_kernel(const DistillArgs a) {
   }
   if (cs > 1) cg::this_cluster().sync();  // every block of the cluster runs
   const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
-  const float zt = first.ok(a) ? to_f32(r.z[first.index]) : 0.f;
+  const Seen seen(a, r.z, first);
   if constexpr (STAGE) asm volatile("cp.async.wait_all;\n" ::: "memory");
-  di_row<T, NV, !STAGE>(a, g, r, di_entries(mem, a.K), rank, weight, grad, src, ze, first, zt, [&](float &M, float &S) {
+  di_row<T, NV, !STAGE>(a, g, r, di_entries(mem, a.K), rank, weight, src, ze, seen, [&](float &M, float &S) {
     if (cs == 1) return;
     cg::cluster_group cl = cg::this_cluster();
     if (g.tid < cs) cl.map_shared_rank(cpart, g.tid)[rank] = make_float2(M, S);
@@ -552,18 +625,142 @@ distill_kernel(const DistillArgs a) {
   });
 }
 
-template <typename T, int NV, bool WARP, bool STAGE>
-int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, cudaStream_t st) {
-  auto kern = distill_kernel<T, NV, WARP, STAGE>;
+// The loss alone, many rows: a block a row, which each thread reads once, kDiStream vectors at a
+// time with the next ones on their way, against its own running maximum.  32 registers, so that 64
+// warps run on an SM (4 vectors at a time with 32 warps: 189 us for 16384 x 32768 bf16 against 197,
+// but 99 against 84 for 40000 x 3000 bf16 and 29 against 25 for 509 x 50021 float32).
+template <typename T>
+__global__ void __launch_bounds__(kDiMaxThreads, 4) distill_loss_kernel(const DistillArgs a) {
+  using W = Vec<T>;
+  __shared__ Part parts[kDiMaxThreads / 32];
+  extern __shared__ __align__(16) unsigned char dyn[];
+  const unsigned row = blockIdx.x;
+  BlockGroup g;
+  g.tid = threadIdx.x, g.n = blockDim.x, g.parts = parts;
+  const float weight = a.weight ? a.weight[row] : 1.f;
+  Entry first = {-1, 0};
+  if (g.tid < a.K) first.read(a, row, g.tid);
+  const Row<T> r(a, row, 0, 1, g.tid);
+  if (weight == 0.f) {
+    if (g.tid == 0) di_no_loss(a, row);
+    return;
+  }
+  uint4 next[kDiStream];
+  auto fetch = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < kDiStream; ++i) next[i] = j + i * g.n < r.cnt ? r.vectors()[j + i * g.n] : di_nothing<T>();
+  };
+  fetch(g.tid);
+  const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
+  float m = ze, s = ze == -INFINITY ? 0.f : ze - ze + 1.f;  // NaN and +inf: NaN
+  for (int j = g.tid; j < r.cnt; j += kDiStream * g.n) {
+    uint4 v[kDiStream];
+#pragma unroll
+    for (int i = 0; i < kDiStream; ++i) v[i] = next[i];
+    if (j + kDiStream * g.n < r.cnt) fetch(j + kDiStream * g.n);
+    typename W::Max vm;
+    vm.start();
+#pragma unroll
+    for (int i = 0; i < kDiStream; ++i) vm.add(v[i]);
+    const float m1 = vm.get(m);
+    const Exps x(m1, a.c);
+    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    auto add = [&](auto exp_of) {
+#pragma unroll
+      for (int i = 0; i < kDiStream; ++i)
+#pragma unroll
+        for (int k = 0; k < W::E / 2; ++k) acc[k & 1] = __fadd2_rn(acc[k & 1], exp_of(W::pair(v[i], k)));
+    };
+    if (!x.far)
+      add([&](float2 z) { return x.near2(z); });
+    else
+      add([&](float2 z) { return x.far2(z); });
+    acc[0] = __fadd2_rn(acc[0], acc[1]);
+    s = fmaf(acc[0].x + acc[0].y, x.corr, di_scaled(s, m, m1, a.c));
+    m = m1;
+  }
+  const Seen seen(a, r.z, first);
+  Part w;
+  w.m = di_warp_redux_max(m);
+  w.s = di_warp_sum(di_scaled(s, m, w.m, a.c));
+  di_sums(a, g, r, di_entries(dyn, a.K), 0, weight, w, seen, [](float &, float &) {});
+}
+
+// The gradient from the row's sums, as the loss left them: every value by itself.  A block
+// (WARP: a warp) takes one of the a.cs slices of a row.
+template <typename T, int NV, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kDiWarpRows : kDiGradThreads, WARP ? 8 : 2)
+distill_grad_kernel(const DistillArgs a) {
+  using W = Vec<T>;
+  constexpr int E = W::E;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = WARP ? 0 : blockIdx.x % a.cs;
+  const unsigned row = WARP ? blockIdx.x * kDiWarpRows + warp : blockIdx.x / a.cs;
+  if (WARP && row >= a.rows) return;  // whole warps
+  std::conditional_t<WARP, WarpGroup, BlockGroup> g;
+  g.tid = WARP ? lane : (int)threadIdx.x, g.n = WARP ? 32 : (int)blockDim.x, g.parts = nullptr;
+  const Row<T> r(a, row, rank, WARP ? 1 : a.cs, g.tid);
+  Entry first = {-1, 0};
+  if (g.tid < a.K) first.read(a, row, g.tid);
+  uint4 v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    v[i] = g.tid + i * g.n < r.cnt ? r.vectors()[g.tid + i * g.n] : di_nothing<T>();
+  const float grad = a.grad ? a.grad[row] : 1.f, cw = (a.weight ? a.weight[row] : 1.f) * a.tau * grad;
+  const float4 st = a.stats[row];
+  if (st.w == 0.f || grad == 0.f) {  // no entries, weight 0; or the loss does not count
+    r.zeros(a, g.tid, g.n);
+    return;
+  }
+  const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
+  const Sums q = {st.x, st.y, st.z, st.w, false};
+  const Entries e = di_entries(dyn + (WARP ? warp * a.group_smem : 0), a.K);
+  const bool entries = g.tid - lane < a.K;
+  e.clear(g.tid, g.n);
+  for (int k = g.tid; k < a.K; k += g.n) {
+    Entry x = first;
+    if (k != g.tid) x.read(a, row, k);
+    const bool ok = x.ok(a);
+    e.index[k] = ok ? (int)x.index : -1;
+    e.t[k] = ok ? raw_scalar_to_f32(x.t, a.teacher_dt) : -INFINITY;
+    e.z[k] = ok && r.has((int)x.index, rank) ? to_f32(r.z[x.index]) : 0.f;
+  }
+  g.sync();
+  if (entries) e.mark(a, g.tid, g.n);
+  const Exps x(q.M, a.c);
+  const float scale = cw * di_rcp(q.S) * x.corr;
+  const float2 scale2 = make_float2(scale, scale);
+  T *pd = r.dz + r.head + (r.v0 + g.tid) * E;
+  auto write = [&](auto exp_of) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint4 o;
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) W::set(o, k, __fmul2_rn(exp_of(W::pair(v[i], k)), scale2));
+      if (g.tid + i * g.n < r.cnt) di_store(r, pd + i * g.n * E, o);
+    }
+  };
+  if (x.far)
+    write([&](float2 z) { return x.far2(z); });
+  else
+    write([&](float2 z) { return x.near2(z); });
+  if (r.edge < a.V) r.dz[r.edge] = from_f32<T>(x.one(ze) * scale);
+  g.sync();
+  if (entries) di_entry_grads(a, g, r, e, rank, q, cw);
+}
+
+// Launches KERN with clusters of `cluster` blocks; `most`: bytes of shared memory it may ask for.
+template <void (*KERN)(const DistillArgs)>
+int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, size_t most, int cluster,
+                cudaStream_t st) {
   // more than 48 KB of shared memory and 16-block clusters (a non-portable size): opt in once
   static thread_local bool opted[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !opted[dev])) {
-    constexpr int groups = WARP ? kDiWarpRows : 1, n = WARP ? 32 : kDiMaxThreads;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             groups * ((STAGE ? n * NV * 16 : 0) + di_smem(kDiMaxK)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(KERN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess && dev < 64) opted[dev] = true;
   }
   if (e == cudaSuccess) {
@@ -574,18 +771,24 @@ int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, 
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.cs;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = a.cs > 1 ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, a);
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, KERN, a);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(DP_ERR_CUDA, std::string("dp_distill: ") + cudaGetErrorString(e));
   }
-  return check_launch("distill_kernel");
+  return check_launch("distill kernel");
+}
+template <typename T, int NV, bool WARP, bool STAGE>
+int distill_run_row(const DistillArgs &a, int64_t blocks, int threads, size_t smem, cudaStream_t st) {
+  constexpr int groups = WARP ? kDiWarpRows : 1, n = WARP ? 32 : kDiMaxThreads;
+  return distill_run<distill_kernel<T, NV, WARP, STAGE>>(
+      a, blocks, threads, smem, groups * ((STAGE ? n * NV * 16 : 0) + di_smem(kDiMaxK)), a.cs, st);
 }
 
 template <typename T>
@@ -596,15 +799,39 @@ int distill_launch(DistillArgs a, cudaStream_t st) {
   a.regular = a.V % E == 0 && (a.rows == a.L || a.sb == a.L * a.st) && a.st * size % 16 == 0 &&
               ((reinterpret_cast<uintptr_t>(a.z) | reinterpret_cast<uintptr_t>(a.dz)) & 15) == 0;
   const int entries = (di_smem(a.K) + 15) / 16 * 16;
+  const size_t most_entries = di_smem(kDiMaxK);
   a.cs = 1;
   if (nvec <= 32 * kDiMaxVec) {
     const int64_t blocks = (a.rows + kDiWarpRows - 1) / kDiWarpRows;
+    const int threads = 32 * kDiWarpRows;
     const bool two = nvec <= 64;
+    if (!a.loss) {
+      a.group_smem = entries;
+      const size_t smem = (size_t)entries * kDiWarpRows, most = most_entries * kDiWarpRows;
+      return two ? distill_run<distill_grad_kernel<T, 2, true>>(a, blocks, threads, smem, most, 1, st)
+                 : distill_run<distill_grad_kernel<T, kDiMaxVec, true>>(a, blocks, threads, smem, most, 1, st);
+    }
     a.stage_bytes = 32 * (two ? 2 : kDiMaxVec) * 16;
     a.group_smem = a.stage_bytes + entries;
     const size_t smem = (size_t)a.group_smem * kDiWarpRows;
-    return two ? distill_run<T, 2, true, true>(a, blocks, 32 * kDiWarpRows, smem, st)
-               : distill_run<T, kDiMaxVec, true, true>(a, blocks, 32 * kDiWarpRows, smem, st);
+    return two ? distill_run_row<T, 2, true, true>(a, blocks, threads, smem, st)
+               : distill_run_row<T, kDiMaxVec, true, true>(a, blocks, threads, smem, st);
+  }
+  if (!a.loss) {
+    // the gradient from the sums: slices that need nothing of one another.  Small blocks overlap
+    // best (16384 x 32768 bf16, K = 64: 128 threads 348 us, 512 threads 365), but each slice goes
+    // through all K entries (1000 x 131072 float32, K = 1024: 339 against 228 us).
+    const int slice = (a.K <= 128 ? 128 : kDiGradThreads) * kDiMaxVec;
+    a.cs = (nvec + slice - 1) / slice;
+    const int per = (nvec + a.cs - 1) / a.cs;
+    const int threads = std::max(64, ((per + kDiMaxVec - 1) / kDiMaxVec + 31) / 32 * 32);
+    return distill_run<distill_grad_kernel<T, kDiMaxVec, false>>(a, a.rows * a.cs, threads, entries, most_entries, 1,
+                                                                 st);
+  }
+  if (!a.dz && a.rows >= 2 * kDiSms) {
+    // 16 vectors a thread (8: 219 against 197 us for 16384 x 32768 bf16)
+    const int threads = std::min(kDiMaxThreads, std::max(64, (nvec / 16 + 31) / 32 * 32));
+    return distill_run<distill_loss_kernel<T>>(a, a.rows, threads, entries, most_entries, 1, st);
   }
   const int most = kDiMaxThreads * kDiMaxVec;
   while (a.cs < kDiMaxCluster && (int64_t)a.cs * most < nvec) a.cs *= 2;
@@ -620,36 +847,71 @@ int distill_launch(DistillArgs a, cudaStream_t st) {
   const int threads = std::max(64, ((per + nv - 1) / nv + 31) / 32 * 32);
   a.stage_bytes = nv == kDiMaxVec ? threads * nv * 16 : 0;
   a.group_smem = a.stage_bytes + entries;
-  if (nv == 1) return distill_run<T, 1, false, false>(a, blocks, threads, a.group_smem, st);
-  if (nv == 4) return distill_run<T, 4, false, false>(a, blocks, threads, a.group_smem, st);
-  return distill_run<T, kDiMaxVec, false, true>(a, blocks, threads, a.group_smem, st);
+  if (nv == 1) return distill_run_row<T, 1, false, false>(a, blocks, threads, a.group_smem, st);
+  if (nv == 4) return distill_run_row<T, 4, false, false>(a, blocks, threads, a.group_smem, st);
+  return distill_run_row<T, kDiMaxVec, false, true>(a, blocks, threads, a.group_smem, st);
 }
 
 }  // namespace
 }  // namespace dp
 
+namespace {
+
+// What both entry points check of their arguments; DP_OK: go on (with B L rows).
+int distill_args(dp::DistillArgs &a, const char *what, const void *z, int z_dtype, const void *index, int index_bytes,
+                 const void *teacher, int teacher_dtype, const float *weight, float tau, void *dz, int B, int L, int V,
+                 int K, const int64_t *strides) {
+  using namespace dp;
+  const std::string w = std::string(what) + ": ";
+  DP_REQUIRE(B >= 0 && L >= 0 && V >= 1 && K >= 1, DP_ERR_INVALID_ARGUMENT, w + "bad sizes");
+  DP_REQUIRE(valid_dtype(z_dtype) && valid_dtype(teacher_dtype), DP_ERR_INVALID_ARGUMENT, w + "unknown dtype code");
+  DP_REQUIRE(index_bytes == 4 || index_bytes == 8, DP_ERR_INVALID_ARGUMENT, w + "index must be int32 or int64");
+  DP_REQUIRE(tau > 1e-30f && tau < 1e30f, DP_ERR_INVALID_ARGUMENT, w + "tau must be positive and finite");
+  DP_REQUIRE(K <= kDiMaxK, DP_ERR_UNSUPPORTED, w + "K must be <= 1024");
+  DP_REQUIRE((int64_t)V * (int64_t)dtype_size(z_dtype) <= (1 << 20) - 32, DP_ERR_UNSUPPORTED,
+             w + "a row of z must be smaller than 1 MiB");
+  a.rows = (int64_t)B * L;
+  if (a.rows == 0) return DP_OK;
+  DP_REQUIRE(z && index && teacher && strides, DP_ERR_INVALID_ARGUMENT, w + "null pointer");
+  DP_REQUIRE(z != dz, DP_ERR_INVALID_ARGUMENT, w + "dz must not be z");
+  DP_REQUIRE(a.rows * kDiMaxSlices < (1ll << 31), DP_ERR_UNSUPPORTED, w + "too many rows");
+  a.z = z, a.sb = strides[0], a.st = strides[1], a.index = index, a.index64 = index_bytes == 8, a.teacher = teacher;
+  a.teacher_dt = teacher_dtype, a.weight = weight, a.dz = dz;
+  a.tau = tau, a.c = 1.4426950408889634f / tau;
+  a.L = L, a.V = V, a.K = K;
+  return DP_OK;
+}
+
+}  // namespace
+
 extern "C" int dp_distill(const void *z, int z_dtype, const void *index, int index_bytes, const void *teacher,
-                          int teacher_dtype, const float *weight, const float *grad, float tau, float *loss, void *dz,
+                          int teacher_dtype, const float *weight, float tau, float *loss, float *stats, void *dz,
                           int B, int L, int V, int K, const int64_t *strides, void *stream) {
   using namespace dp;
-  DP_REQUIRE(B >= 0 && L >= 0 && V >= 1 && K >= 1, DP_ERR_INVALID_ARGUMENT, "dp_distill: bad sizes");
-  DP_REQUIRE(valid_dtype(z_dtype) && valid_dtype(teacher_dtype), DP_ERR_INVALID_ARGUMENT,
-             "dp_distill: unknown dtype code");
-  DP_REQUIRE(index_bytes == 4 || index_bytes == 8, DP_ERR_INVALID_ARGUMENT, "dp_distill: index must be int32 or int64");
-  DP_REQUIRE(tau > 1e-30f && tau < 1e30f, DP_ERR_INVALID_ARGUMENT, "dp_distill: tau must be positive and finite");
-  DP_REQUIRE(K <= kDiMaxK, DP_ERR_UNSUPPORTED, "dp_distill: K must be <= 1024");
-  DP_REQUIRE((int64_t)V * (int64_t)dtype_size(z_dtype) <= (1 << 20) - 32, DP_ERR_UNSUPPORTED,
-             "dp_distill: a row of z must be smaller than 1 MiB");
-  if (B == 0 || L == 0) return DP_OK;
-  DP_REQUIRE(z && index && teacher && strides && (loss || dz), DP_ERR_INVALID_ARGUMENT, "dp_distill: null pointer");
-  DP_REQUIRE(z != dz, DP_ERR_INVALID_ARGUMENT, "dp_distill: dz must not be z");
-  const int64_t rows = (int64_t)B * L;
-  DP_REQUIRE(rows * kDiMaxCluster < (1ll << 31), DP_ERR_UNSUPPORTED, "dp_distill: too many rows");
   DistillArgs a = {};
-  a.z = z, a.sb = strides[0], a.st = strides[1], a.index = index, a.index64 = index_bytes == 8, a.teacher = teacher;
-  a.teacher_dt = teacher_dtype, a.weight = weight, a.grad = grad, a.loss = loss, a.dz = dz;
-  a.tau = tau, a.c = 1.4426950408889634f / tau;
-  a.rows = rows, a.L = L, a.V = V, a.K = K;
+  const int rc = distill_args(a, "dp_distill", z, z_dtype, index, index_bytes, teacher, teacher_dtype, weight, tau, dz,
+                              B, L, V, K, strides);
+  if (rc != DP_OK || a.rows == 0) return rc;
+  DP_REQUIRE(loss, DP_ERR_INVALID_ARGUMENT, "dp_distill: null pointer");
+  DP_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, DP_ERR_MISALIGNED,
+             "dp_distill: stats must be 16-byte aligned");
+  a.loss = loss, a.stats = reinterpret_cast<float4 *>(stats);
+  cudaStream_t st = as_stream(stream);
+  return dispatch_dtype(z_dtype, [&](auto t) { return distill_launch<decltype(t)>(a, st); });
+}
+
+extern "C" int dp_distill_bwd(const void *z, int z_dtype, const void *index, int index_bytes, const void *teacher,
+                              int teacher_dtype, const float *weight, const float *stats, const float *grad, float tau,
+                              void *dz, int B, int L, int V, int K, const int64_t *strides, void *stream) {
+  using namespace dp;
+  DistillArgs a = {};
+  const int rc = distill_args(a, "dp_distill_bwd", z, z_dtype, index, index_bytes, teacher, teacher_dtype, weight, tau,
+                              dz, B, L, V, K, strides);
+  if (rc != DP_OK || a.rows == 0) return rc;
+  DP_REQUIRE(stats && dz, DP_ERR_INVALID_ARGUMENT, "dp_distill_bwd: null pointer");
+  DP_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, DP_ERR_MISALIGNED,
+             "dp_distill_bwd: stats must be 16-byte aligned");
+  a.grad = grad, a.stats = reinterpret_cast<float4 *>(const_cast<float *>(stats));
   cudaStream_t st = as_stream(stream);
   return dispatch_dtype(z_dtype, [&](auto t) { return distill_launch<decltype(t)>(a, st); });
 }

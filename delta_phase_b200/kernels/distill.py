@@ -60,14 +60,16 @@ def _check(student_logits, teacher_index, teacher_logits, temperature, weight):
 
 
 class DistillCudaFunction(torch.autograd.Function):
-    """Autograd wrapper of dp_distill on arguments that distill_loss has checked: the loss in the
-    forward pass; the backward pass reads the logits again and writes their gradient."""
+    """Autograd wrapper on arguments that distill_loss has checked: forward on dp_distill, which
+    also leaves the rows' maxima and sums; backward on dp_distill_bwd, which makes the gradient
+    of them and the logits."""
 
     @staticmethod
     def forward(ctx, student_logits, index, teacher, tau, weight):
         loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
-        _capi.distill(*_rows(student_logits), index, teacher, weight, None, tau, loss=loss)
-        ctx.save_for_backward(student_logits, index, teacher, weight)
+        stats = loss.new_empty((loss.numel(), 4))
+        _capi.distill(*_rows(student_logits), index, teacher, weight, tau, loss, stats=stats)
+        ctx.save_for_backward(student_logits, index, teacher, weight, stats)
         ctx.tau = tau
         return loss
 
@@ -79,9 +81,9 @@ class DistillCudaFunction(torch.autograd.Function):
 
 
 def _backward(ctx, grad_loss):
-    logits, index, teacher, weight = ctx.saved_tensors
+    logits, index, teacher, weight, stats = ctx.saved_tensors
     dz = _like(logits)
-    _capi.distill(*_rows(logits), index, teacher, weight, grad_loss.contiguous(), ctx.tau, dz=dz)
+    _capi.distill_bwd(*_rows(logits), index, teacher, weight, stats, grad_loss.contiguous(), ctx.tau, dz)
     return dz, None, None, None, None
 
 
@@ -108,7 +110,7 @@ def distill_loss(student_logits, teacher_index, teacher_logits, temperature=1.0,
     if recording and student_logits.requires_grad:
         return DistillCudaFunction.apply(student_logits, index, teacher, tau, w)
     loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
-    _capi.distill(*_rows(student_logits), index, teacher, w, None, tau, loss=loss)
+    _capi.distill(*_rows(student_logits), index, teacher, w, tau, loss)
     return loss
 
 
@@ -120,5 +122,5 @@ def distill_loss_and_grad(student_logits, teacher_index, teacher_logits, tempera
         tau, index, teacher, w = _check(student_logits, teacher_index, teacher_logits, temperature, weight)
         loss = torch.empty(student_logits.shape[:-1], device=student_logits.device, dtype=torch.float32)
         dz = _like(student_logits)
-        _capi.distill(*_rows(student_logits), index, teacher, w, None, tau, loss=loss, dz=dz)
+        _capi.distill(*_rows(student_logits), index, teacher, w, tau, loss, dz=dz)
     return loss, dz

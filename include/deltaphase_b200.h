@@ -424,27 +424,39 @@ DP_API int dp_scan_step(const float *state_in, float *state_out, const void *x, 
                     int mode, void *out, int B, int D, const int64_t *strides, void *stream);
 
 /*
- * Distillation from a teacher's top logits: the loss, its gradient, or both in one pass over
- * the student's logits.  Per row, with p = softmax(teacher / tau) over the row's K entries and
+ * Distillation from a teacher's top logits: the loss, and with dz the gradient of the sum of all
+ * losses in the same pass over the student's logits.  Per row, with p = softmax(teacher / tau) over the row's K entries and
  * q = softmax(z / tau) over its V logits:
  *   loss  = weight tau^2 sum_k p_k (log p_k - log q_{index_k})
- *   dz_v  = grad weight tau (q_v - sum_{k: index_k = v} p_k)
+ *   dz_v  = weight tau (q_v - sum_{k: index_k = v} p_k)
  *   z       : (B, L, V) of z_dtype, unit stride over V; a row is one (b, t)
  *   index   : (B, L, K) contiguous, int64 (index_bytes 8) or int32 (4); an entry outside
  *             0 .. V - 1 is padding and left out; an index may occur more than once
  *   teacher : (B, L, K) of teacher_dtype, contiguous; -inf leaves the entry out
  *   weight  : (B, L) float32, contiguous, or NULL (= 1).  A row of weight 0 and a row without
  *             entries have loss 0 and gradient 0, whatever z holds
- *   grad    : (B, L) float32, contiguous, the gradient that reaches each row's loss, or NULL
- *             (= 1); where it is 0, so is the row's gradient, whatever z holds
- *   loss    : (B, L) float32, contiguous, or NULL
- *   dz      : (B, L, V) of z_dtype, contiguous, not z, or NULL (loss and dz not both NULL)
+ *   loss    : (B, L) float32, contiguous
+ *   stats   : (B, L, 4) float32, contiguous and 16-byte aligned, the row's maxima and sums for
+ *             dp_distill_bwd; or NULL
+ *   dz      : (B, L, V) of z_dtype, contiguous, not z; or NULL
  *   strides[2] : {sb, st} of z
  * Limits: 1 <= K <= 1024; V times the element size below 1 MiB; 1e-30 < tau < 1e30.
  */
 DP_API int dp_distill(const void *z, int z_dtype, const void *index, int index_bytes,
-                  const void *teacher, int teacher_dtype, const float *weight, const float *grad, float tau,
-                  float *loss, void *dz, int B, int L, int V, int K, const int64_t *strides, void *stream);
+                  const void *teacher, int teacher_dtype, const float *weight, float tau, float *loss,
+                  float *stats, void *dz, int B, int L, int V, int K, const int64_t *strides, void *stream);
+
+/*
+ * Backward of dp_distill: dz_v = grad weight tau (q_v - sum_{k: index_k = v} p_k), in one pass
+ * over the logits.
+ *   stats : as dp_distill wrote it for the same z, index, teacher, weight and tau
+ *   grad  : (B, L) float32, contiguous, the gradient that reaches each row's loss, or NULL (= 1);
+ *           where it is 0, so is the row's gradient, whatever z holds
+ */
+DP_API int dp_distill_bwd(const void *z, int z_dtype, const void *index, int index_bytes,
+                      const void *teacher, int teacher_dtype, const float *weight, const float *stats,
+                      const float *grad, float tau, void *dz, int B, int L, int V, int K,
+                      const int64_t *strides, void *stream);
 
 #ifdef __cplusplus
 }

@@ -81,16 +81,22 @@ def test_scan_arguments():
 def test_distill_arguments():
     L = _capi.lib()
 
-    def call(z=P, zd=0, ib=8, td=0, tau=1.0, loss=P, dz=2 * P, B=1, T=2, V=100, K=4):
-        return L.dp_distill(z, zd, P, ib, P, td, None, None, tau, loss, dz, B, T, V, K, _strides(2), None)
+    def fwd(z=P, zd=0, ib=8, td=0, tau=1.0, loss=P, stats=None, dz=2 * P, B=1, T=2, V=100, K=4):
+        return L.dp_distill(z, zd, P, ib, P, td, None, tau, loss, stats, dz, B, T, V, K, _strides(2), None)
 
-    assert call(B=-1) == 1 and call(T=-1) == 1 and call(V=0) == 1 and call(K=0) == 1
-    assert call(zd=4) == 1 and call(td=4) == 1 and call(ib=2) == 1
-    assert call(tau=0.0) == 1 and call(tau=-1.0) == 1 and call(tau=float("nan")) == 1 and call(tau=float("inf")) == 1
-    assert call(z=None) == 1 and call(loss=None, dz=None) == 1 and call(dz=P) == 1
-    assert call(K=1025) == 2 and call(V=1 << 18) == 2 and call(zd=1, V=1 << 19) == 2
-    assert call(B=1 << 14, T=1 << 14) == 2
-    assert call(B=0, z=None) == 0 and call(T=0, z=None) == 0
+    def bwd(z=P, zd=0, ib=8, td=0, tau=1.0, stats=P, dz=2 * P, B=1, T=2, V=100, K=4):
+        return L.dp_distill_bwd(z, zd, P, ib, P, td, None, stats, None, tau, dz, B, T, V, K, _strides(2), None)
+
+    for call in (fwd, bwd):
+        assert call(B=-1) == 1 and call(T=-1) == 1 and call(V=0) == 1 and call(K=0) == 1
+        assert call(zd=4) == 1 and call(td=4) == 1 and call(ib=2) == 1
+        for tau in (0.0, -1.0, float("nan"), float("inf")):
+            assert call(tau=tau) == 1
+        assert call(z=None) == 1 and call(dz=P) == 1 and call(stats=P + 4) == 3
+        assert call(K=1025) == 2 and call(V=1 << 18) == 2 and call(zd=1, V=1 << 19) == 2
+        assert call(B=1 << 14, T=1 << 14) == 2
+        assert call(B=0, z=None) == 0 and call(T=0, z=None) == 0
+    assert fwd(loss=None) == 1 and bwd(stats=None) == 1 and bwd(dz=None) == 1
 
 
 def test_python_refusals():

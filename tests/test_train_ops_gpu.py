@@ -473,9 +473,9 @@ def distill_case(z, index, teacher, tau, weight):
     g = torch.rand(loss.shape, generator=gen(1), device="cuda")
     leaf = z.detach().requires_grad_(True)
     loss2 = dp.distill_loss(leaf, index, teacher, tau, weight)
-    assert torch.equal(loss2, loss)
+    check(loss2, rl, el, "loss alone")
     with torch.no_grad():
-        assert torch.equal(dp.distill_loss(z, index, teacher, tau, weight), loss)
+        assert torch.equal(dp.distill_loss(z, index, teacher, tau, weight), loss2)
     dz2, = torch.autograd.grad(loss2, leaf, g)
     _, _, rd, ed = distill_ref(z, index, teacher, tau, weight, g)
     check(dz2, rd, ed, "dz autograd")
@@ -549,6 +549,49 @@ def test_distill_masked_values():
         z[3, 5] = math.nan              # one that counts
         loss, dz = dp.distill_loss_and_grad(z, index, teacher, 2.0, weight)
         assert bool(loss[3].isnan()) and bool(dz[3].isnan().all()) and not bool(loss[[0, 4, 5, 6, 7]].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("N,V,K", [(300, 1101, 70), (310, 3001, 300), (297, 8192, 1), (300, 40007, 3), (500, 2081, 1024)])
+def test_distill_many_rows(N, V, K, dtype):
+    z, index, teacher, weight = distill_inputs(N, V, K, dtype, 31)
+    distill_case(z, index, teacher, 1.5, weight)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", [700, 4003, 20000])
+def test_distill_masked_values_in_many_rows(V, dtype):
+    """The masks of the test above where the loss alone and the backward pass have their own
+    kernels; values that rise or fall along the row, so that the running maximum moves always or
+    never; a NaN and an infinity that count."""
+    z, index, teacher, weight = distill_inputs(320, V, 6, dtype, 32)
+    low = torch.finfo(dtype).min
+    z[3, 100:] = -math.inf
+    index[3] = torch.arange(6, device="cuda")
+    z[4, 100:] = low
+    z[5] = low
+    z[6, :-1] = -math.inf
+    index[6] = V - 1
+    z[7] = torch.linspace(-20, 20, V, device="cuda").to(dtype)
+    z[8] = torch.linspace(20, -20, V, device="cuda").to(dtype)
+    teacher[9, 2:] = -math.inf
+    teacher[10] = torch.finfo(F32).min
+    z[1] = math.nan                 # weight 0
+    z[2] = math.nan                 # no entries
+    index[3:5, 5] = index[3:5, 0]
+    index[4] = index[4] % 100
+    distill_case(z, index, teacher, 2.0, weight)
+    z[11, V // 2] = math.nan
+    z[12, V // 3] = math.inf
+    z[13] = -math.inf
+    z[14, 0] = math.nan             # with V on an odd grid a single element before the vectors
+    leaf = z.requires_grad_(True)
+    loss = dp.distill_loss(leaf, index, teacher, 2.0, weight)
+    dz, = torch.autograd.grad(loss.sum(), leaf)
+    bad = torch.zeros(320, dtype=torch.bool, device="cuda")
+    bad[11:15] = True
+    assert torch.equal(loss.isnan(), bad) and torch.equal(dz.isnan().any(-1), bad)
+    assert bool(dz[11].isnan().all()) and bool(dz[13].isnan().all()) and bool(dz[14].isnan().all())
 
 
 def test_distill_entry_with_no_student_probability():
