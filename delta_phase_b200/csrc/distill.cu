@@ -18,14 +18,16 @@
 // Statistics and products are float32; the gradient is rounded once.
 //
 // Measured (B200, K = 64, copy rate 6540 GB/s):
-//                          loss and gradient     loss alone          gradient from the sums
-//   16384 x 32768 bf16     387 us (85% of rate)  192 us (86%)        346 us (95%)
-//   2048 x 32768 bf16      59 us (70%; 4.6 waves of blocks)  36 us (57%)  50 us (83%)
-//   4096 x 32768 float32   215 us (76%)          98 us (84%)         164 us (100%)
-//   4096 x 32767 bf16 (rows off the 16-byte grid)  113 us (72%)  61 us (67%)  96 us (86%)
-//   20000 x 8192 bf16      140 us (72%)          72 us (70%)         116 us (87%)
-// Loss alone through the staged rows was 235 us (70%) and 140 us (59%) for the first and third,
-// their backward pass without sums 405 and 213 us.
+//                          loss and gradient      loss alone      gradient from the sums
+//   16384 x 32768 bf16     387 us (85% of rate)   174 us (94%)    346 us (95%)
+//   2048 x 32768 bf16      59 us (70%)            33 us (62%)     50 us (83%)
+//   4096 x 32768 float32   215 us (76%)           88 us (93%)     164 us (100%)
+//   4096 x 32767 bf16 (rows off the 16-byte grid)
+//                          113 us (72%)           56 us (73%)     96 us (86%)
+//   20000 x 8192 bf16      140 us (72%)           64 us (78%)     116 us (87%)
+// The loss alone through the staged rows was 235 us (70%) and 140 us (59%) for the first and third,
+// their backward pass without sums 405 and 213 us; with the running sum rescaled for every new
+// maximum the loss was 192 and 98 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -49,7 +51,8 @@ constexpr int kDiMaxCluster = 16;
 constexpr int kDiMaxSlices = 32;  // blocks a row in any launch, at most
 constexpr int kDiSms = 148;
 constexpr int kDiWarpRows = 4;    // rows of a block where a warp holds a row
-constexpr int kDiStream = 2;      // loss alone: vectors a thread reads at a time
+constexpr int kDiLossThreads = 256;
+constexpr int kDiStream = 4;      // loss alone: vectors a thread reads at a time
 constexpr int kDiGradThreads = 512;  // gradient from the sums, at most
 
 struct DistillArgs {
@@ -626,11 +629,10 @@ distill_kernel(const DistillArgs a) {
 }
 
 // The loss alone, many rows: a block a row, which each thread reads once, kDiStream vectors at a
-// time with the next ones on their way, against its own running maximum.  32 registers, so that 64
-// warps run on an SM (4 vectors at a time with 32 warps: 189 us for 16384 x 32768 bf16 against 197,
-// but 99 against 84 for 40000 x 3000 bf16 and 29 against 25 for 509 x 50021 float32).
+// time; 48 warps an SM are what hides the loads (2 vectors and 64 warps: 189 against 174 us for
+// 16384 x 32768 bf16, 8 and 32: 193).
 template <typename T>
-__global__ void __launch_bounds__(kDiMaxThreads, 4) distill_loss_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(kDiLossThreads, 6) distill_loss_kernel(const DistillArgs a) {
   using W = Vec<T>;
   __shared__ Part parts[kDiMaxThreads / 32];
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -645,43 +647,59 @@ __global__ void __launch_bounds__(kDiMaxThreads, 4) distill_loss_kernel(const Di
     if (g.tid == 0) di_no_loss(a, row);
     return;
   }
-  uint4 next[kDiStream];
+  const uint4 *vec = r.vectors() + g.tid;
+  const int step = kDiStream * g.n, full = r.cnt / step;
+  uint4 v[kDiStream];
   auto fetch = [&](int j) {
 #pragma unroll
-    for (int i = 0; i < kDiStream; ++i) next[i] = j + i * g.n < r.cnt ? r.vectors()[j + i * g.n] : di_nothing<T>();
+    for (int i = 0; i < kDiStream; ++i) v[i] = vec[j + i * g.n];
   };
-  fetch(g.tid);
-  const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
-  float m = ze, s = ze == -INFINITY ? 0.f : ze - ze + 1.f;  // NaN and +inf: NaN
-  for (int j = g.tid; j < r.cnt; j += kDiStream * g.n) {
-    uint4 v[kDiStream];
+  auto fetch_end = [&] {
 #pragma unroll
-    for (int i = 0; i < kDiStream; ++i) v[i] = next[i];
-    if (j + kDiStream * g.n < r.cnt) fetch(j + kDiStream * g.n);
-    typename W::Max vm;
-    vm.start();
+    for (int i = 0; i < kDiStream; ++i)
+      v[i] = g.tid + full * step + i * g.n < r.cnt ? vec[full * step + i * g.n] : di_nothing<T>();
+  };
+  const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
+  // The exponentials' sum s is against m, which follows the maximum vm where that is 2^32 ahead:
+  // until then the terms are larger, and as exact, as against the maximum itself.
+  typename W::Max vm;
+  vm.start();
+  float m = ze, s = ze == -INFINITY ? 0.f : ze - ze + 1.f;  // NaN and +inf: NaN
+  Exps x(m, a.c);
+  auto add = [&] {
 #pragma unroll
     for (int i = 0; i < kDiStream; ++i) vm.add(v[i]);
     const float m1 = vm.get(m);
-    const Exps x(m1, a.c);
+    if ((m1 - m) * a.c > 32.f) {
+      s = di_scaled(s, m, m1, a.c);
+      m = m1;
+      x = Exps(m, a.c);
+    }
     float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    auto add = [&](auto exp_of) {
+    auto sum = [&](auto exp_of) {
 #pragma unroll
       for (int i = 0; i < kDiStream; ++i)
 #pragma unroll
         for (int k = 0; k < W::E / 2; ++k) acc[k & 1] = __fadd2_rn(acc[k & 1], exp_of(W::pair(v[i], k)));
     };
     if (!x.far)
-      add([&](float2 z) { return x.near2(z); });
+      sum([&](float2 z) { return x.near2(z); });
     else
-      add([&](float2 z) { return x.far2(z); });
+      sum([&](float2 z) { return x.far2(z); });
     acc[0] = __fadd2_rn(acc[0], acc[1]);
-    s = fmaf(acc[0].x + acc[0].y, x.corr, di_scaled(s, m, m1, a.c));
-    m = m1;
+    s = fmaf(acc[0].x + acc[0].y, x.corr, s);
+  };
+  for (int j = 0; j < full; ++j) {
+    fetch(j * step);
+    add();
+  }
+  if (full * step < r.cnt) {
+    fetch_end();
+    add();
   }
   const Seen seen(a, r.z, first);
   Part w;
-  w.m = di_warp_redux_max(m);
+  w.m = di_warp_redux_max(vm.get(ze));
   w.s = di_warp_sum(di_scaled(s, m, w.m, a.c));
   di_sums(a, g, r, di_entries(dyn, a.K), 0, weight, w, seen, [](float &, float &) {});
 }
@@ -829,8 +847,9 @@ int distill_launch(DistillArgs a, cudaStream_t st) {
                                                                  st);
   }
   if (!a.dz && a.rows >= 2 * kDiSms) {
-    // 16 vectors a thread (8: 219 against 197 us for 16384 x 32768 bf16)
-    const int threads = std::min(kDiMaxThreads, std::max(64, (nvec / 16 + 31) / 32 * 32));
+    // 16 vectors a thread in small blocks (20000 x 8192 bf16: 64 us, with 8 vectors 72; 509 x 50021
+    // float32 in blocks of 512: 29 us against 25)
+    const int threads = std::min(kDiLossThreads, std::max(64, (nvec / 16 + 31) / 32 * 32));
     return distill_run<distill_loss_kernel<T>>(a, a.rows, threads, entries, most_entries, 1, st);
   }
   const int most = kDiMaxThreads * kDiMaxVec;
