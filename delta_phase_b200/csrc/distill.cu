@@ -21,10 +21,10 @@
 //                          loss and gradient      loss alone      gradient from the sums
 //   16384 x 32768 bf16     387 us (85% of rate)   174 us (94%)    346 us (95%)
 //   2048 x 32768 bf16      59 us (70%)            33 us (62%)     50 us (83%)
-//   4096 x 32768 float32   215 us (76%)           88 us (93%)     164 us (100%)
+//   4096 x 32768 float32   210 us (78%)           88 us (93%)     164 us (100%)
 //   4096 x 32767 bf16 (rows off the 16-byte grid)
 //                          113 us (72%)           56 us (73%)     96 us (86%)
-//   20000 x 8192 bf16      140 us (72%)           64 us (78%)     116 us (87%)
+//   20000 x 8192 bf16      146 us (69%)           64 us (78%)     116 us (87%)
 // The loss alone through the staged rows was 235 us (70%) and 140 us (59%) for the first and third,
 // their backward pass without sums 405 and 213 us; with the running sum rescaled for every new
 // maximum the loss was 192 and 98 us.
@@ -52,7 +52,7 @@ constexpr int kDiMaxSlices = 32;  // blocks a row in any launch, at most
 constexpr int kDiSms = 148;
 constexpr int kDiWarpRows = 4;    // rows of a block where a warp holds a row
 constexpr int kDiLossThreads = 256;
-constexpr int kDiStream = 4;      // loss alone: vectors a thread reads at a time
+constexpr int kDiStream = 4;      // vectors a thread adds to its running sum at a time
 constexpr int kDiGradThreads = 512;  // gradient from the sums, at most
 
 struct DistillArgs {
@@ -366,6 +366,49 @@ struct Exps {
   __device__ __forceinline__ float one(float z) const { return far ? far1(z) : near1(z); }
 };
 
+// The maximum and the sum of exponentials of a thread's logits as they come by (from `one` on, a
+// single one or -inf).  The sum s is against m, which follows the maximum where that is 2^32 ahead:
+// until then the terms are larger, and as exact, as against the maximum itself.
+template <typename T>
+struct Running {
+  typename Vec<T>::Max vm;
+  float one, m, s;
+  Exps x;
+  __device__ __forceinline__ Running(float one_, float c) : one(one_), m(one_), x(one_, c) {
+    vm.start();
+    s = one == -INFINITY ? 0.f : one - one + 1.f;  // NaN and +inf: NaN
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const uint4 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) vm.add(v[i]);
+    const float m1 = vm.get(m);
+    if ((m1 - m) * x.c > 32.f) {
+      s = di_scaled(s, m, m1, x.c);
+      m = m1;
+      x = Exps(m, x.c);
+    }
+    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    auto sum = [&](auto exp_of) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < Vec<T>::E / 2; ++k) acc[k & 1] = __fadd2_rn(acc[k & 1], exp_of(Vec<T>::pair(v[i], k)));
+    };
+    if (!x.far)
+      sum([&](float2 z) { return x.near2(z); });
+    else
+      sum([&](float2 z) { return x.far2(z); });
+    acc[0] = __fadd2_rn(acc[0], acc[1]);
+    s = fmaf(acc[0].x + acc[0].y, x.corr, s);
+  }
+  // the warp's
+  __device__ __forceinline__ void finish(Part &w) const {
+    w.m = di_warp_redux_max(vm.get(one));
+    w.s = di_warp_sum(di_scaled(s, m, w.m, x.c));
+  }
+};
+
 // What a row's sums are: the maximum and the sum of its logits' exponentials, those of the
 // teacher's, and whether it has no teacher entries.
 struct Sums {
@@ -489,8 +532,9 @@ __device__ __forceinline__ void di_store(const Row<T> &r, T *p, const uint4 &o) 
 
 // Loss and gradient of a row (ze: the thread's single element, -inf if none).
 // KEEP: the exponentials, against the warp's maximum, are kept in float32 registers and the
-// gradient is their multiple; otherwise the gradient's pass computes them again, against the
-// row's.
+// gradient is their multiple; otherwise a running sum takes kDiStream vectors at a time (16384 x
+// 32768 bf16: 387 us; 2: 422, 8: 465 with spilled registers) and the gradient's pass computes the
+// exponentials again, against the row's maximum.
 template <typename T, int NV, bool KEEP, class G, class Src, class Join>
 __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e, int rank,
                                        float weight, const Src &src, float ze, const Seen &first,
@@ -499,40 +543,42 @@ __device__ __forceinline__ void di_row(const DistillArgs &a, const G &g, const R
   constexpr int E = W::E;
   const int tid = g.tid, n = g.n, lane = threadIdx.x & 31;
   Part w;
-  typename W::Max vm;
-  vm.start();
-#pragma unroll
-  for (int i = 0; i < NV; ++i) vm.add(src(i));
-  w.m = di_warp_redux_max(vm.get(ze));
-  const Exps x(w.m, a.c);
   float2 ev[KEEP ? NV * E / 2 : 1];
-  const float ee = x.one(ze);
-  float2 acc[2] = {make_float2(ee, 0.f), make_float2(0.f, 0.f)};
+  if constexpr (KEEP) {
+    typename W::Max vm;
+    vm.start();
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint4 v = src(i);
+    for (int i = 0; i < NV; ++i) vm.add(src(i));
+    w.m = di_warp_redux_max(vm.get(ze));
+    const Exps x(w.m, a.c);
+    float2 acc[2] = {make_float2(x.one(ze), 0.f), make_float2(0.f, 0.f)};
+    auto sum = [&](auto exp_of) {
 #pragma unroll
-    for (int k = 0; k < E / 2; ++k) {
-      const float2 y = x.near2(W::pair(v, k));
-      if (KEEP) ev[i * (E / 2) + k] = y;
-      acc[k & 1] = __fadd2_rn(acc[k & 1], y);
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          ev[i * (E / 2) + k] = exp_of(W::pair(src(i), k));
+          acc[k & 1] = __fadd2_rn(acc[k & 1], ev[i * (E / 2) + k]);
+        }
+    };
+    if (!x.far)
+      sum([&](float2 z) { return x.near2(z); });
+    else
+      sum([&](float2 z) { return x.far2(z); });
+    acc[0] = __fadd2_rn(acc[0], acc[1]);
+    w.s = di_warp_sum(acc[0].x + acc[0].y) * x.corr;
+  } else {
+    constexpr int H = NV < kDiStream ? NV : kDiStream;
+    Running<T> sum(ze, a.c);
+#pragma unroll
+    for (int i = 0; i < NV; i += H) {
+      uint4 v[H];
+#pragma unroll
+      for (int k = 0; k < H; ++k) v[k] = src(i + k);
+      sum.add(v);
     }
+    sum.finish(w);
   }
-  if (x.far) {
-    acc[0] = make_float2(ee, 0.f), acc[1] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint4 v = src(i);
-#pragma unroll
-      for (int k = 0; k < E / 2; ++k) {
-        const float2 y = x.far2(W::pair(v, k));
-        if (KEEP) ev[i * (E / 2) + k] = y;
-        acc[k & 1] = __fadd2_rn(acc[k & 1], y);
-      }
-    }
-  }
-  acc[0] = __fadd2_rn(acc[0], acc[1]);
-  w.s = di_warp_sum(acc[0].x + acc[0].y) * x.corr;
   const Sums q = di_sums(a, g, r, e, rank, weight, w, first, join);
   if (!a.dz) return;
   if (q.empty) {
@@ -660,47 +706,18 @@ __global__ void __launch_bounds__(kDiLossThreads, 6) distill_loss_kernel(const D
       v[i] = g.tid + full * step + i * g.n < r.cnt ? vec[full * step + i * g.n] : di_nothing<T>();
   };
   const float ze = r.edge < a.V ? to_f32(r.z[r.edge]) : -INFINITY;
-  // The exponentials' sum s is against m, which follows the maximum vm where that is 2^32 ahead:
-  // until then the terms are larger, and as exact, as against the maximum itself.
-  typename W::Max vm;
-  vm.start();
-  float m = ze, s = ze == -INFINITY ? 0.f : ze - ze + 1.f;  // NaN and +inf: NaN
-  Exps x(m, a.c);
-  auto add = [&] {
-#pragma unroll
-    for (int i = 0; i < kDiStream; ++i) vm.add(v[i]);
-    const float m1 = vm.get(m);
-    if ((m1 - m) * a.c > 32.f) {
-      s = di_scaled(s, m, m1, a.c);
-      m = m1;
-      x = Exps(m, a.c);
-    }
-    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    auto sum = [&](auto exp_of) {
-#pragma unroll
-      for (int i = 0; i < kDiStream; ++i)
-#pragma unroll
-        for (int k = 0; k < W::E / 2; ++k) acc[k & 1] = __fadd2_rn(acc[k & 1], exp_of(W::pair(v[i], k)));
-    };
-    if (!x.far)
-      sum([&](float2 z) { return x.near2(z); });
-    else
-      sum([&](float2 z) { return x.far2(z); });
-    acc[0] = __fadd2_rn(acc[0], acc[1]);
-    s = fmaf(acc[0].x + acc[0].y, x.corr, s);
-  };
+  Running<T> sum(ze, a.c);
   for (int j = 0; j < full; ++j) {
     fetch(j * step);
-    add();
+    sum.add(v);
   }
   if (full * step < r.cnt) {
     fetch_end();
-    add();
+    sum.add(v);
   }
   const Seen seen(a, r.z, first);
   Part w;
-  w.m = di_warp_redux_max(vm.get(ze));
-  w.s = di_warp_sum(di_scaled(s, m, w.m, a.c));
+  sum.finish(w);
   di_sums(a, g, r, di_entries(dyn, a.K), 0, weight, w, seen, [](float &, float &) {});
 }
 
