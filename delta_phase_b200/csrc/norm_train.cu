@@ -8,13 +8,14 @@
 // All statistics, products and sums are float32.  HBM bounds both passes: a row is held in
 // registers between its read and its write, so each pass moves every tensor once.
 //   forward : a warp a row up to d = 1024 (no barrier), a block of 256 up to 8192; parameters in
-//             pieces from L1, so that 24 warps an SM fit their rows into registers.
+//             pieces from L1, so that 24 warps an SM (32 without a
+//             residual) fit their rows into registers.
 //   backward: eight columns a thread, so that dw and db of a thread's columns stay in registers
 //             while its block walks over the rows; the next rows are loaded meanwhile.  Two
 //             resident blocks of 256 threads without spills beat three with (183 against 222 us
 //             below); 16-bit rows, half as large, go two at a time (90 against 132 us).
 // Measured (B200, copy rate 6540 GB/s), forward and backward: 65536 x 1024 bf16 with the float32
-// residual 132 us (94% of the copy rate) and 183 us (90%), without 78 us (52%) and 90 us (69%);
+// residual 132 us (94% of the copy rate) and 183 us (90%), without 70 us (58%) and 90 us (69%);
 // 16384 x 2048 float32 with residual 91 us (91%) and 109 us (94%); 8192 x 4096 bf16 44 us (47%) and
 // 56 us (55%); 32768 x 1000 bf16 with residual 76 us (79%) and 100 us (80%).
 #include <algorithm>
@@ -159,9 +160,10 @@ __device__ __forceinline__ float ln_group_sum(float v, float *slot) {
   return t;
 }
 
-// G threads per row, 8 NV columns per thread.
-template <int G, int NV, bool VEC>
-__global__ void __launch_bounds__(G == 32 ? 128 : G, G == 32 ? 6 : 2) ln_fwd_kernel(LnFwdArgs a) {
+// G threads per row, 8 NV columns per thread.  RES: there may be a residual; without its registers a
+// third to twice as many warps fit on an SM (65536 x 1024 bf16 80 -> 70 us, 8192 x 8192 83 -> 71).
+template <int G, int NV, bool VEC, bool RES>
+__global__ void __launch_bounds__(G == 32 ? 128 : G, G == 32 ? (RES ? 6 : 8) : RES ? 2 : 4) ln_fwd_kernel(LnFwdArgs a) {
   __shared__ float slot[2][G / 32];
   const int g = threadIdx.x % G;
   const int64_t r = (int64_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
@@ -169,9 +171,9 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G, G == 32 ? 6 : 2) ln_fwd_ker
   const int64_t off = r * a.d;
   float v[NV][8], t[NV][8];
   // the residual first: x is converted, and waited for, where it is loaded (132 against 138 us)
-  if (a.res) ln_load_row<G, NV, VEC>(a.res + off, g, a.d, t);
+  if (RES && a.res) ln_load_row<G, NV, VEC>(a.res + off, g, a.d, t);
   ln_load_row<G, NV, VEC>(a.x, a.x_dt, off, g, a.d, v);
-  if (a.res) {
+  if (RES && a.res) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -516,26 +518,33 @@ extern "C" int dp_layernorm_fwd(const void *x, int x_dtype, const float *residua
   cudaStream_t st = as_stream(stream);
   const bool vec = d % 8 == 0 && ln_al16(x) && ln_al16(residual) && ln_al16(ln_w) && ln_al16(ln_b) &&
                    ln_al16(sum_out) && ln_al16(y);
-  auto launch = [&](auto kern, int G) {
-    const int threads = G == 32 ? 128 : G;
-    const int per = threads / G;
-    kern<<<(unsigned)((rows + per - 1) / per), threads, 0, st>>>(a);
-  };
   // a warp per row up to d = 1024 (no barrier), a block of 256 up to 8192, then the wide kernel
-  if (d <= 256)
-    vec ? launch(ln_fwd_kernel<32, 1, true>, 32) : launch(ln_fwd_kernel<32, 1, false>, 32);
-  else if (d <= 512)
-    vec ? launch(ln_fwd_kernel<32, 2, true>, 32) : launch(ln_fwd_kernel<32, 2, false>, 32);
-  else if (d <= 1024)
-    vec ? launch(ln_fwd_kernel<32, 4, true>, 32) : launch(ln_fwd_kernel<32, 4, false>, 32);
-  else if (d <= 2048)
-    vec ? launch(ln_fwd_kernel<256, 1, true>, 256) : launch(ln_fwd_kernel<256, 1, false>, 256);
-  else if (d <= 4096)
-    vec ? launch(ln_fwd_kernel<256, 2, true>, 256) : launch(ln_fwd_kernel<256, 2, false>, 256);
-  else if (d <= 8192)
-    vec ? launch(ln_fwd_kernel<256, 4, true>, 256) : launch(ln_fwd_kernel<256, 4, false>, 256);
-  else
+  auto run = [&](auto v, auto res) {
+    constexpr bool V = decltype(v)::value, R = decltype(res)::value;
+    auto launch = [&](auto kern, int G) {
+      const int threads = G == 32 ? 128 : G;
+      const int per = threads / G;
+      kern<<<(unsigned)((rows + per - 1) / per), threads, 0, st>>>(a);
+    };
+    if (d <= 256)
+      launch(ln_fwd_kernel<32, 1, V, R>, 32);
+    else if (d <= 512)
+      launch(ln_fwd_kernel<32, 2, V, R>, 32);
+    else if (d <= 1024)
+      launch(ln_fwd_kernel<32, 4, V, R>, 32);
+    else if (d <= 2048)
+      launch(ln_fwd_kernel<256, 1, V, R>, 256);
+    else if (d <= 4096)
+      launch(ln_fwd_kernel<256, 2, V, R>, 256);
+    else
+      launch(ln_fwd_kernel<256, 4, V, R>, 256);
+  };
+  if (d > 8192)
     ln_fwd_wide_kernel<<<(unsigned)rows, 1024, 0, st>>>(a);
+  else if (vec)
+    residual ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
+  else  // single values: bound by their many loads, not by warps (20000 x 1001 f16: 36 us, without RES 39)
+    run(std::false_type{}, std::true_type{});
   return check_launch("dp_layernorm_fwd");
 }
 
