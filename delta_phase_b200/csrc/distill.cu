@@ -92,10 +92,9 @@ __device__ __forceinline__ float di_warp_redux_max(float v) {  // NaN is passed 
 }
 
 // What a warp knows of its part of the row: the maximum m of its logits, s = sum 2^((z - m) c)
-// with c = log2(e) / tau; the maximum tm of its teacher entries, ts = sum 2^((t - tm) c), and
-// d = sum 2^((t - tm) c) ((t - tm) - (z_index - m)), from which the loss follows.
+// with c = log2(e) / tau; the maximum tm of its teacher entries and ts = sum 2^((t - tm) c).
 struct Part {
-  float m, s, tm, ts, d;
+  float m, s, tm, ts;
 };
 
 // A 16-byte vector of the row as pairs of float32, and back.
@@ -424,9 +423,9 @@ template <typename T, class G, class Join>
 __device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const Row<T> &r, const Entries &e, int rank,
                                         float weight, Part w, const Seen &first, Join join) {
   const int tid = g.tid, n = g.n, lane = threadIdx.x & 31, warps = n >> 5;
-  const float c = a.c, m0 = w.m == -INFINITY ? 0.f : w.m;
+  const float c = a.c;
   const bool entries = tid - lane < a.K;  // a warp that has some
-  w.tm = -INFINITY, w.ts = w.d = 0.f;
+  w.tm = -INFINITY, w.ts = 0.f;
   if (entries) {
     float tm = -INFINITY;
     auto put = [&](int k, const Seen &x) {
@@ -441,23 +440,17 @@ __device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const 
     }
     w.tm = di_warp_redux_max(tm);
     const float t0 = w.tm == -INFINITY ? 0.f : w.tm;
-    for (int k = tid; k < a.K; k += n) {
-      const float t = e.t[k] - t0, x = di_ex2(t * c);
-      w.ts += x;
-      if (x != 0.f && e.index[k] >= 0) w.d = fmaf(x, t - (e.z[k] - m0), w.d);
-    }
+    for (int k = tid; k < a.K; k += n) w.ts += di_ex2((e.t[k] - t0) * c);
     w.ts = di_warp_sum(w.ts);
-    w.d = di_warp_sum(w.d);
   }
   if (a.dz) e.clear(tid, n);
   // the parts of all warps: maxima, then sums relative to them; what the teacher's side gives
   // is needed where entries are handled and by the thread that writes the loss
-  float D = w.d;
   Sums q = {w.m, w.s, w.tm, w.ts, w.ts == 0.f};
   if (warps > 1) {
     if (lane == 0) g.parts[tid >> 5] = w;
     g.sync();
-    Part o = {-INFINITY, 0.f, -INFINITY, 0.f, 0.f};
+    Part o = {-INFINITY, 0.f, -INFINITY, 0.f};
     if (lane < warps) o = g.parts[lane];
     q.M = di_warp_redux_max(o.m);
     const float os = di_scaled(o.s, o.m, q.M, c);
@@ -467,25 +460,31 @@ __device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const 
       q.TM = di_warp_redux_max(o.tm);
       const float f = o.tm == -INFINITY ? 1.f : di_ex2((o.tm - q.TM) * c);
       q.TS = di_warp_sum(o.ts * f);
-      // d against the common maxima (a part without entries has ts = d = 0)
-      if (o.ts != 0.f)
-        o.d = f * fmaf(o.ts, (o.tm - q.TM) - ((o.m == -INFINITY ? 0.f : o.m) - (q.M == -INFINITY ? 0.f : q.M)), o.d);
-      D = di_warp_sum(o.d);
     }
   } else {
     g.sync();
   }
   if (a.dz && entries) e.mark(a, tid, n);  // the maps were cleared before the barrier
-  const float M0 = q.M;
   join(q.M, q.S);
   // masked throughout (or NaN throughout): 0 / 0
   if (q.M == -INFINITY) q.S = NAN;
-  if (rank == 0 && tid == 0) {
+  if (rank == 0 && tid < 32) {
     // sum p (log p - log q) = sum p ((t - TM) - (z - M)) / tau - log TS + log S; times tau^2
-    // without tau^2 or 1 / tau, which may leave the float32 range
-    const float d = D / q.TS - ((M0 == -INFINITY ? 0.f : M0) - q.M);
-    a.loss[r.row] = q.empty ? 0.f : weight * (a.tau * (d + a.tau * (logf(q.S) - logf(q.TS))));
-    if (a.stats) a.stats[r.row] = make_float4(q.M, q.S, q.TM, q.TS);
+    // without tau^2 or 1 / tau, which may leave the float32 range.  One warp forms it from the
+    // row's own maxima: a warp's maximum may be that of masked logits or entries only, and
+    // differences from it keep no digits of z.  p, not its multiple, so that the sum of masked
+    // logits stays in range; a p that is 0 counts nothing, whatever z is.
+    const float inv_TS = di_rcp(q.TS);
+    float d = 0.f;
+    for (int k = tid; k < a.K; k += 32) {
+      const float t = e.t[k] - q.TM, p = di_ex2(t * c) * inv_TS;
+      if (p != 0.f) d = fmaf(p, t - (e.z[k] - q.M), d);
+    }
+    d = di_warp_sum(d);
+    if (tid == 0) {
+      a.loss[r.row] = q.empty ? 0.f : weight * (a.tau * (d + a.tau * (logf(q.S) - logf(q.TS))));
+      if (a.stats) a.stats[r.row] = make_float4(q.M, q.S, q.TM, q.TS);
+    }
   }
   return q;
 }
