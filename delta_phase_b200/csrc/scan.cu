@@ -155,27 +155,30 @@ __device__ __forceinline__ F step_(F n, F h, F x) {
 }
 
 // ---------------------------------------------------------------- affine maps of the state
-// What some tokens do to the state: h -> a h + H.  16-bit inputs keep a itself (kTok factors,
-// each rounded once: far below the outputs' rounding).  float32 keeps n = a - 1 like the
-// tokens do; a dropped state (n = -1) then stays dropped by a test, not by rounding.
-template <bool EXACT, typename F>
+// What some tokens do to the state: h -> a h + H, kept as n = a - 1 like the tokens keep it: a
+// itself has lost the digits of 1 - a, and a sequence of open gates is as many such losses as it
+// has tiles.  A dropped state (n = -1) stays dropped by a test, not by rounding.
+template <typename F>
 struct __align__(2 * sizeof(F)) Map {
-  F a, H;
+  F n, H;
 };
-template <bool EXACT, typename F>
-__device__ __forceinline__ Map<EXACT, F> identity() {
-  return {all_<F>(EXACT ? 0.f : 1.f), all_<F>(0.f)};
+template <typename F>
+__device__ __forceinline__ Map<F> identity() {
+  return {all_<F>(0.f), all_<F>(0.f)};
 }
-template <bool EXACT, typename F>
-__device__ __forceinline__ F apply(const Map<EXACT, F> &m, F h) {
-  return EXACT ? add_(fma_(m.a, h, h), m.H) : fma_(m.a, h, m.H);
+template <typename F>
+__device__ __forceinline__ F apply(const Map<F> &m, F h) {
+  return add_(fma_(m.n, h, h), m.H);
 }
-template <bool EXACT, typename F>
+__device__ __forceinline__ float if_dropped(float least, float n) { return least == -1.f ? -1.f : n; }
+__device__ __forceinline__ float2 if_dropped(float2 least, float2 n) {
+  return make_float2(if_dropped(least.x, n.x), if_dropped(least.y, n.y));
+}
+__device__ __forceinline__ float min_(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float2 min_(float2 a, float2 b) { return make_float2(fminf(a.x, b.x), fminf(a.y, b.y)); }
+template <typename F>
 __device__ __forceinline__ F compose(F r, F w) {  // first r, then w
-  if constexpr (EXACT)
-    return r == -1.f || w == -1.f ? -1.f : fmaf(w, r, r) + w;
-  else
-    return mul_(w, r);
+  return if_dropped(min_(r, w), add_(fma_(w, r, r), w));
 }
 
 struct ScanArgs {
@@ -303,39 +306,33 @@ __device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[
 
 // The map of a thread's tokens.  KEEP: their words stay in registers for the second pass.
 template <typename T, int V, int MODE, bool KEEP = false, typename F>
-__device__ __forceinline__ Map<sizeof(T) == 4, F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok],
-                                                                uint32_t *kept = nullptr) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  Map<EXACT, F> m = identity<EXACT, F>();
+__device__ __forceinline__ Map<F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok], uint32_t *kept = nullptr) {
+  Map<F> m = identity<F>();
+  F least = all_<F>(0.f);
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {
     const uint32_t word = xw[i * 32];
     if constexpr (KEEP) kept[i] = word;
     m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(word));
-    m.a = fma_(nd[i], m.a, m.a);
-    if constexpr (EXACT) m.a = add_(m.a, nd[i]);
+    m.n = add_(fma_(nd[i], m.n, m.n), nd[i]);
+    least = min_(least, nd[i]);
   }
-  if constexpr (EXACT) {
-    float least = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) least = fminf(least, nd[i]);
-    if (least == -1.f) m.a = -1.f;
-  }
+  m.n = if_dropped(least, m.n);
   return m;
 }
 
-template <typename F, bool EXACT, int NX>
+template <typename F, int NX>
 struct ScanShared {
   uint32_t gate[kWarps][kTok][32];
   uint32_t x[NX][2][kWarps][kTok][32];      // x, and dout in the backward pass
-  Map<EXACT, F> wmap[kWarps][32];           // the warps' maps, then those of the warps before each
-  Map<EXACT, F> bmap[2][kMaxCluster][32];   // the blocks' maps
+  Map<F> wmap[kWarps][32];           // the warps' maps, then those of the warps before each
+  Map<F> bmap[2][kMaxCluster][32];   // the blocks' maps
   F carry[32];                              // the state (gradient) that reaches the block
   uint64_t bar[2];                          // one per buffer of bmap
   uint64_t gate_bar[kWarps], x_bar[kWarps];  // the warps' bulk copies
 };
-template <typename F, bool EXACT>
-struct ScanSharedBwd : ScanShared<F, EXACT, 2> {
+template <typename F>
+struct ScanSharedBwd : ScanShared<F, 2> {
   F wq[kWarps][32];  // H of the warps' gradient maps
 };
 
@@ -344,10 +341,9 @@ template <typename T, int V, int MODE, bool TMA>
 __global__ void __launch_bounds__(kThreads, 3)
 scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   using F = typename Lane<T, V>::F;
-  constexpr bool EXACT = sizeof(T) == 4;
   constexpr bool kKeep = V == 1;  // word pairs have no registers left for it (spills: 89 -> 109 us)
   extern __shared__ __align__(128) unsigned char smem[];
-  auto &sh = *reinterpret_cast<ScanShared<F, EXACT, 1> *>(smem);
+  auto &sh = *reinterpret_cast<ScanShared<F, 1> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
   const int b = chain / a.tiles_c, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = (chain % a.tiles_c) * 32 * V, c = c0 + lane * V, cc = min(c, a.D - V);
@@ -416,19 +412,19 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     if (TMA && more) fetch_x(base + span, buf ^ 1);
     __syncthreads();
     if (warp == kWarps - 1) {
-      Map<EXACT, F> r = identity<EXACT, F>();
+      Map<F> r = identity<F>();
 #pragma unroll
       for (int j = 0; j < kWarps; ++j) {
-        const Map<EXACT, F> w = sh.wmap[j][lane];
+        const Map<F> w = sh.wmap[j][lane];
         sh.wmap[j][lane] = r;
         r.H = apply(w, r.H);
-        r.a = compose<EXACT>(r.a, w.a);
+        r.n = compose(r.n, w.n);
       }
       F in = h;
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
-          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.n, r.H);
         if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
 #pragma unroll 4
         for (int k = 0; k < a.cs; ++k) {
@@ -476,9 +472,8 @@ template <typename T, int V, int MODE, bool TMA>
 __global__ void __launch_bounds__(kThreads, 2)
 scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   using F = typename Lane<T, V>::F;
-  constexpr bool EXACT = sizeof(T) == 4;
   extern __shared__ __align__(128) unsigned char smem[];
-  auto &sh = *reinterpret_cast<ScanSharedBwd<F, EXACT> *>(smem);
+  auto &sh = *reinterpret_cast<ScanSharedBwd<F> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
   const int b = chain / a.tiles_c, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = (chain % a.tiles_c) * 32 * V, c = c0 + lane * V, cc = min(c, a.D - V);
@@ -565,24 +560,24 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       // in the place of each warp's maps the state before it and the map of the warps behind it
 #pragma unroll
       for (int j = 0; j < kWarps; ++j) {
-        const Map<EXACT, F> w = sh.wmap[j][lane];
+        const Map<F> w = sh.wmap[j][lane];
         sh.wmap[j][lane].H = in;
         in = apply(w, in);
       }
-      Map<EXACT, F> r = identity<EXACT, F>();
+      Map<F> r = identity<F>();
 #pragma unroll
       for (int j = kWarps - 1; j >= 0; --j) {
-        const Map<EXACT, F> w = {sh.wmap[j][lane].a, sh.wq[j][lane]};
-        sh.wmap[j][lane].a = r.a;
+        const Map<F> w = {sh.wmap[j][lane].n, sh.wq[j][lane]};
+        sh.wmap[j][lane].n = r.n;
         sh.wq[j][lane] = r.H;
         r.H = apply(w, r.H);
-        r.a = compose<EXACT>(r.a, w.a);
+        r.n = compose(r.n, w.n);
       }
       F qin = q;
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
-          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.n, r.H);
         if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
 #pragma unroll 4
         for (int k = a.cs - 1; k >= 0; --k) {
@@ -595,7 +590,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       sh.carry[lane] = qin;
     }
     __syncthreads();
-    F qi = apply(Map<EXACT, F>{sh.wmap[warp][lane].a, sh.wq[warp][lane]}, sh.carry[lane]);
+    F qi = apply(Map<F>{sh.wmap[warp][lane].n, sh.wq[warp][lane]}, sh.carry[lane]);
     in = sh.wmap[warp][lane].H;
     // backwards over the tokens; the states before them are run forwards again, half of the
     // tokens at a time (registers)
@@ -757,11 +752,11 @@ template <bool BWD, typename T, int V, bool TMA>
 int scan_run_mode(const ScanArgs &a, const ScanMaps &maps, int mode, cudaStream_t st, const char *what) {
   using F = typename Lane<T, V>::F;
   if constexpr (BWD) {
-    constexpr size_t kSmem = sizeof(ScanSharedBwd<F, sizeof(T) == 4>);
+    constexpr size_t kSmem = sizeof(ScanSharedBwd<F>);
     return mode == DP_SCAN_SIGMOID ? scan_launch<scan_bwd_kernel<T, V, DP_SCAN_SIGMOID, TMA>, kSmem>(a, maps, st, what)
                                    : scan_launch<scan_bwd_kernel<T, V, DP_SCAN_DECAY, TMA>, kSmem>(a, maps, st, what);
   } else {
-    constexpr size_t kSmem = sizeof(ScanShared<F, sizeof(T) == 4, 1>);
+    constexpr size_t kSmem = sizeof(ScanShared<F, 1>);
     return mode == DP_SCAN_SIGMOID ? scan_launch<scan_fwd_kernel<T, V, DP_SCAN_SIGMOID, TMA>, kSmem>(a, maps, st, what)
                                    : scan_launch<scan_fwd_kernel<T, V, DP_SCAN_DECAY, TMA>, kSmem>(a, maps, st, what);
   }

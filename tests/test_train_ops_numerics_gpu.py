@@ -9,7 +9,9 @@ import pytest
 import torch
 
 import delta_phase_b200 as dp
-from test_train_ops_gpu import BF16, F16, F32, distill_case, distill_inputs
+from delta_phase_b200 import _capi
+from delta_phase_b200.kernels import gated_scan
+from test_train_ops_gpu import BF16, F16, F32, U, check, distill_case, distill_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +77,53 @@ def test_distill_likely_entries_at_the_lowest_logit(N, V):
     teacher[3] = 0.0
     loss, _ = distill_case(z, index, teacher, 1.0, None)
     assert 1e38 < float(loss[3]) < math.inf
+
+
+# ---------------------------------------------------------------- gated recurrence, open gates
+def constant_gate(gate, mode):
+    """a and 1 - a of a gate in float64, and a as float32 holds it: the digits of 1 - a lost."""
+    a, d = (1 / (1 + math.exp(-gate)), 1 / (1 + math.exp(gate))) if mode == "sigmoid" else \
+        (math.exp(gate), -math.expm1(gate))
+    return a, d, float(torch.tensor(a, dtype=F32))
+
+
+@pytest.mark.parametrize("D", [8, 37])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("gate", [16.0, 16.25, 17.0])
+def test_scan_open_gates_hold_the_fixed_point(gate, dtype, D):
+    """x = 1 and h0 = 1: the state is 1 for ever."""
+    L = 1 << 18
+    x = torch.ones(1, L, D, device="cuda", dtype=dtype)
+    g = torch.full((1, L, D), gate, device="cuda", dtype=dtype)
+    out, fin = gated_scan(x, g, torch.ones(1, D, device="cuda"), gate_mode="sigmoid")
+    # two roundings of the state a tile of tokens, and a tile's tokens one after another
+    lim = (2 * L / _capi.scan_tile() + 2 * _capi.scan_tile()) * U
+    assert float((fin - 1).abs().max()) <= lim
+    assert float((out.double() - 1).abs().max()) <= lim + torch.finfo(dtype).eps / 2
+    # a rounded to float32 would show: the state would run to (1 - a) / (1 - a32)
+    a, d, a32 = constant_gate(gate, "sigmoid")
+    assert gate != 16.25 or abs(d / (1 - a32) - 1) * -math.expm1(-L * d) > lim
+
+
+@pytest.mark.parametrize("D", [8, 37])
+@pytest.mark.parametrize("dtype,gate,mode", [(F32, -1.3e-6, "decay"), (BF16, -1.3e-6, "decay"), (F16, -2.0 ** -19, "decay"),
+                                             (F32, 14.1, "sigmoid"), (BF16, 14.0, "sigmoid"), (F16, 14.1, "sigmoid")])
+def test_scan_open_gates_decay_as_defined(dtype, gate, mode, D):
+    """x = 0: h_L = a^L h0, and with dL/dh_L = 1 the gradients a^L of h0 and (1 - a) a^L or a^L h0 of
+    every gate, forward and backward through the maps of 2048 tiles."""
+    L = 1 << 18
+    gates = torch.full((1, L, D), gate, device="cuda", dtype=dtype).requires_grad_(True)
+    x = torch.zeros(1, L, D, device="cuda", dtype=dtype).requires_grad_(True)
+    h0 = torch.full((1, D), 1.5, device="cuda").requires_grad_(True)
+    _, fin = gated_scan(x, gates, h0, gate_mode=mode)
+    _, dg, dh = torch.autograd.grad(fin, (x, gates, h0), torch.ones_like(fin))
+    a, d, a32 = constant_gate(float(gates[0, 0, 0].detach()), mode)
+    rest = math.exp(L * (math.log1p(-d)))
+    # relative: two roundings a tile, a tile's tokens one after another, 1 - a within 8 U of itself
+    rel = (2 * L / _capi.scan_tile() + 2 * _capi.scan_tile() + 8 * L * d) * U
+    check(fin.detach(), torch.full_like(fin, 1.5 * rest, dtype=torch.float64), 1.5 * rest * rel, "h_L")
+    check(dh, torch.full_like(dh, rest, dtype=torch.float64), rest * rel, "dh0")
+    each = 1.5 * rest * (d if mode == "sigmoid" else 1.0)
+    check(dg, torch.full_like(dg, each, dtype=torch.float64), 2 * each * rel, "dgate")
+    # with a rounded to float32 the first two would fail (-2^-19 loses next to nothing that way)
+    assert gate == -2.0 ** -19 or abs(a32 ** L / rest - 1) > rel
