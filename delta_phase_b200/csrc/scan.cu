@@ -7,9 +7,12 @@
 //   decay: dx = p, dgate = q h_{t-1};  sigmoid: dx = d p, dgate = q d (h_{t-1} - x)
 //   and dL/dh_{-1} = q_0.
 //
-// The recurrence runs on -d, not on a: a close to 1 has lost the digits of 1 - a, which is
-// what a long memory consists of.  h - d h is one fused multiply-add, exact in d, and a gate
-// that drops the state (d = 1) leaves exactly nothing of it.
+// No float32 holds both ends of a gate: an a close to 1 has lost the digits of 1 - a, which is
+// what a long memory consists of, and a d close to 1 those of a, which is all that the old state
+// and the gate's gradient see.  Tokens use a (and in sigmoid mode d beside it), each exact to its
+// own digits: the few of a block lose nothing that shows.  What goes on from block to block is a
+// map whose factor is a - 1 where the product of the a is close to 1 and the product elsewhere.  A
+// gate that drops the state (a = 0) leaves exactly nothing of it.
 //
 // Layout: a lane owns the channels of one 4-byte word (two 16-bit values, packed two-wide
 // float32 arithmetic, or one float), a warp kTok consecutive tokens of its 32 words, a block
@@ -24,13 +27,15 @@
 // else by cp.async of single words and plain stores.  No warp waits for another one's copies.
 //
 // HBM bounds it where enough channels and tokens run at once (about 1.7 blocks an SM), the chain
-// of spans (2.2 to 2.8 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
-// and backward: 2 x 32768 x 1024 bf16 88 us (70% of the copy rate) and 123 us (83%), 8 x 8192 x
-// 1024 bf16 86 us (71%) and 121 us (85%), 4 x 8192 x 512 float32 48 us (65%) and 62 us (83%),
-// 1 x 65536 x 256 bf16 (4 chains) 72 us (21%) and 91 us (28%).  With every warp combining the maps
-// the first was 97 and 130 us (769 instead of 637 instructions a warp and span forward); before
-// that with single words instead of boxes 144 and 216 us (address arithmetic: 1048 instructions),
-// and with a cluster barrier instead of messages 179 and 321 us (its fence).
+// of spans (2.3 to 2.8 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
+// and backward: 2 x 32768 x 1024 bf16 84 us (73% of the copy rate) and 117 us (88%), 8 x 8192 x
+// 1024 bf16 in sigmoid mode 84 us (73%) and 129 us (79%), 4 x 8192 x 512 float32 39 us (78%) and
+// 66 us (78%), 1 x 65536 x 256 bf16 (4 chains) 74 us (21%) and 90 us (28%).  The first was 148 and
+// 190 us with a marked factor, and the selection that goes with it, for every token, and 93 and
+// 125 us with one for every warp.  Older versions of it: every warp combining the maps 97 and
+// 130 us against 88 and 123 by one (769 and 637 instructions a warp and span forward); single words
+// instead of boxes 144 and 216 us (address arithmetic: 1048 instructions), and with a cluster
+// barrier instead of messages 179 and 321 us (its fence).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -109,7 +114,7 @@ struct Lane<__half, 2> {
   }
 };
 
-// ---------------------------------------------------------------- gates: -d = a - 1
+// ---------------------------------------------------------------- gates
 __device__ __forceinline__ float ex2_(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -122,64 +127,116 @@ __device__ __forceinline__ float rcp_(float x) {
   return y;
 }
 __device__ __forceinline__ float2 rcp_(float2 x) { return make_float2(rcp_(x.x), rcp_(x.y)); }
-__device__ __forceinline__ float near0(float g, float a, float b) { return fabsf(g) < 0.0625f ? a : b; }
-__device__ __forceinline__ float2 near0(float2 g, float2 a, float2 b) {
-  return make_float2(near0(g.x, a.x, b.x), near0(g.y, a.y, b.y));
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN stays
+  float m;
+  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
-// 16-bit gates: exp(g) - 1 by its Taylor series g + ... + g^4/24 where |g| < 1/16 (the first
-// term left out is below 2^-22 of the value), by the hardware exponential elsewhere (its
-// error of 2^-22 against |a - 1| > 0.06: below 2^-18), far below the rounding of g itself;
-// sigmoid(f) - 1 = -1 / (1 + exp(f)) within a few 2^-22.  float32: the library's functions.
+__device__ __forceinline__ float2 min_nan(float2 a, float b) { return make_float2(min_nan(a.x, b), min_nan(a.y, b)); }
+
+// a of a gate, and in sigmoid mode d, each within a few steps of its own value.  16-bit gates: the
+// hardware exponential and reciprocal (2^-22, and |gate| 2^-24 from the exponent's rounding):
+// f = exp(gate), d = 1 / (1 + f), a = f d; f ends at 2^125, where a is 1 and d 2^-125.  float32: the
+// library's functions.
 template <typename T, int MODE, typename F>
-__device__ __forceinline__ F neg_drop(F g) {
+__device__ __forceinline__ void gate_(F g, F &a, F &d) {
+  d = all_<F>(0.f);  // not used in decay mode
   if constexpr (sizeof(T) == 4) {
-    return MODE == DP_SCAN_SIGMOID ? -1.f / (1.f + expf(g)) : expm1f(g);
-  } else if constexpr (MODE == DP_SCAN_SIGMOID) {
-    return mul_(rcp_(add_(ex2_(mul_(g, all_<F>(1.4426950408889634f))), all_<F>(1.f))), all_<F>(-1.f));
+    if constexpr (MODE == DP_SCAN_SIGMOID) {
+      const float v = 1.f / (1.f + expf(fabsf(g))), w = 1.f - v;
+      a = g < 0.f ? v : w, d = g < 0.f ? w : v;
+    } else {
+      a = expf(g);
+    }
   } else {
-    F p = fma_(g, all_<F>(1.f / 24.f), all_<F>(1.f / 6.f));
-    p = fma_(p, g, all_<F>(0.5f));
-    p = fma_(p, g, all_<F>(1.f));
-    const F e = ex2_(mul_(g, all_<F>(1.4426950408889634f)));
-    return near0(g, mul_(g, p), add_(e, all_<F>(-1.f)));
+    a = ex2_(mul_(g, all_<F>(1.4426950408889634f)));
+    if constexpr (MODE == DP_SCAN_SIGMOID) {
+      a = min_nan(a, 4.2535296e37f);
+      d = rcp_(add_(a, all_<F>(1.f)));
+      a = mul_(a, d);
+    }
   }
 }
 
-// h' = h - d h + u from n = -d; u = x or d x
-template <int MODE, typename F>
-__device__ __forceinline__ F step_(F n, F h, F x) {
-  if constexpr (MODE == DP_SCAN_SIGMOID)
-    return fma_(n, fma_(x, all_<F>(-1.f), h), h);  // h - d (h - x)
-  else
-    return add_(fma_(n, h, h), x);
-}
-
 // ---------------------------------------------------------------- affine maps of the state
-// What some tokens do to the state: h -> a h + H, kept as n = a - 1 like the tokens keep it: a
-// itself has lost the digits of 1 - a, and a sequence of open gates is as many such losses as it
-// has tiles.  A dropped state (n = -1) stays dropped by a test, not by rounding.
+// What some tokens do to the state: h -> a h + H.  Inside a block a is enough, like it is for tokens.
+// What the chain of blocks applies to the state, block after block, keeps a and n = a - 1, each to
+// its own digits, in one word m: n where a lies in [1/2, 2], else a.  Its lowest bit tells which
+// (1: n), for which it is cut to 23 bits; n = 0 becomes 2^-149, which no state sees.
 template <typename F>
 struct __align__(2 * sizeof(F)) Map {
-  F n, H;
+  F a, H;  // of a block: m, H
 };
+__device__ __forceinline__ bool near_one(float n) { return fabsf(n - 0.25f) <= 0.75f; }
+__device__ __forceinline__ float marked(float a, float n) {
+  return __uint_as_float(near_one(n) ? __float_as_uint(n) | 1u : __float_as_uint(a) & ~1u);
+}
+__device__ __forceinline__ float2 marked(float2 a, float2 n) { return make_float2(marked(a.x, n.x), marked(a.y, n.y)); }
+__device__ __forceinline__ float if_near(float m, float h) { return __float_as_uint(m) & 1u ? h : 0.f; }
+__device__ __forceinline__ float2 if_near(float2 m, float2 h) { return make_float2(if_near(m.x, h.x), if_near(m.y, h.y)); }
+// a h + H from m; the small part first, so that a state at its fixed point stays there
 template <typename F>
-__device__ __forceinline__ Map<F> identity() {
-  return {all_<F>(0.f), all_<F>(0.f)};
+__device__ __forceinline__ F apply_marked(const Map<F> &m, F h) {
+  return add_(if_near(m.a, h), fma_(m.a, h, m.H));
 }
 template <typename F>
 __device__ __forceinline__ F apply(const Map<F> &m, F h) {
-  return add_(fma_(m.n, h, h), m.H);
+  return fma_(m.a, h, m.H);
 }
-__device__ __forceinline__ float if_dropped(float least, float n) { return least == -1.f ? -1.f : n; }
-__device__ __forceinline__ float2 if_dropped(float2 least, float2 n) {
-  return make_float2(if_dropped(least.x, n.x), if_dropped(least.y, n.y));
-}
-__device__ __forceinline__ float min_(float a, float b) { return fminf(a, b); }
-__device__ __forceinline__ float2 min_(float2 a, float2 b) { return make_float2(fminf(a.x, b.x), fminf(a.y, b.y)); }
+// The map of r and then w, and the n of both.
 template <typename F>
-__device__ __forceinline__ F compose(F r, F w) {  // first r, then w
-  return if_dropped(min_(r, w), add_(fma_(w, r, r), w));
+__device__ __forceinline__ void follow(Map<F> &r, F &n, const Map<F> &w, F wn) {
+  r.H = apply(w, r.H);
+  r.a = mul_(r.a, w.a);
+  n = add_(fma_(wn, n, n), wn);
 }
+
+// exp(s) - 1 beside a = exp(s): by its Taylor series where |s| < ln 2 (the first term left out is
+// below 2^-26 of the value).
+__device__ __forceinline__ float in_ln2(float s, float series, float other) { return fabsf(s) < 0.6931472f ? series : other; }
+__device__ __forceinline__ float2 in_ln2(float2 s, float2 series, float2 other) {
+  return make_float2(in_ln2(s.x, series.x, other.x), in_ln2(s.y, series.y, other.y));
+}
+template <typename F>
+__device__ __forceinline__ F exp_less1(F s, F a) {
+  F p = fma_(s, all_<F>(1.f / 362880.f), all_<F>(1.f / 40320.f));
+  p = fma_(p, s, all_<F>(1.f / 5040.f));
+  p = fma_(p, s, all_<F>(1.f / 720.f));
+  p = fma_(p, s, all_<F>(1.f / 120.f));
+  p = fma_(p, s, all_<F>(1.f / 24.f));
+  p = fma_(p, s, all_<F>(1.f / 6.f));
+  p = fma_(p, s, all_<F>(0.5f));
+  p = fma_(p, s, all_<F>(1.f));
+  return in_ln2(s, mul_(p, s), add_(a, all_<F>(-1.f)));
+}
+
+// a, and from n where that has more digits
+__device__ __forceinline__ float best_a(float a, float n) { return near_one(n) ? n + 1.f : a; }
+__device__ __forceinline__ float2 best_a(float2 a, float2 n) { return make_float2(best_a(a.x, n.x), best_a(a.y, n.y)); }
+
+// The factor of a warp's tokens, as their gates come by.  Decay: from the gates' sum, whose exponential
+// is the product (float32: the product itself where that is small, as the sum's roundings would show).
+// Sigmoid: 1 - a follows a recurrence of its own, of positive terms: d + a D.
+template <typename T, int MODE, typename F>
+struct Product {
+  F a = all_<F>(1.f), s = all_<F>(0.f);
+  __device__ __forceinline__ void add(F gate, F ta, F td) {
+    s = MODE == DP_SCAN_SIGMOID ? fma_(ta, s, td) : add_(s, gate);
+    if (MODE == DP_SCAN_SIGMOID || sizeof(T) == 4) a = mul_(a, ta);
+  }
+  __device__ __forceinline__ void get(F &pa, F &pn) const {
+    if constexpr (MODE == DP_SCAN_SIGMOID) {
+      pa = a, pn = mul_(s, all_<F>(-1.f));
+    } else {
+      if constexpr (sizeof(T) == 4)
+        pa = a;
+      else
+        pa = ex2_(mul_(s, all_<F>(1.4426950408889634f)));
+      pn = exp_less1(s, pa);
+    }
+    pa = best_a(pa, pn);
+  }
+};
 
 struct ScanArgs {
   const void *x, *gate, *dout;  // (B, L, D), strides {sb, st}
@@ -292,40 +349,52 @@ __device__ __forceinline__ void scan_start(Shared &sh, int cs) {
   else
     __syncthreads();
 }
-// The n = -d of a thread's tokens from the staged gates; tokens past the end keep the state.
+// a and d of a thread's tokens from the staged gates, and the factor of them all.  Tokens past the
+// end keep the state: their gates and x are staged as 0, which in decay mode is a = 1 already.
 template <typename T, int V, int MODE, typename F>
-__device__ __forceinline__ void load_gates(const uint32_t *slot, int n, F (&nd)[kTok]) {
+__device__ __forceinline__ Product<T, MODE, F> load_gates(const uint32_t *slot, int n, F (&a)[kTok], F (&d)[kTok]) {
+  Product<T, MODE, F> p;
+  auto load = [&](auto whole) {
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) nd[i] = neg_drop<T, MODE>(Lane<T, V>::get(slot[i * 32]));
-  if (n < kTok) {
-#pragma unroll
-    for (int i = 0; i < kTok; ++i)
-      if (i >= n) nd[i] = all_<F>(0.f);
-  }
+    for (int i = 0; i < kTok; ++i) {
+      const F g = Lane<T, V>::get(slot[i * 32]);
+      gate_<T, MODE>(g, a[i], d[i]);
+      if (!decltype(whole)::value && i >= n) a[i] = all_<F>(1.f), d[i] = all_<F>(0.f);
+      p.add(g, a[i], d[i]);
+    }
+  };
+  if (MODE == DP_SCAN_DECAY || n == kTok)
+    load(std::true_type{});
+  else
+    load(std::false_type{});
+  return p;
 }
 
-// The map of a thread's tokens.  KEEP: their words stay in registers for the second pass.
-template <typename T, int V, int MODE, bool KEEP = false, typename F>
-__device__ __forceinline__ Map<F> reduce_tokens(const uint32_t *xw, const F (&nd)[kTok], uint32_t *kept = nullptr) {
-  Map<F> m = identity<F>();
-  F least = all_<F>(0.f);
+// h' of a token
+template <int MODE, typename F>
+__device__ __forceinline__ F step_(F a, F d, F h, F x) {
+  return fma_(a, h, MODE == DP_SCAN_SIGMOID ? mul_(d, x) : x);
+}
+
+// The H of a thread's tokens.  KEEP: their u stay in registers (d's) for the second pass.
+template <typename T, int V, int MODE, bool KEEP, typename F>
+__device__ __forceinline__ F reduce_tokens(const uint32_t *xw, const F (&a)[kTok], F (&d)[kTok]) {
+  F H = all_<F>(0.f);
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {
-    const uint32_t word = xw[i * 32];
-    if constexpr (KEEP) kept[i] = word;
-    m.H = step_<MODE>(nd[i], m.H, Lane<T, V>::get(word));
-    m.n = add_(fma_(nd[i], m.n, m.n), nd[i]);
-    least = min_(least, nd[i]);
+    const F x = Lane<T, V>::get(xw[i * 32]), u = MODE == DP_SCAN_SIGMOID ? mul_(d[i], x) : x;
+    if constexpr (KEEP) d[i] = u;
+    H = fma_(a[i], H, u);
   }
-  m.n = if_dropped(least, m.n);
-  return m;
+  return H;
 }
 
 template <typename F, int NX>
 struct ScanShared {
   uint32_t gate[kWarps][kTok][32];
   uint32_t x[NX][2][kWarps][kTok][32];      // x, and dout in the backward pass
-  Map<F> wmap[kWarps][32];           // the warps' maps, then those of the warps before each
+  Map<F> wmap[kWarps][32];                  // the warps' maps, then those of the warps before each
+  F wn[kWarps][32];                         // their n
   Map<F> bmap[2][kMaxCluster][32];   // the blocks' maps
   F carry[32];                              // the state (gradient) that reaches the block
   uint64_t bar[2];                          // one per buffer of bmap
@@ -337,11 +406,16 @@ struct ScanSharedBwd : ScanShared<F, 2> {
 };
 
 // ---------------------------------------------------------------- forward
+// u in registers between the two passes: single values, and pairs in sigmoid mode, where it is d x
+// (two blocks an SM instead of three; the usual launch has 1.7).  Pairs in decay mode read x again:
+// three blocks an SM have no registers left for it.
+template <int V, int MODE>
+constexpr bool kKeepU = V == 1 || MODE == DP_SCAN_SIGMOID;
 template <typename T, int V, int MODE, bool TMA>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, V == 2 && kKeepU<V, MODE> ? 2 : 3)
 scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
   using F = typename Lane<T, V>::F;
-  constexpr bool kKeep = V == 1;  // word pairs have no registers left for it (spills: 89 -> 109 us)
+  constexpr bool kKeep = kKeepU<V, MODE>;
   extern __shared__ __align__(128) unsigned char smem[];
   auto &sh = *reinterpret_cast<ScanShared<F, 1> *>(smem);
   const int rank = blockIdx.x % a.cs, chain = blockIdx.x / a.cs;
@@ -391,14 +465,14 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     const int64_t t0 = base + off;
     const int n = (int)max((int64_t)0, min((int64_t)kTok, a.L - t0));
     uint32_t *xw = &sh.x[0][buf][warp][0][lane];
-    F nd[kTok];
+    F ta[kTok], td[kTok];
     const bool more = base + span < a.L;
     if constexpr (TMA) {
       if (alive) alive = mbar_wait(&sh.gate_bar[warp], phase & 1, kWaitNs);
     } else {
       stage_wait();
     }
-    load_gates<T, V, MODE>(gw, n, nd);
+    const Product<T, MODE, F> product = load_gates<T, V, MODE>(gw, n, ta, td);
     if constexpr (TMA) {
       __syncwarp();  // every lane has its gates
       if (more) fetch_gate(base + span);
@@ -407,32 +481,35 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       fetch_gate(base + span);
       fetch_x(base + span, buf ^ 1);
     }
-    uint32_t kept[kKeep ? kTok : 1];
-    sh.wmap[warp][lane] = reduce_tokens<T, V, MODE, kKeep>(xw, nd, kept);
+    Map<F> own;
+    product.get(own.a, sh.wn[warp][lane]);
+    own.H = reduce_tokens<T, V, MODE, kKeep>(xw, ta, td);
+    sh.wmap[warp][lane] = own;
     if (TMA && more) fetch_x(base + span, buf ^ 1);
     __syncthreads();
     if (warp == kWarps - 1) {
-      Map<F> r = identity<F>();
+      Map<F> r = {all_<F>(1.f), all_<F>(0.f)};
+      F rn = all_<F>(0.f);
 #pragma unroll
       for (int j = 0; j < kWarps; ++j) {
         const Map<F> w = sh.wmap[j][lane];
         sh.wmap[j][lane] = r;
-        r.H = apply(w, r.H);
-        r.n = compose(r.n, w.n);
+        follow(r, rn, w, sh.wn[j][lane]);
       }
+      r.a = marked(r.a, rn);
       F in = h;
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
-          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.n, r.H);
+          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
         if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
 #pragma unroll 4
         for (int k = 0; k < a.cs; ++k) {
           if (k == rank) in = h;
-          h = apply(sh.bmap[buf][k][lane], h);
+          h = apply_marked(sh.bmap[buf][k][lane], h);
         }
       } else {
-        h = apply(r, h);
+        h = apply_marked(r, h);
       }
       sh.carry[lane] = in;
       const int64_t tile = base / kTile + rank;
@@ -444,7 +521,7 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     T *o = at(out, t0, a.ot);
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      in = step_<MODE>(nd[i], in, Lane<T, V>::get(kKeep ? kept[i] : xw[i * 32]));
+      in = kKeep ? fma_(ta[i], in, td[i]) : step_<MODE>(ta[i], td[i], in, Lane<T, V>::get(xw[i * 32]));
       if constexpr (TMA)
         Lane<T, V>::store(reinterpret_cast<T *>(xw + i * 32), in);  // over the x that it took
       else if (i < lim)
@@ -530,14 +607,14 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     F in = all_<F>(0.f);  // the state before the tile
     if (warp == 0 && on && base + rank * kTile < a.L)
       load_state(a.saved + ((int64_t)b * tiles + base / kTile + rank) * a.D + c, in);
-    F nd[kTok];
+    F ta[kTok], td[kTok];
     const bool more = base > 0;
     if constexpr (TMA) {
       if (alive) alive = mbar_wait(&sh.gate_bar[warp], phase & 1, kWaitNs);
     } else {
       stage_wait();
     }
-    load_gates<T, V, MODE>(gw, n, nd);
+    const Product<T, MODE, F> product = load_gates<T, V, MODE>(gw, n, ta, td);
     if constexpr (TMA) {
       __syncwarp();  // every lane has its gates
       if (more) fetch_gate(base - span);
@@ -546,12 +623,14 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       fetch_gate(base - span);
       fetch_x(base - span, buf ^ 1);
     }
-    sh.wmap[warp][lane] = reduce_tokens<T, V, MODE>(xw, nd);
+    Map<F> own;
+    product.get(own.a, sh.wn[warp][lane]);
+    own.H = reduce_tokens<T, V, MODE, false>(xw, ta, td);
+    sh.wmap[warp][lane] = own;
     F Q = all_<F>(0.f);
 #pragma unroll
     for (int i = kTok - 1; i >= 0; --i) {
-      Q = add_(Q, Lane<T, V>::get(yw[i * 32]));
-      Q = fma_(nd[i], Q, Q);
+      Q = mul_(ta[i], add_(Q, Lane<T, V>::get(yw[i * 32])));
     }
     sh.wq[warp][lane] = Q;
     if (TMA && more) fetch_x(base - span, buf ^ 1);
@@ -564,33 +643,34 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
         sh.wmap[j][lane].H = in;
         in = apply(w, in);
       }
-      Map<F> r = identity<F>();
+      Map<F> r = {all_<F>(1.f), all_<F>(0.f)};
+      F rn = all_<F>(0.f);
 #pragma unroll
       for (int j = kWarps - 1; j >= 0; --j) {
-        const Map<F> w = {sh.wmap[j][lane].n, sh.wq[j][lane]};
-        sh.wmap[j][lane].n = r.n;
+        const Map<F> w = {sh.wmap[j][lane].a, sh.wq[j][lane]};
+        sh.wmap[j][lane].a = r.a;
         sh.wq[j][lane] = r.H;
-        r.H = apply(w, r.H);
-        r.n = compose(r.n, w.n);
+        follow(r, rn, w, sh.wn[j][lane]);
       }
+      r.a = marked(r.a, rn);
       F qin = q;
       if (a.cs > 1) {
         if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
         for (int k = 0; k < a.cs; ++k)
-          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.n, r.H);
+          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
         if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
 #pragma unroll 4
         for (int k = a.cs - 1; k >= 0; --k) {
           if (k == rank) qin = q;
-          q = apply(sh.bmap[buf][k][lane], q);
+          q = apply_marked(sh.bmap[buf][k][lane], q);
         }
       } else {
-        q = apply(r, q);
+        q = apply_marked(r, q);
       }
       sh.carry[lane] = qin;
     }
     __syncthreads();
-    F qi = apply(Map<F>{sh.wmap[warp][lane].n, sh.wq[warp][lane]}, sh.carry[lane]);
+    F qi = apply(Map<F>{sh.wmap[warp][lane].a, sh.wq[warp][lane]}, sh.carry[lane]);
     in = sh.wmap[warp][lane].H;
     // backwards over the tokens; the states before them are run forwards again, half of the
     // tokens at a time (registers)
@@ -599,25 +679,24 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     T *px = at(dx, t0, st), *pg = at(dg, t0, st);
     F mid = in;
 #pragma unroll
-    for (int i = 0; i < kHalf; ++i) mid = step_<MODE>(nd[i], mid, Lane<T, V>::get(xw[i * 32]));
+    for (int i = 0; i < kHalf; ++i) mid = step_<MODE>(ta[i], td[i], mid, Lane<T, V>::get(xw[i * 32]));
 #pragma unroll
     for (int half = 1; half >= 0; --half) {
       F hb[kHalf];  // the state before each token
       hb[0] = half ? mid : in;
 #pragma unroll
       for (int i = 1; i < kHalf; ++i)
-        hb[i] = step_<MODE>(nd[half * kHalf + i - 1], hb[i - 1],
+        hb[i] = step_<MODE>(ta[half * kHalf + i - 1], td[half * kHalf + i - 1], hb[i - 1],
                             Lane<T, V>::get(xw[(half * kHalf + i - 1) * 32]));
 #pragma unroll
       for (int k = kHalf - 1; k >= 0; --k) {
         const int i = half * kHalf + k;
         const F p = add_(qi, Lane<T, V>::get(yw[i * 32]));
-        qi = fma_(nd[i], p, p);
+        qi = mul_(ta[i], p);
         F ox = p, og = mul_(qi, hb[k]);
         if constexpr (MODE == DP_SCAN_SIGMOID) {
-          const F d = mul_(nd[i], all_<F>(-1.f));
-          ox = mul_(p, d);
-          og = mul_(mul_(qi, d), fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k]));
+          ox = mul_(p, td[i]);
+          og = mul_(mul_(qi, td[i]), fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k]));
         }
         if constexpr (TMA) {  // over the dout and the x that they took
           Lane<T, V>::store(reinterpret_cast<T *>(yw + i * 32), ox);
@@ -654,8 +733,14 @@ scan_step_kernel(const float *state, float *state_out, const T *x, const T *gate
   if (i >= n) return;
   const int64_t b = i / D;
   const int c = (int)(i - b * D);
-  const float nd = neg_drop<float, MODE>(to_f32(gate[b * gs + c])), xv = to_f32(x[b * xs + c]);
-  const float r = step_<MODE>(nd, state[i], xv);
+  const float g = to_f32(gate[b * gs + c]), xv = to_f32(x[b * xs + c]), h = state[i];
+  // the state goes on from call to call, so an open gate's 1 - a counts here
+  float r, ta, td;
+  gate_<float, MODE>(g, ta, td);
+  if (MODE == DP_SCAN_SIGMOID)
+    r = ta < 0.5f ? fmaf(ta, h, td * xv) : fmaf(td, xv - h, h);
+  else
+    r = fabsf(g) < 0.6931472f ? h + fmaf(expm1f(g), h, xv) : fmaf(ta, h, xv);
   state_out[i] = r;
   out[b * os + c] = from_f32<T>(r);
 }

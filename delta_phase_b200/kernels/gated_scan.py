@@ -105,7 +105,7 @@ def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
     where the channel stride is 1); initial_state (B, D) float32 or None, never modified.  Any L up to 2^30.
     Returns ``(out (B, L, D) of x's dtype, h_L (B, D) float32)``; the state is float32
     throughout and the order of all sums depends on L alone.  A value that is not finite stays in
-    its channel, from its token on (an infinite state continues as NaN).  Differentiable once when autograd
+    its channel, from its token on (an infinite state may continue as NaN).  Differentiable once when autograd
     records and an input requires grad.  A backward pass that is captured into a CUDA graph
     needs, as any in torch, leaves that no eager graph still refers to.
     """

@@ -395,7 +395,7 @@ DP_API int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int dy_d
  *                  dp_scan_bwd; or NULL
  *   strides[6]   : {sb, st} of x, gate, out
  * The state is float32 throughout; the order of all sums is fixed by L.  0 <= L <= 2^30.
- * The kernels compute h - (1 - a) h for a h: a state that has become infinite continues as NaN.
+ * A state that has become infinite may continue as NaN.
  * Made for 0 <= a <= 1; larger a are computed too, but a product of a over 128 tokens that
  * overflows float32 may turn a zero state into NaN.  Token strides up to 2^28 elements.
  */

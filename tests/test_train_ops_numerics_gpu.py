@@ -10,7 +10,7 @@ import torch
 
 import delta_phase_b200 as dp
 from delta_phase_b200 import _capi
-from delta_phase_b200.kernels import gated_scan
+from delta_phase_b200.kernels import gated_scan, gated_scan_step
 from test_train_ops_gpu import BF16, F16, F32, U, check, distill_case, distill_inputs
 
 pytestmark = pytest.mark.gpu
@@ -127,3 +127,105 @@ def test_scan_open_gates_decay_as_defined(dtype, gate, mode, D):
     check(dg, torch.full_like(dg, each, dtype=torch.float64), 2 * each * rel, "dgate")
     # with a rounded to float32 the first two would fail (-2^-19 loses next to nothing that way)
     assert gate == -2.0 ** -19 or abs(a32 ** L / rest - 1) > rel
+
+
+@pytest.mark.parametrize("D", [8, 37])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("gate", [16.0, 16.25, 17.0])
+def test_scan_open_gates_hold_the_fixed_point_for_a_million_tokens(gate, dtype, D):
+    """What a tile adds to a state at its fixed point is 0 but for the roundings of its own small terms,
+    so the state does not collect a rounding a tile."""
+    L = 1 << 20
+    x = torch.ones(1, L, D, device="cuda", dtype=dtype)
+    g = torch.full((1, L, D), gate, device="cuda", dtype=dtype)
+    _, fin = gated_scan(x, g, torch.ones(1, D, device="cuda"), gate_mode="sigmoid")
+    # n + H of a tile: both 128 d within 128 roundings; the state runs to -H / n at most
+    assert float((fin - 1).abs().max()) <= 2 * _capi.scan_tile() * U
+
+
+# ---------------------------------------------------------------- gated recurrence, closed gates
+def a_of(gate, mode):
+    g = gate.double()
+    return torch.sigmoid(g) if mode == "sigmoid" else torch.exp(g)
+
+
+@pytest.mark.parametrize("mode", ["decay", "sigmoid"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cuts", [(0,), (5,), (127,), (128,), (699,), (20, 25), (100, 300), (3, 130, 690)])
+def test_scan_closed_gates_keep_the_digits_of_a(cuts, dtype, mode):
+    """Gates of -1 to -40 at some tokens, open ones elsewhere, no input: what is left of the state, and
+    the gradients of the gates and of the initial state, to the digits of their own value."""
+    L, D = 700, 79
+    closed = -torch.linspace(1, 40, D, device="cuda").to(dtype) / len(cuts)
+    closed = closed.to(dtype)
+    open_ = math.inf if mode == "sigmoid" else 0.0
+    gate = torch.full((1, L, D), open_, device="cuda", dtype=dtype)
+    for t in cuts:
+        gate[:, t] = closed
+    x = torch.zeros(1, L, D, device="cuda", dtype=dtype).requires_grad_(True)
+    h0 = torch.linspace(0.5, 3.0, D, device="cuda")[None].requires_grad_(True)
+    leaf = gate.clone().requires_grad_(True)
+    out, fin = gated_scan(x, leaf, h0, gate_mode=mode)
+    _, dg, dh = torch.autograd.grad(fin, (x, leaf, h0), torch.ones_like(fin))
+    a = a_of(closed, mode)[None]
+    # relative: exp within 4 U (8 U and 2 |gate| U from the hardware exponential), the factor cut to
+    # 23 bits 2 U, a product and a state 2 U each; the open tokens change nothing
+    rel = (24 * len(cuts) + 2 * len(cuts) * closed.double().abs()[None]) * U
+    left = h0.detach().double()
+    start = 0
+    for t in cuts:
+        if t > start:
+            check(out[:, start:t].detach(), left[:, None].expand(1, t - start, D), (rel * left)[:, None], t)
+        left, start = left * a, t
+    check(out[:, start:].detach(), left[:, None].expand(1, L - start, D), (rel * left)[:, None], "out")
+    check(fin.detach(), left, rel * left, "h_L")
+    check(dh, left / h0.detach().double(), rel * left / h0.detach().double(), "dh0")
+    for t in cuts:
+        want = left * (torch.sigmoid(-closed.double()) if mode == "sigmoid" else 1.0)
+        check(dg[:, t], want, 2 * rel * want, "dgate")
+
+
+@pytest.mark.parametrize("mode", ["decay", "sigmoid"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_closed_gates_against_a_large_state(dtype, mode):
+    """A state far larger than the inputs, then a closed gate: out is a h + u to its own digits."""
+    D = 64
+    x = torch.linspace(0.25, 1.0, D, device="cuda").to(dtype).expand(1, 300, D)
+    for at in (0, 7, 128, 200):
+        for g in (-8.0, -20.0, -30.0, -math.inf):
+            gate = torch.full((1, 300, D), math.inf if mode == "sigmoid" else 0.0, device="cuda", dtype=dtype)
+            gate[:, at] = g
+            xs = x.clone()
+            xs[:, :at] = 0
+            h0 = torch.full((1, D), 1e6, device="cuda")
+            out, _ = gated_scan(xs, gate, h0, gate_mode=mode)
+            a = float(a_of(torch.tensor(g), mode))
+            u = xs[0, at].double() * (float(torch.sigmoid(-torch.tensor(g).double())) if mode == "sigmoid" else 1.0)
+            want = a * 1e6 + u
+            check(out[0, at], want, (32 + 2 * min(abs(g), 100)) * U * want, (at, g))
+            o, h = gated_scan_step(h0, xs[:, at], gate[:, at], gate_mode=mode)
+            check(o[0], want, 32 * U * want, (at, g))
+            check(h[0], want, 32 * U * want, (at, g))
+
+
+@pytest.mark.parametrize("mode", ["decay", "sigmoid"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_gates_on_both_sides_of_a_half(dtype, mode):
+    """Gates around the one where the factor changes its form; in decay mode growth, too."""
+    D, L = 66, 40
+    mid = 0.0 if mode == "sigmoid" else -math.log(2.0)
+    gate = (torch.linspace(-0.02, 0.02, D, device="cuda") + mid).to(dtype).expand(1, L, D).clone()
+    x = torch.zeros(1, L, D, device="cuda", dtype=dtype)
+    h0 = torch.ones(1, D, device="cuda")
+    _, fin = gated_scan(x, gate, h0, gate_mode=mode)
+    want = a_of(gate[:, 0], mode) ** L
+    check(fin, want, want * L * 96 * U)  # 16-bit gates: 1 - a within 64 U
+    if mode == "decay":
+        for lo, hi, n in ((1e-5, 1e-3, 4000), (0.1, 3.0, 12)):
+            gate = torch.linspace(lo, hi, D, device="cuda").to(dtype).expand(1, n, D)
+            x = torch.zeros(1, n, D, device="cuda", dtype=dtype)
+            _, fin = gated_scan(x, gate, h0)
+            want = torch.exp(n * gate[:, 0].double())
+            # 2 U a tile or token and 8 U (64 U from the hardware exponential) of each n, or of a
+            rel = (4 * n / 16 + 32 + n * 96 * gate[:, 0].double().expm1()) * U
+            check(fin, want, want * rel)
