@@ -502,6 +502,7 @@ def layernorm_bwd(s, dy, ln_w, stats, grad_sum=None, dx=None, grad_residual=None
 
 
 DP_SCAN_DECAY, DP_SCAN_SIGMOID = 0, 1
+SCAN_MAX_TOKEN_STRIDE = 1 << 28  # of dp_scan_fwd and dp_scan_bwd, in elements
 _scan_tile = None
 
 

@@ -30,6 +30,17 @@ def _unit(t):
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _seq(t):
+    """A (B, L, D) tensor as the kernels read it: unit channel stride, token strides within their
+    32 bits (a copy where it has neither)."""
+    t = _unit(t)
+    if t.stride(1) > _capi.SCAN_MAX_TOKEN_STRIDE:
+        t = t.contiguous()
+        if t.stride(1) > _capi.SCAN_MAX_TOKEN_STRIDE:  # one token: its stride moves nothing
+            t = t.as_strided(t.shape, (t.stride(0), t.shape[2], 1))
+    return t
+
+
 def _check_inputs(x, gate, dims, what):
     if x.dim() != dims or gate.shape != x.shape or x.shape[-1] < 1:
         raise ValueError(f"x and gate must both be {what}")
@@ -55,7 +66,7 @@ def _forward(x, gate, initial_state, mode, keep):
     if keep:
         tile = _capi.scan_tile()
         saved = final.new_empty((B, (L + tile - 1) // tile, D))
-    _capi.scan_fwd(_unit(x), _unit(gate), mode, h0, out, final, saved)
+    _capi.scan_fwd(_seq(x), _seq(gate), mode, h0, _seq(out), final, saved)
     return out, final, saved
 
 
@@ -84,10 +95,10 @@ def _backward(ctx, grad_out, grad_final):
         return None, None, None, None
     need_x, need_gate, need_state, _ = ctx.needs_input_grad
     dx, dg = _like(x), _like(x)
-    go = torch.zeros_like(dx) if grad_out is None else _unit(grad_out)
+    go = torch.zeros_like(dx) if grad_out is None else _seq(grad_out)
     gf = None if grad_final is None else grad_final.contiguous()
     dh = saved.new_empty((x.shape[0], x.shape[2])) if need_state else None
-    _capi.scan_bwd(_unit(x), _unit(gate), go, ctx.mode, saved, gf, dx, dg, dh)
+    _capi.scan_bwd(_seq(x), _seq(gate), go, ctx.mode, saved, gf, dx, dg, dh)
     return dx if need_x else None, dg if need_gate else None, dh, None
 
 
@@ -102,7 +113,7 @@ def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
     * ``gate_mode="sigmoid"``: h_t = sigmoid(gate_t) h_{t-1} + (1 - sigmoid(gate_t)) x_t
 
     x, gate (B, L, D) of one dtype (float32 / bfloat16 / float16; any strides, without a copy
-    where the channel stride is 1); initial_state (B, D) float32 or None, never modified.  Any L up to 2^30.
+    where the channel stride is 1 and tokens are at most 2^28 elements apart); initial_state (B, D) float32 or None, never modified.  Any L up to 2^30.
     Returns ``(out (B, L, D) of x's dtype, h_L (B, D) float32)``; the state is float32
     throughout and the order of all sums depends on L alone.  A value that is not finite stays in
     its channel, from its token on (an infinite state may continue as NaN).  Differentiable once when autograd

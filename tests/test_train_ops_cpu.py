@@ -2,6 +2,7 @@
 the C entry points check their arguments before they touch a device, the Python entry points
 before they launch.  No GPU needed."""
 import ctypes
+import importlib
 
 import pytest
 import torch
@@ -184,3 +185,17 @@ def test_step_output_rows_must_not_share_memory():
     z = torch.zeros
     with pytest.raises(ValueError, match="out"):
         dp.gated_scan_step(z(2, 8), z(2, 8), z(2, 8), out=z(1, 8).expand(2, 8))
+
+
+def test_scan_sequences_reach_the_kernels_within_their_strides():
+    seq = importlib.import_module("delta_phase_b200.kernels.gated_scan")._seq
+    far = (1 << 28) + 8
+    for shape, stride in (((1, 2, 8), (8, far, 1)), ((3, 1, 8), (8, far, 1)), ((1, 1, 8), (far, far, 1)),
+                          ((2, 5, 8), (40, 8, 1)), ((2, 5, 8), (8, 16, 1)), ((2, 5, 1), (40, 8, 7)),
+                          ((2, 0, 8), (8, far, 1))):
+        x = torch.empty_strided(shape, stride, dtype=torch.bfloat16)
+        if x.numel():
+            x[:] = torch.arange(x.numel(), dtype=torch.bfloat16).view(shape)
+        s = seq(x)
+        assert s.shape == x.shape and s.stride(1) <= 1 << 28 and torch.equal(s, x)
+        assert (s.data_ptr() == x.data_ptr()) == (stride[1] != far or shape[1] != 2)

@@ -229,3 +229,21 @@ def test_scan_gates_on_both_sides_of_a_half(dtype, mode):
             # 2 U a tile or token and 8 U (64 U from the hardware exponential) of each n, or of a
             rel = (4 * n / 16 + 32 + n * 96 * gate[:, 0].double().expm1()) * U
             check(fin, want, want * rel)
+
+
+# ---------------------------------------------------------------- gated recurrence, layouts
+def test_scan_tokens_far_apart():
+    """Tokens further apart than the kernels' 32 bits of bytes, and one token whose stride moves nothing."""
+    far = (1 << 28) + 8
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for shape, stride in (((1, 2, 8), (8, far, 1)), ((3, 1, 8), (8, far, 1))):
+        plain = torch.randn(shape, generator=gen, device="cuda").to(BF16)
+        x = torch.empty_strided(shape, stride, dtype=BF16, device="cuda")
+        x.copy_(plain)
+        gate = -plain.abs()
+        ref_leaf, leaf = plain.clone().requires_grad_(True), x.requires_grad_(True)
+        ref, rf = gated_scan(ref_leaf, gate)
+        out, fin = gated_scan(leaf, gate)
+        assert torch.equal(out, ref) and torch.equal(fin, rf)
+        dout = torch.empty_strided(shape, stride, dtype=BF16, device="cuda").copy_(plain)
+        assert torch.equal(torch.autograd.grad(out, leaf, dout)[0], torch.autograd.grad(ref, ref_leaf, plain)[0])
