@@ -39,6 +39,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <string>
 #include <type_traits>
 
@@ -875,6 +876,26 @@ int scan_dispatch(const ScanArgs &a, int dtype, int mode, bool pairs, cudaStream
   return pairs ? scan_run<BWD, __half, 2>(a, mode, st, what) : scan_run<BWD, __half, 1>(a, mode, st, what);
 }
 
+// (B, D) values of `size` bytes, rows `row` bytes apart.
+struct Rows {
+  const void *p;
+  int64_t row, size;
+};
+// An output may lie on another tensor element for element (a thread reads its channel of all inputs
+// before it writes it), but share no memory with it otherwise.
+bool scan_clash(const Rows &o, const Rows &t, int B, int D) {
+  const int64_t p = (int64_t)reinterpret_cast<uintptr_t>(o.p), q = (int64_t)reinterpret_cast<uintptr_t>(t.p);
+  const int64_t pw = o.size * D, qw = t.size * D, pr = (B - 1) * o.row, qr = (B - 1) * t.row;
+  if (p == q && o.size == t.size && pr == qr) return false;
+  if (p + std::max<int64_t>(pr, 0) + pw <= q + std::min<int64_t>(qr, 0) ||
+      q + std::max<int64_t>(qr, 0) + qw <= p + std::min<int64_t>(pr, 0))
+    return false;
+  if (B == 1 || o.row != t.row || o.row == 0) return true;
+  // slices of one buffer's rows lie between one another
+  const int64_t row = std::abs(o.row), off = ((q - p) % row + row) % row;
+  return off < pw || off + qw > row;
+}
+
 }  // namespace
 }  // namespace dp
 
@@ -946,6 +967,13 @@ extern "C" int dp_scan_step(const float *state_in, float *state_out, const void 
   if (B == 0) return DP_OK;
   DP_REQUIRE(state_in && state_out && x && gate && out && strides, DP_ERR_INVALID_ARGUMENT,
              "dp_scan_step: null pointer");
+  const int64_t e = (int64_t)dtype_size(dtype);
+  const Rows outs[] = {{state_out, 4ll * D, 4}, {out, strides[2] * e, e}};
+  const Rows ins[] = {outs[1], {state_in, 4ll * D, 4}, {x, strides[0] * e, e}, {gate, strides[1] * e, e}};
+  for (int k = 0; k < 2; ++k)
+    for (int j = k; j < 4; ++j)
+      DP_REQUIRE(!scan_clash(outs[k], ins[j], B, D), DP_ERR_INVALID_ARGUMENT,
+                 "dp_scan_step: state_out or out overlaps another tensor");
   const int64_t n = (int64_t)B * D, blocks = (n + 255) / 256;
   DP_REQUIRE(blocks < (1ll << 31), DP_ERR_UNSUPPORTED, "dp_scan_step: too many channels");
   return dispatch_dtype(dtype, [&](auto t) {

@@ -131,7 +131,8 @@ def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
 
 def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None):
     """One token of :func:`gated_scan`: state (B, D) float32, x and gate (B, D).  Returns
-    ``(out (B, D) of x's dtype, new_state)``; ``state_out=state`` updates the state in place.
+    ``(out (B, D) of x's dtype, new_state)``; ``state_out=state`` updates the state in place.  An
+    output may lie on another tensor of its type element for element, but not overlap it otherwise.
     Not differentiable (like ``decode_step``)."""
     mode = _mode(gate_mode)
     _check_inputs(x, gate, 2, "(B, D)")

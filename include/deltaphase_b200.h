@@ -417,8 +417,10 @@ DP_API int dp_scan_bwd(const void *x, const void *gate, const void *grad_out, in
 
 /*
  * One token of the recurrence: state_out = a state_in + u, out = state_out.
- *   state_in, state_out : (B, D) float32, contiguous; may alias (in-place update)
+ *   state_in, state_out : (B, D) float32, contiguous; may be the same (in-place update)
  *   x, gate, out        : (B, D) of `dtype`, unit channel stride;  strides[3] : sb of x, gate, out
+ * state_out and out may lie on another tensor element for element (the same address, type and
+ * strides); where they overlap one otherwise the call is refused.
  */
 DP_API int dp_scan_step(const float *state_in, float *state_out, const void *x, const void *gate, int dtype,
                     int mode, void *out, int B, int D, const int64_t *strides, void *stream);

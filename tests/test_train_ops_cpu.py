@@ -199,3 +199,31 @@ def test_scan_sequences_reach_the_kernels_within_their_strides():
         s = seq(x)
         assert s.shape == x.shape and s.stride(1) <= 1 << 28 and torch.equal(s, x)
         assert (s.data_ptr() == x.data_ptr()) == (stride[1] != far or shape[1] != 2)
+
+
+def test_step_outputs_must_not_overlap_other_tensors():
+    """dp_scan_step refuses outputs that overlap another tensor, except element for element, before it
+    touches a device; addresses that are never read, 4 rows of 8 values."""
+    f = _capi.lib().dp_scan_step
+    B, D = 4, 8
+
+    def refused(h=1 << 20, h2=2 << 20, x=3 << 20, gate=4 << 20, out=5 << 20, dt=0, strides=(8, 8, 8), B=B):
+        rc = f(h, h2, x, gate, dt, 0, out, B, D, (ctypes.c_int64 * 3)(*strides), None)
+        assert rc in (1, 4)  # 4: launched, without a device here
+        assert (rc == 1) == (b"overlaps" in _capi.lib().dp_last_error())
+        return rc == 1
+
+    P, row = 1 << 20, 32
+    if torch.cuda.is_available():
+        pytest.skip("calls that are not refused would run")
+    assert not refused() and not refused(h2=P) and not refused(out=3 << 20) and not refused(out=4 << 20)
+    assert refused(h2=P + 4) and refused(h2=P - row) and refused(h2=P + 3 * row) and not refused(h2=P + 4 * row)
+    assert refused(h2=(3 << 20) + row) and refused(out=P + 8) and refused(out=(2 << 20) - 4)
+    assert refused(out=P, dt=1)  # 16-bit outputs on a float32 state
+    # slices of the rows of one buffer: x | gate | out, 24 values a row, then out one value too far left
+    for dt, e in ((0, 4), (1, 2)):
+        assert not refused(x=3 << 20, gate=(3 << 20) + 8 * e, out=(3 << 20) + 16 * e, dt=dt, strides=(24, 24, 24))
+        assert refused(x=3 << 20, gate=(3 << 20) + 8 * e, out=(3 << 20) + 15 * e, dt=dt, strides=(24, 24, 24))
+        assert refused(x=3 << 20, out=(3 << 20) + 17 * e, dt=dt, strides=(24, 8, 24))
+    assert refused(x=3 << 20, out=3 << 20, strides=(0, 8, 8)) and refused(x=3 << 20, out=3 << 20, strides=(16, 8, 8))
+    assert not refused(x=3 << 20, out=3 << 20, strides=(0, 8, 8), B=1)
