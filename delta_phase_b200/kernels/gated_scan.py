@@ -138,6 +138,7 @@ def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None)
     _check_inputs(x, gate, 2, "(B, D)")
     B, D = x.shape
     _check_state(state, B, D, "state")
+    given = [t for t in (state_out, out) if t is not None]
     if state_out is None:
         state_out = _like(state)
     else:
@@ -150,4 +151,6 @@ def gated_scan_step(state, x, gate, gate_mode="decay", state_out=None, out=None)
             (B > 1 and out.stride(0) < D):
         raise ValueError("out must be a (B, D) tensor of x's dtype with unit channel stride and rows apart")
     _capi.scan_step(state.contiguous(), state_out, _unit(x), _unit(gate), mode, out)
+    if given:  # autograd notices a change of what it has saved
+        torch.autograd.graph.increment_version(given)
     return out, state_out

@@ -231,6 +231,22 @@ def test_scan_gates_on_both_sides_of_a_half(dtype, mode):
             check(fin, want, want * rel)
 
 
+def test_scan_step_in_place_is_noticed_by_autograd():
+    """A state that a graph has saved and the step then overwrites."""
+    x = torch.randn(2, 30, 16, device="cuda", requires_grad=True)
+    gate = -torch.rand(2, 30, 16, device="cuda")
+    for name in ("state_out", "out"):
+        _, h = gated_scan(x, gate)
+        loss = h.square().sum()  # saves h
+        with torch.no_grad():
+            gated_scan_step(h, x[:, 0], gate[:, 0], **{name: h})
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
+    with torch.inference_mode():
+        h = torch.zeros(2, 16, device="cuda")
+        gated_scan_step(h, x[:, 0], gate[:, 0], state_out=h)
+
+
 # ---------------------------------------------------------------- gated recurrence, layouts
 def test_scan_tokens_far_apart():
     """Tokens further apart than the kernels' 32 bits of bytes, and one token whose stride moves nothing."""
