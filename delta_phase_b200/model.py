@@ -178,21 +178,33 @@ class DeltaPhaseModel(nn.Module):
 
     def distill_step(self, input_ids: torch.Tensor, teacher_index: torch.Tensor, teacher_logits: torch.Tensor,
                      temperature: float = 1.0, weight: Optional[torch.Tensor] = None,
-                     states: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
+                     states: Optional[List[torch.Tensor]] = None, loss_scale: float = 1.0) -> torch.Tensor:
         """Forward and backward pass of one distillation step: logits of ``input_ids`` (B, L)
         against the teacher's top logits ``teacher_index`` / ``teacher_logits`` (B, L, K), loss
         and logit gradient in one pass (:func:`distill_loss_and_grad`).  ``weight`` (B, L) scales
         each token's loss (0 for padding); None takes the mean over the tokens.  Parameter
-        gradients are accumulated as by ``loss.backward()``; returns the detached loss, summed
-        over the tokens.  There is no counterpart in the reference."""
+        gradients are accumulated as by ``(loss_scale * loss).backward()``; returns the detached
+        loss, summed over the tokens, without the scale.  float16 logits need one: most gradients
+        of a mean over many tokens are below float16's range.  With a GradScaler it is
+        ``scaler.scale(torch.ones((), device=...))`` (a number or a tensor of one value).  There
+        is no counterpart in the reference."""
         if not torch.is_grad_enabled():
             raise RuntimeError("distill_step computes gradients: call it with gradients enabled")
+        scaled = isinstance(loss_scale, torch.Tensor) or loss_scale != 1.0
+        if isinstance(loss_scale, torch.Tensor):
+            if loss_scale.numel() != 1:
+                raise ValueError("loss_scale must be one value")
+            loss_scale = loss_scale.detach().to(device=input_ids.device, dtype=torch.float32).reshape(())
+        elif not 0.0 < loss_scale < float("inf"):
+            raise ValueError("loss_scale must be positive and finite")
         logits = self.forward(input_ids, states)
         if weight is None:
             weight = torch.full(input_ids.shape, 1.0 / max(1, input_ids.numel()), device=logits.device)
+        if scaled:
+            weight = weight * loss_scale
         loss, grad = distill_loss_and_grad(logits, teacher_index, teacher_logits, temperature, weight)
         logits.backward(grad)
-        return loss.sum()
+        return loss.sum() / loss_scale if scaled else loss.sum()
 
     def print_substrate_report(self):
         print("=" * 72)

@@ -181,6 +181,14 @@ def test_sizes_past_the_c_interface_are_refused():
             dp.distill_loss(one.expand(*lead, V), idx.expand(*lead, K), one.expand(*lead, K))
 
 
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("nan"), float("inf"), torch.ones(2)])
+def test_distill_step_refuses_loss_scales(scale):
+    model = dp.DeltaPhaseModel(dp.DeltaPhaseConfig(dim=16, emb_dim=8, n_layers=1, n_heads=2, vocab_size=32))
+    idx = torch.zeros(1, 4, 2, dtype=torch.long)
+    with pytest.raises(ValueError, match="loss_scale"):
+        model.distill_step(torch.zeros(1, 4, dtype=torch.long), idx, idx.float(), loss_scale=scale)
+
+
 def test_step_output_rows_must_not_share_memory():
     z = torch.zeros
     with pytest.raises(ValueError, match="out"):

@@ -11,7 +11,7 @@ import torch
 import delta_phase_b200 as dp
 from delta_phase_b200 import _capi
 from delta_phase_b200.kernels import gated_scan, gated_scan_step
-from test_train_ops_gpu import BF16, F16, F32, U, check, distill_case, distill_inputs
+from test_train_ops_gpu import BF16, F16, F32, U, check, distill_case, distill_inputs, distill_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -77,6 +77,31 @@ def test_distill_likely_entries_at_the_lowest_logit(N, V):
     teacher[3] = 0.0
     loss, _ = distill_case(z, index, teacher, 1.0, None)
     assert 1e38 < float(loss[3]) < math.inf
+
+
+@pytest.mark.parametrize("as_tensor", [False, True])
+def test_model_distill_step_keeps_float16_gradients_in_range(as_tensor, monkeypatch):
+    """The mean over many tokens puts most of float16 logits' gradients below the type's range; with a
+    loss scale they reach the parameters, and the loss comes back without it."""
+    V, B, L, K, scale = 4000, 4, 512, 8, 2.0 ** 20
+    model = dp.DeltaPhaseModel(dp.DeltaPhaseConfig(dim=16, emb_dim=8, n_layers=1, n_heads=2, vocab_size=V)).cuda()
+    z, index, teacher, _ = distill_inputs(B * L, V, K, F16, 3)
+    leaf = z.view(B, L, V).clone().requires_grad_(True)
+    monkeypatch.setattr(model, "forward", lambda ids, states=None: leaf * 1.0)
+    args = torch.zeros(B, L, dtype=torch.long, device="cuda"), index.view(B, L, K), teacher.view(B, L, K), 1.5
+    plain = model.distill_step(*args)
+    tiny = float((leaf.grad == 0).double().mean())
+    leaf.grad = None
+    s = torch.amp.GradScaler("cuda", init_scale=scale).scale(torch.ones((), device="cuda")) if as_tensor else scale
+    loss = model.distill_step(*args, loss_scale=s)
+    w = torch.full((B * L,), scale / (B * L), device="cuda")
+    rl, el, rd, ed = distill_ref(z, index, teacher, 1.5, w)
+    check(leaf.grad.view(B * L, V), rd, ed, "dz")
+    lost = (leaf.grad.view(B * L, V) == 0) & (rd.abs() > 2.0 ** -24)
+    assert tiny > 0.5 and not bool(lost.any())
+    # a sum of 2048 float32 losses: 64 roundings at most in a row, and the two products
+    assert abs(float(loss) - float(rl.sum()) / scale) <= (float(el.sum()) + 70 * U * float(rl.abs().sum())) / scale
+    assert abs(float(loss) - float(plain)) <= 140 * U * float(rl.abs().sum()) / scale + 2 * float(el.sum()) / scale
 
 
 # ---------------------------------------------------------------- gated recurrence, open gates
