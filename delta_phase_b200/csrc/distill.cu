@@ -48,7 +48,7 @@ constexpr int kDiMaxVec = 8;  // 16-byte vectors of a row per thread, at most
 constexpr int kDiMaxThreads = 512;
 constexpr int kDiMaxK = 1024;
 constexpr int kDiMaxCluster = 16;
-constexpr int kDiMaxSlices = 32;  // blocks a row in any launch, at most
+constexpr int64_t kDiMaxRows = 1 << 26;  // of a call, below this
 constexpr int kDiSms = 148;
 constexpr int kDiWarpRows = 4;    // rows of a block where a warp holds a row
 constexpr int kDiLossThreads = 256;
@@ -788,6 +788,7 @@ distill_grad_kernel(const DistillArgs a) {
 template <void (*KERN)(const DistillArgs)>
 int distill_run(const DistillArgs &a, int64_t blocks, int threads, size_t smem, size_t most, int cluster,
                 cudaStream_t st) {
+  DP_REQUIRE(blocks < (1ll << 31), DP_ERR_UNSUPPORTED, "dp_distill: too many rows of this width");
   // more than 48 KB of shared memory and 16-block clusters (a non-portable size): opt in once
   static thread_local bool opted[64] = {};
   int dev = 0;
@@ -911,7 +912,7 @@ int distill_args(dp::DistillArgs &a, const char *what, const void *z, int z_dtyp
   if (a.rows == 0) return DP_OK;
   DP_REQUIRE(z && index && teacher && strides, DP_ERR_INVALID_ARGUMENT, w + "null pointer");
   DP_REQUIRE(z != dz, DP_ERR_INVALID_ARGUMENT, w + "dz must not be z");
-  DP_REQUIRE(a.rows * kDiMaxSlices < (1ll << 31), DP_ERR_UNSUPPORTED, w + "too many rows");
+  DP_REQUIRE(a.rows < kDiMaxRows, DP_ERR_UNSUPPORTED, w + "too many rows");
   a.z = z, a.sb = strides[0], a.st = strides[1], a.index = index, a.index64 = index_bytes == 8, a.teacher = teacher;
   a.teacher_dt = teacher_dtype, a.weight = weight, a.dz = dz;
   a.tau = tau, a.c = 1.4426950408889634f / tau;

@@ -442,7 +442,8 @@ DP_API int dp_scan_step(const float *state_in, float *state_out, const void *x, 
  *             dp_distill_bwd; or NULL
  *   dz      : (B, L, V) of z_dtype, contiguous, not z; or NULL
  *   strides[2] : {sb, st} of z
- * Limits: 1 <= K <= 1024; V times the element size below 1 MiB; 1e-30 < tau < 1e30.
+ * Limits: 1 <= K <= 1024; V times the element size below 1 MiB; 1e-30 < tau < 1e30; fewer than 2^26
+ * rows, and fewer than 2^31 blocks of them (a row of z above 16 KB may take several).
  */
 DP_API int dp_distill(const void *z, int z_dtype, const void *index, int index_bytes,
                   const void *teacher, int teacher_dtype, const float *weight, float tau, float *loss,

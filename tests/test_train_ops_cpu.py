@@ -235,3 +235,11 @@ def test_step_outputs_must_not_overlap_other_tensors():
         assert refused(x=3 << 20, out=(3 << 20) + 17 * e, dt=dt, strides=(24, 8, 24))
     assert refused(x=3 << 20, out=3 << 20, strides=(0, 8, 8)) and refused(x=3 << 20, out=3 << 20, strides=(16, 8, 8))
     assert not refused(x=3 << 20, out=3 << 20, strides=(0, 8, 8), B=1)
+
+
+def test_distill_more_blocks_than_a_launch_holds():
+    """Rows that are few enough, but so wide that the gradient from the sums takes 64 blocks for each."""
+    L, P2 = _capi.lib(), 2 * P
+    for rows in ((1 << 26) - 1, 1 << 25):
+        rc = L.dp_distill_bwd(P, 0, P, 8, P, 0, None, P, None, 1.0, P2, 1, rows, 262136, 4, _strides(2), None)
+        assert rc == 2 and b"too many rows" in L.dp_last_error()
