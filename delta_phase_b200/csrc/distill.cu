@@ -47,6 +47,7 @@ using namespace ptx;
 constexpr int kDiMaxVec = 8;  // 16-byte vectors of a row per thread, at most
 constexpr int kDiMaxThreads = 512;
 constexpr int kDiMaxK = 1024;
+constexpr float kDiShrink = 1.f / kDiMaxK;
 constexpr int kDiMaxCluster = 16;
 constexpr int64_t kDiMaxRows = 1 << 26;  // of a call, below this
 constexpr int kDiSms = 148;
@@ -425,6 +426,8 @@ __device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const 
   const int tid = g.tid, n = g.n, lane = threadIdx.x & 31, warps = n >> 5;
   const float c = a.c;
   const bool entries = tid - lane < a.K;  // a warp that has some
+  constexpr bool kWhole = std::is_same_v<G, WarpGroup>;  // the warp has the whole row
+  float d = 0.f;
   w.tm = -INFINITY, w.ts = 0.f;
   if (entries) {
     float tm = -INFINITY;
@@ -440,7 +443,11 @@ __device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const 
     }
     w.tm = di_warp_redux_max(tm);
     const float t0 = w.tm == -INFINITY ? 0.f : w.tm;
-    for (int k = tid; k < a.K; k += n) w.ts += di_ex2((e.t[k] - t0) * c);
+    for (int k = tid; k < a.K; k += n) {
+      const float t = e.t[k] - t0, x = di_ex2(t * c);
+      w.ts += x;
+      if (kWhole && x != 0.f) d = fmaf(x * kDiShrink, t - (e.z[k] - w.m), d);
+    }
     w.ts = di_warp_sum(w.ts);
   }
   if (a.dz) e.clear(tid, n);
@@ -471,16 +478,17 @@ __device__ __forceinline__ Sums di_sums(const DistillArgs &a, const G &g, const 
   if (rank == 0 && tid < 32) {
     // sum p (log p - log q) = sum p ((t - TM) - (z - M)) / tau - log TS + log S; times tau^2
     // without tau^2 or 1 / tau, which may leave the float32 range.  One warp forms it from the
-    // row's own maxima: a warp's maximum may be that of masked logits or entries only, and
-    // differences from it keep no digits of z.  p, not its multiple, so that the sum of masked
-    // logits stays in range; a p that is 0 counts nothing, whatever z is.
+    // row's own maxima: a part's maximum may be that of masked logits or entries only, and
+    // differences from it keep no digits of z.  p, or its multiple made small, so that the sum of
+    // masked logits stays in range; a p that is 0 counts nothing, whatever z is.
     const float inv_TS = di_rcp(q.TS);
-    float d = 0.f;
-    for (int k = tid; k < a.K; k += 32) {
-      const float t = e.t[k] - q.TM, p = di_ex2(t * c) * inv_TS;
-      if (p != 0.f) d = fmaf(p, t - (e.z[k] - q.M), d);
-    }
+    if (!kWhole)
+      for (int k = tid; k < a.K; k += 32) {
+        const float t = e.t[k] - q.TM, p = di_ex2(t * c) * inv_TS;
+        if (p != 0.f) d = fmaf(p, t - (e.z[k] - q.M), d);
+      }
     d = di_warp_sum(d);
+    if (kWhole) d = d * inv_TS / kDiShrink;
     if (tid == 0) {
       a.loss[r.row] = q.empty ? 0.f : weight * (a.tau * (d + a.tau * (logf(q.S) - logf(q.TS))));
       if (a.stats) a.stats[r.row] = make_float4(q.M, q.S, q.TM, q.TS);
