@@ -634,7 +634,6 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       Q = mul_(ta[i], add_(Q, Lane<T, V>::get(yw[i * 32])));
     }
     sh.wq[warp][lane] = Q;
-    if (TMA && more) fetch_x(base - span, buf ^ 1);
     __syncthreads();
     if (warp == 0) {
       // in the place of each warp's maps the state before it and the map of the warps behind it
@@ -671,6 +670,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       sh.carry[lane] = qin;
     }
     __syncthreads();
+    if (TMA && more) fetch_x(base - span, buf ^ 1);
     F qi = apply(Map<F>{sh.wmap[warp][lane].a, sh.wq[warp][lane]}, sh.carry[lane]);
     in = sh.wmap[warp][lane].H;
     // backwards over the tokens; the states before them are run forwards again, half of the
@@ -683,12 +683,17 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     for (int i = 0; i < kHalf; ++i) mid = step_<MODE>(ta[i], td[i], mid, Lane<T, V>::get(xw[i * 32]));
 #pragma unroll
     for (int half = 1; half >= 0; --half) {
-      F hb[kHalf];  // the state before each token
-      hb[0] = half ? mid : in;
+      // what q times is the gate's gradient: the state before the token, in sigmoid mode d (h - x),
+      // which single values form at the end (registers: 3 x 4000 x 777 bf16 99 -> 91 us)
+      constexpr bool kDiff = MODE == DP_SCAN_SIGMOID && V == 2;
+      F hb[kHalf], h = half ? mid : in;
 #pragma unroll
-      for (int i = 1; i < kHalf; ++i)
-        hb[i] = step_<MODE>(ta[half * kHalf + i - 1], td[half * kHalf + i - 1], hb[i - 1],
-                            Lane<T, V>::get(xw[(half * kHalf + i - 1) * 32]));
+      for (int k = 0; k < kHalf; ++k) {
+        const int i = half * kHalf + k;
+        const F xv = kDiff || k + 1 < kHalf ? Lane<T, V>::get(xw[i * 32]) : h;
+        hb[k] = kDiff ? mul_(td[i], fma_(xv, all_<F>(-1.f), h)) : h;
+        if (k + 1 < kHalf) h = step_<MODE>(ta[i], td[i], h, xv);
+      }
 #pragma unroll
       for (int k = kHalf - 1; k >= 0; --k) {
         const int i = half * kHalf + k;
@@ -697,7 +702,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
         F ox = p, og = mul_(qi, hb[k]);
         if constexpr (MODE == DP_SCAN_SIGMOID) {
           ox = mul_(p, td[i]);
-          og = mul_(mul_(qi, td[i]), fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k]));
+          if (!kDiff) og = mul_(mul_(qi, td[i]), fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k]));
         }
         if constexpr (TMA) {  // over the dout and the x that they took
           Lane<T, V>::store(reinterpret_cast<T *>(yw + i * 32), ox);
