@@ -702,7 +702,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
         F ox = p, og = mul_(qi, hb[k]);
         if constexpr (MODE == DP_SCAN_SIGMOID) {
           ox = mul_(p, td[i]);
-          if (!kDiff) og = mul_(mul_(qi, td[i]), fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k]));
+          if (!kDiff) og = mul_(qi, mul_(td[i], fma_(Lane<T, V>::get(xw[i * 32]), all_<F>(-1.f), hb[k])));
         }
         if constexpr (TMA) {  // over the dout and the x that they took
           Lane<T, V>::store(reinterpret_cast<T *>(yw + i * 32), ox);
