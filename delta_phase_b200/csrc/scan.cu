@@ -334,9 +334,16 @@ __device__ __forceinline__ void box_store(const CUtensorMap *m, const void *src,
 // after it has used those of the span before, so whoever has received the maps of span s may
 // send those of span s + 1 into the buffer of span s - 1.  No message is left when a block
 // ends: it has received all that is sent to it.
+//
+// Every wait has a limit (kWaitNs; a GPU that answers is far below it).  A thread whose wait ran out
+// arms no barrier, starts no copy, sends and stores nothing more: it goes through the remaining
+// spans without waits, so that the others pass their barriers; threads that wait for its messages
+// follow.  At the end (scan_end) it waits once more, with the same limit, for what it has in flight,
+// and the block until no block of the cluster can send to it any more; the error word is set.
 template <typename Shared>
 __device__ __forceinline__ void scan_start(Shared &sh, int cs) {
   if (threadIdx.x == 0) {
+    sh.expired = 0;
     mbar_init(&sh.bar[0], 1);
     mbar_init(&sh.bar[1], 1);
     for (int w = 0; w < kWarps; ++w) {
@@ -350,6 +357,26 @@ __device__ __forceinline__ void scan_start(Shared &sh, int cs) {
   else
     __syncthreads();
 }
+// After the loop, by all threads.
+template <bool TMA, typename Shared>
+__device__ __forceinline__ void scan_end(Shared &sh, bool alive, int cs, int *err) {
+  if (!alive) {
+    sh.expired = 1;
+    atomicCAS(err, 0, DP_ERR_TIMEOUT);
+    if (TMA)  // the phase in flight, if any, is one of the two; the other one's wait passes or runs out
+      for (int k = 0; k < 4; ++k)
+        mbar_wait_loop(k & 1 ? &sh.x_bar[threadIdx.x >> 5] : &sh.gate_bar[threadIdx.x >> 5], k >> 1, kWaitNs);
+  }
+  __syncthreads();
+  if (sh.expired && cs > 1) {
+    // blocks that ended well have left and do not count; the others come here, too, and what they
+    // sent before arrives within the time below
+    cg::this_cluster().sync();
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 1000000) __nanosleep(1000);
+  }
+}
+
 // a and d of a thread's tokens from the staged gates, and the factor of them all.  Tokens past the
 // end keep the state: their gates and x are staged as 0, which in decay mode is a = 1 already.
 template <typename T, int V, int MODE, typename F>
@@ -400,6 +427,7 @@ struct ScanShared {
   F carry[32];                              // the state (gradient) that reaches the block
   uint64_t bar[2];                          // one per buffer of bmap
   uint64_t gate_bar[kWarps], x_bar[kWarps];  // the warps' bulk copies
+  int expired;                               // a wait of the block ran out
 };
 template <typename F>
 struct ScanSharedBwd : ScanShared<F, 2> {
@@ -476,7 +504,7 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     const Product<T, MODE, F> product = load_gates<T, V, MODE>(gw, n, ta, td);
     if constexpr (TMA) {
       __syncwarp();  // every lane has its gates
-      if (more) fetch_gate(base + span);
+      if (more && alive) fetch_gate(base + span);
       if (alive) alive = mbar_wait(&sh.x_bar[warp], phase & 1, kWaitNs);
     } else if (more) {
       fetch_gate(base + span);
@@ -486,7 +514,7 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     product.get(own.a, sh.wn[warp][lane]);
     own.H = reduce_tokens<T, V, MODE, kKeep>(xw, ta, td);
     sh.wmap[warp][lane] = own;
-    if (TMA && more) fetch_x(base + span, buf ^ 1);
+    if (TMA && more && alive) fetch_x(base + span, buf ^ 1);
     __syncthreads();
     if (warp == kWarps - 1) {
       Map<F> r = {all_<F>(1.f), all_<F>(0.f)};
@@ -500,10 +528,12 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       r.a = marked(r.a, rn);
       F in = h;
       if (a.cs > 1) {
-        if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
-        for (int k = 0; k < a.cs; ++k)
-          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
-        if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
+        if (alive) {
+          if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
+          for (int k = 0; k < a.cs; ++k)
+            cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+          alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
+        }
 #pragma unroll 4
         for (int k = 0; k < a.cs; ++k) {
           if (k == rank) in = h;
@@ -531,14 +561,14 @@ scan_fwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     if constexpr (TMA) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && n > 0) {
+      if (lane == 0 && n > 0 && alive) {
         box_store(&maps.out, &sh.x[0][buf][warp][0][0], c0, (int)t0, b);
         bulk_commit_group();
       }
     }
   }
   if (TMA && lane == 0) bulk_wait_all();
-  if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
+  scan_end<TMA>(sh, alive, a.cs, a.err);
   if (on && rank == 0 && warp == kWarps - 1) store_state(a.hL + (int64_t)b * a.D + c, h);
 }
 
@@ -618,7 +648,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     const Product<T, MODE, F> product = load_gates<T, V, MODE>(gw, n, ta, td);
     if constexpr (TMA) {
       __syncwarp();  // every lane has its gates
-      if (more) fetch_gate(base - span);
+      if (more && alive) fetch_gate(base - span);
       if (alive) alive = mbar_wait(&sh.x_bar[warp], phase & 1, kWaitNs);
     } else if (more) {
       fetch_gate(base - span);
@@ -655,10 +685,12 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       r.a = marked(r.a, rn);
       F qin = q;
       if (a.cs > 1) {
-        if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
-        for (int k = 0; k < a.cs; ++k)
-          cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
-        if (alive) alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
+        if (alive) {
+          if (lane == 0) mbar_arrive_expect_tx(&sh.bar[buf], (uint32_t)(a.cs * sizeof(sh.bmap[0][0])));
+          for (int k = 0; k < a.cs; ++k)
+            cluster_send(peer_addr(&sh.bmap[buf][rank][lane], k), peer_addr(&sh.bar[buf], k), r.a, r.H);
+          alive = cluster_wait(&sh.bar[buf], phase >> 1 & 1);
+        }
 #pragma unroll 4
         for (int k = a.cs - 1; k >= 0; --k) {
           if (k == rank) qin = q;
@@ -670,7 +702,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
       sh.carry[lane] = qin;
     }
     __syncthreads();
-    if (TMA && more) fetch_x(base - span, buf ^ 1);
+    if (TMA && more && alive) fetch_x(base - span, buf ^ 1);
     F qi = apply(Map<F>{sh.wmap[warp][lane].a, sh.wq[warp][lane]}, sh.carry[lane]);
     in = sh.wmap[warp][lane].H;
     // backwards over the tokens; the states before them are run forwards again, half of the
@@ -716,7 +748,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     if constexpr (TMA) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && n > 0) {
+      if (lane == 0 && n > 0 && alive) {
         box_store(&maps.dx, &sh.x[1][buf][warp][0][0], c0, (int)t0, b);
         box_store(&maps.dgate, &sh.x[0][buf][warp][0][0], c0, (int)t0, b);
         bulk_commit_group();
@@ -724,7 +756,7 @@ scan_bwd_kernel(const ScanArgs a, const __grid_constant__ ScanMaps maps) {
     }
   }
   if (TMA && lane == 0) bulk_wait_all();
-  if (!alive && lane == 0) atomicCAS(a.err, 0, DP_ERR_TIMEOUT);
+  scan_end<TMA>(sh, alive, a.cs, a.err);
   if (on && rank == 0 && warp == 0 && a.dh0) store_state(a.dh0 + (int64_t)b * a.D + c, q);
 }
 

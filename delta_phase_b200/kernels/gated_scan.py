@@ -118,7 +118,9 @@ def gated_scan(x, gate, initial_state=None, gate_mode="decay"):
     throughout and the order of all sums depends on L alone.  A value that is not finite stays in
     its channel, from its token on (an infinite state may continue as NaN).  Differentiable once when autograd
     records and an input requires grad.  A backward pass that is captured into a CUDA graph
-    needs, as any in torch, leaves that no eager graph still refers to.
+    needs, as any in torch, leaves that no eager graph still refers to.  Like the other kernels whose
+    blocks wait for one another, these give a wait up after 2 s and report it through
+    ``_capi.device_error()``, not through this call; the results are not to be used then.
     """
     mode = _mode(gate_mode)
     _check_inputs(x, gate, 3, "(B, L, D)")

@@ -396,6 +396,8 @@ DP_API int dp_layernorm_bwd(const void *s, int s_dtype, const void *dy, int dy_d
  *   strides[6]   : {sb, st} of x, gate, out
  * The state is float32 throughout; the order of all sums is fixed by L.  0 <= L <= 2^30.
  * A state that has become infinite may continue as NaN.
+ * The kernels' waits end after 2 s each: the call has returned by then, its outputs are not to be
+ * used, and dp_device_error reports DP_ERR_TIMEOUT (dp_scan_bwd likewise).
  * Made for 0 <= a <= 1; larger a are computed too, but a product of a over 128 tokens that
  * overflows float32 may turn a zero state into NaN.  Token strides up to 2^28 elements.
  */
