@@ -19,15 +19,18 @@
 //
 // Measured (B200, K = 64, copy rate 6540 GB/s):
 //                          loss and gradient      loss alone      gradient from the sums
-//   16384 x 32768 bf16     387 us (85% of rate)   174 us (94%)    346 us (95%)
-//   2048 x 32768 bf16      59 us (70%)            33 us (62%)     50 us (83%)
-//   4096 x 32768 float32   210 us (78%)           88 us (93%)     164 us (100%)
+//   16384 x 32768 bf16     383 us (86% of rate)   176 us (93%)    347 us (95%)
+//   2048 x 32768 bf16      58 us (71%)            33 us (62%)     50 us (83%)
+//   4096 x 32768 float32   203 us (81%)           88 us (93%)     164 us (100%)
 //   4096 x 32767 bf16 (rows off the 16-byte grid)
-//                          113 us (72%)           56 us (73%)     96 us (86%)
-//   20000 x 8192 bf16      146 us (69%)           64 us (78%)     116 us (87%)
+//                          113 us (73%)           56 us (74%)     95 us (87%)
+//   20000 x 8192 bf16      144 us (70%)           66 us (76%)     116 us (87%)
+//   65536 x 1000 bf16, K = 16
+//                          82 us (49%)            50 us (40%)     60 us (67%)
 // The loss alone through the staged rows was 235 us (70%) and 140 us (59%) for the first and third,
 // their backward pass without sums 405 and 213 us; with the running sum rescaled for every new
-// maximum the loss was 192 and 98 us.
+// maximum the loss was 192 and 98 us (versions before this one).  What the loss sums over the
+// entries goes against the row's own maxima, after the exchange (1 to 3% of the loss alone).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -729,7 +732,8 @@ __global__ void __launch_bounds__(kDiLossThreads, 6) distill_loss_kernel(const D
 }
 
 // The gradient from the row's sums, as the loss left them: every value by itself.  A block
-// (WARP: a warp) takes one of the a.cs slices of a row.
+// (WARP: a warp) takes one of the a.cs slices of a row.  64 registers a thread, of which eight
+// vectors spill 8 to 48 bytes.
 template <typename T, int NV, bool WARP>
 __global__ void __launch_bounds__(WARP ? 32 * kDiWarpRows : kDiGradThreads, WARP ? 8 : 2)
 distill_grad_kernel(const DistillArgs a) {
@@ -884,8 +888,8 @@ int distill_launch(DistillArgs a, cudaStream_t st) {
   DP_REQUIRE((int64_t)a.cs * most >= nvec, DP_ERR_UNSUPPORTED, "dp_distill: V too large");
   // few rows: split each over more blocks, down to a vector per thread (one row of 131072
   // float32 logits: 16 blocks); enough rows to fill the GPU are split only as far as they must
-  // (16384 x 32768 bf16, loss and gradient: 1 / 2 / 4 blocks a row 498 / 558 / 591 us, measured
-  // on the version before this one)
+  // (loss and gradient at 1 / 2 / 4 / 8 blocks a row: 16384 x 32768 bf16 383 / 439 / 547 / 917 us, 2048
+  // rows 58 / 66 / 78 / 121; 16 or 200 rows, from the host, 18 to 22 us with any of them)
   while (a.cs < kDiMaxCluster && a.rows * a.cs < kDiSms && nvec / a.cs >= 2 * kDiMaxThreads) a.cs *= 2;
   const int per = (nvec + a.cs - 1) / a.cs;
   const int64_t blocks = a.rows * a.cs;

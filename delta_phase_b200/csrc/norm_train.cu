@@ -13,11 +13,15 @@
 //   backward: eight columns a thread, so that dw and db of a thread's columns stay in registers
 //             while its block walks over the rows; the next rows are loaded meanwhile.  Two
 //             resident blocks of 256 threads without spills beat three with (183 against 222 us
-//             below); 16-bit rows, half as large, go two at a time (90 against 132 us).
+//             below); 16-bit rows, half as large, go two at a time (90 against 132 us).  Spills are
+//             left where single 16-bit values are loaded (12 to 40 bytes a thread up to d = 1024) and
+//             from d = 4097 on, where a block of 1024 has 64 registers a thread (32 to 128 bytes).
 // Measured (B200, copy rate 6540 GB/s), forward and backward: 65536 x 1024 bf16 with the float32
-// residual 132 us (94% of the copy rate) and 183 us (90%), without 70 us (58%) and 90 us (69%);
-// 16384 x 2048 float32 with residual 91 us (91%) and 109 us (94%); 8192 x 4096 bf16 44 us (47%) and
-// 56 us (55%); 32768 x 1000 bf16 with residual 76 us (79%) and 100 us (80%).
+// residual 132 us (94% of the copy rate) and 183 us (90%), without 70 us (59%) and 89 us (69%);
+// 16384 x 2048 float32 with residual 88 us (93%) and 109 us (94%); 8192 x 4096 bf16 44 us (47%) and
+// 56 us (55%); 4096 x 8192 bf16 with residual 82 us (75%) and 122 us (67%); 32768 x 1000 bf16 with
+// residual 78 us (77%) and 99 us (81%).  Above d = 8192, single values and several passes over a row:
+// 2048 x 16384 bf16 475 us for both.
 #include <algorithm>
 #include <string>
 #include <type_traits>

@@ -27,15 +27,16 @@
 // else by cp.async of single words and plain stores.  No warp waits for another one's copies.
 //
 // HBM bounds it where enough channels and tokens run at once (about 1.7 blocks an SM), the chain
-// of spans (2.3 to 2.8 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
-// and backward: 2 x 32768 x 1024 bf16 84 us (73% of the copy rate) and 117 us (88%), 8 x 8192 x
-// 1024 bf16 in sigmoid mode 84 us (73%) and 129 us (79%), 4 x 8192 x 512 float32 39 us (78%) and
-// 66 us (78%), 1 x 65536 x 256 bf16 (4 chains) 74 us (21%) and 90 us (28%).  The first was 148 and
-// 190 us with a marked factor, and the selection that goes with it, for every token, and 93 and
-// 125 us with one for every warp.  Older versions of it: every warp combining the maps 97 and
-// 130 us against 88 and 123 by one (769 and 637 instructions a warp and span forward); single words
-// instead of boxes 144 and 216 us (address arithmetic: 1048 instructions), and with a cluster
-// barrier instead of messages 179 and 321 us (its fence).
+// of spans (2.3 to 2.9 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
+// and backward: 2 x 32768 x 1024 bf16 84 us (73% of the copy rate) and 121 us (85%), 8 x 8192 x
+// 1024 bf16 78 us (79%) and 116 us (88%), in sigmoid mode 86 us (71%) and 129 us (79%), 4 x 8192 x
+// 512 float32 39 us (78%) and 62 us (83%), 1 x 65536 x 256 bf16 (4 chains) 74 us (21%) and 92 us
+// (28%).  The first was 148 and 190 us with a marked factor, and the selection that goes with it,
+// for every token, and 93 and 125 us with one for every warp.  The backward pass fetches the next
+// span's x and gradient after the second barrier: before the first, loads and stores meet (8 x
+// 8192 x 1024 134 us, the first 117).  Older versions: every warp combining the maps 97 and 130 us
+// against 88 and 123 by one; single words instead of boxes 144 and 216 us (address arithmetic), and
+// with a cluster barrier instead of messages 179 and 321 us (its fence).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -436,8 +437,9 @@ struct ScanSharedBwd : ScanShared<F, 2> {
 
 // ---------------------------------------------------------------- forward
 // u in registers between the two passes: single values, and pairs in sigmoid mode, where it is d x
-// (two blocks an SM instead of three; the usual launch has 1.7).  Pairs in decay mode read x again:
-// three blocks an SM have no registers left for it.
+// (two blocks an SM instead of three: 8 x 8192 x 1024 bf16 84 us against 96 with a and d in one
+// marked word; 11 x 8192 x 512, 352 blocks, 75 against 68, as they no longer all run at once).  Pairs
+// in decay mode read x again: three blocks an SM have no registers left for it.
 template <int V, int MODE>
 constexpr bool kKeepU = V == 1 || MODE == DP_SCAN_SIGMOID;
 template <typename T, int V, int MODE, bool TMA>
@@ -786,9 +788,10 @@ scan_step_kernel(const float *state, float *state_out, const T *x, const T *gate
 // Blocks of a cluster.  Smaller clusters wait less for one another, but a sequence's chain of
 // spans has to be split until about 1.7 blocks an SM run; sizes that are no power of two pack
 // badly into the GPU's processor clusters.  Measured (us forward, backward at 2 / 4 / 8 / 9 / 16
-// blocks): 32 chains x 32768 tokens bf16 215, 289 / 113, 154 / 88, 123 / 115, 183 / 103, 164;
-// 128 chains x 8192 tokens bf16 86, 121 / 86, 128 / 96, 144 / 101, 156 / 105, 175 (the 9 and the
-// second 8 taken with every warp combining the maps).
+// blocks): 32 chains x 32768 tokens bf16 226, 289 / 119, 162 / 84, 121 / 93, 180 / 99, 170;
+// 128 chains x 8192 tokens bf16 78, 116 / 94, 123 / 83, 132 / 87, 146 / 103, 172, in sigmoid mode
+// 86, 129 / 91, 136 / 102, 148 / 113, 162 / 138, 191; 4 chains x 65536 tokens bf16 439, 557 / 228,
+// 292 / 125, 158 / 115, 144 / 74, 93.
 int scan_cluster(int L, int64_t chains) {
   int cs = 1;
   while (cs < kMaxCluster && cs * kTile < L && chains * cs < 256) cs *= 2;
