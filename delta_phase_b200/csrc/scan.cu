@@ -138,8 +138,8 @@ __device__ __forceinline__ float2 min_nan(float2 a, float b) { return make_float
 
 // a of a gate, and in sigmoid mode d, each within a few steps of its own value.  16-bit gates: the
 // hardware exponential and reciprocal (2^-22, and |gate| 2^-24 from the exponent's rounding):
-// f = exp(gate), d = 1 / (1 + f), a = f d; f ends at 2^125, where a is 1 and d 2^-125.  float32: the
-// library's functions.
+// f = exp(gate), d = 1 / (1 + f), a = f d; f ends at 2^125, where a is 1, and the 2^-125 that is d
+// there is taken from every d.  float32: the library's functions.
 template <typename T, int MODE, typename F>
 __device__ __forceinline__ void gate_(F g, F &a, F &d) {
   d = all_<F>(0.f);  // not used in decay mode
@@ -156,6 +156,7 @@ __device__ __forceinline__ void gate_(F g, F &a, F &d) {
       a = min_nan(a, 4.2535296e37f);
       d = rcp_(add_(a, all_<F>(1.f)));
       a = mul_(a, d);
+      d = add_(d, all_<F>(-2.3509887e-38f));
     }
   }
 }
@@ -424,7 +425,7 @@ struct ScanShared {
   uint32_t x[NX][2][kWarps][kTok][32];      // x, and dout in the backward pass
   Map<F> wmap[kWarps][32];                  // the warps' maps, then those of the warps before each
   F wn[kWarps][32];                         // their n
-  Map<F> bmap[2][kMaxCluster][32];   // the blocks' maps
+  Map<F> bmap[2][kMaxCluster][32];          // the blocks' maps
   F carry[32];                              // the state (gradient) that reaches the block
   uint64_t bar[2];                          // one per buffer of bmap
   uint64_t gate_bar[kWarps], x_bar[kWarps];  // the warps' bulk copies

@@ -201,7 +201,7 @@ class DeltaPhaseModel(nn.Module):
         if weight is None:
             weight = torch.full(input_ids.shape, 1.0 / max(1, input_ids.numel()), device=logits.device)
         if scaled:
-            weight = weight * loss_scale
+            weight = weight.to(torch.float32) * loss_scale
         loss, grad = distill_loss_and_grad(logits, teacher_index, teacher_logits, temperature, weight)
         logits.backward(grad)
         return loss.sum() / loss_scale if scaled else loss.sum()

@@ -102,6 +102,9 @@ def test_model_distill_step_keeps_float16_gradients_in_range(as_tensor, monkeypa
     # a sum of 2048 float32 losses: 64 roundings at most in a row, and the two products
     assert abs(float(loss) - float(rl.sum()) / scale) <= (float(el.sum()) + 70 * U * float(rl.abs().sum())) / scale
     assert abs(float(loss) - float(plain)) <= 140 * U * float(rl.abs().sum()) / scale + 2 * float(el.sum()) / scale
+    # a weight of fewer bits takes the scale in float32
+    mask = torch.ones(B, L, device="cuda", dtype=F16)
+    assert math.isfinite(float(model.distill_step(*args, weight=mask / (B * L), loss_scale=s)))
 
 
 # ---------------------------------------------------------------- gated recurrence, open gates
@@ -231,6 +234,21 @@ def test_scan_closed_gates_against_a_large_state(dtype, mode):
             o, h = gated_scan_step(h0, xs[:, at], gate[:, at], gate_mode=mode)
             check(o[0], want, 32 * U * want, (at, g))
             check(h[0], want, 32 * U * want, (at, g))
+
+
+@pytest.mark.parametrize("D", [64, 33])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("gate", [math.inf, 1000.0, 200.0])
+def test_scan_gates_that_let_nothing_in(gate, dtype, D):
+    """sigmoid = 1 in float32, and 1 - sigmoid below its range: the state stays, bit for bit, and x has
+    no part in it and no gradient."""
+    x = torch.linspace(-1e4, 1e4, 300 * D, device="cuda").view(1, 300, D).to(dtype).requires_grad_(True)
+    g = torch.full((1, 300, D), gate, device="cuda", dtype=dtype)
+    for h0 in (torch.zeros(1, D, device="cuda"), torch.linspace(-3, 3, D, device="cuda")[None]):
+        out, fin = gated_scan(x, g, h0, gate_mode="sigmoid")
+        assert torch.equal(fin, h0) and torch.equal(out, h0[:, None].expand(1, 300, D).to(dtype))
+        dx, = torch.autograd.grad((out, fin), x, (torch.ones_like(out), fin.detach()))
+        assert not dx.any()
 
 
 @pytest.mark.parametrize("mode", ["decay", "sigmoid"])
