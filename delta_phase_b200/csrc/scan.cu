@@ -29,7 +29,7 @@
 // HBM bounds it where enough channels and tokens run at once (about 1.7 blocks an SM), the chain
 // of spans (2.3 to 2.9 us each) where there are few.  Measured (B200, copy rate 6540 GB/s), forward
 // and backward: 2 x 32768 x 1024 bf16 84 us (73% of the copy rate) and 121 us (85%), 8 x 8192 x
-// 1024 bf16 78 us (79%) and 116 us (88%), in sigmoid mode 86 us (71%) and 129 us (79%), 4 x 8192 x
+// 1024 bf16 78 us (79%) and 116 us (88%), in sigmoid mode 86 us (71%) and 132 us (78%), 4 x 8192 x
 // 512 float32 39 us (78%) and 62 us (83%), 1 x 65536 x 256 bf16 (4 chains) 74 us (21%) and 92 us
 // (28%).  The first was 148 and 190 us with a marked factor, and the selection that goes with it,
 // for every token, and 93 and 125 us with one for every warp.  The backward pass fetches the next
@@ -791,7 +791,7 @@ scan_step_kernel(const float *state, float *state_out, const T *x, const T *gate
 // badly into the GPU's processor clusters.  Measured (us forward, backward at 2 / 4 / 8 / 9 / 16
 // blocks): 32 chains x 32768 tokens bf16 226, 289 / 119, 162 / 84, 121 / 93, 180 / 99, 170;
 // 128 chains x 8192 tokens bf16 78, 116 / 94, 123 / 83, 132 / 87, 146 / 103, 172, in sigmoid mode
-// 86, 129 / 91, 136 / 102, 148 / 113, 162 / 138, 191; 4 chains x 65536 tokens bf16 439, 557 / 228,
+// 86, 132 / 91, 136 / 102, 148 / 113, 162 / 138, 191; 4 chains x 65536 tokens bf16 439, 557 / 228,
 // 292 / 125, 158 / 115, 144 / 74, 93.
 int scan_cluster(int L, int64_t chains) {
   int cs = 1;
